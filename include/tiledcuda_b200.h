@@ -85,6 +85,65 @@ int64_t tc_gemm_host_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int tc_gemm_f16_f32_host(const void* hA, const void* hB, void* hC, int64_t M, int64_t N, int64_t K, void* d_workspace,
                          int64_t workspace_bytes, tc_stream_t stream);
 
+/* Element types of the entry points that take more than one. */
+enum tc_type { TC_F32 = 0, TC_F16 = 1, TC_BF16 = 4 };
+
+/* Rounds each row (token, or output channel of a weight) of x to 8-bit integers with one fp32 scale:
+ *   scale[r] = max(max_c |x[r,c]| / 127, 2^-126),   q[r,c] = x[r,c] / scale[r] rounded to nearest, ties to even,
+ * so that q[r,c] * scale[r] stands for x[r,c] and |q| <= 127. The quotient is rounded as the exact one would be (the
+ * division leaves no rounding of its own). A row of zeros gives zeros; a row with an infinity or NaN gives
+ * scale = inf or NaN and q = 0, so that what is computed from it is NaN. x is [rows, cols] of x_type (tc_type) with row
+ * stride ldx, q int8 with row stride ldq, scale fp32 [rows]; no alignment is asked for beyond that of the types.
+ * The reference has no 8-bit path; no counterpart there. */
+int tc_quantize_rows(const void* x, void* q, float* scale, int64_t rows, int64_t cols, int64_t ldx, int64_t ldq,
+                     int x_type, tc_stream_t stream);
+
+/* C[M,N] = scale_a[m] * scale_b[n] * sum_k A[m,k] B[n,k], A int8 [M,K] (lda), B int8 [N,K] (ldb, the column-major
+ * [K,N] of tc_gemm_f16_f32), scales fp32 [M] and [N] (one per token and per output channel), C of c_type (tc_type)
+ * with row stride ldc. The sum over K is exact (32-bit integers; K <= 131071, so that it cannot overflow for any
+ * 8-bit values), then (float(sum) * scale_a) * scale_b in fp32 is rounded once to c_type. M may be 0. Needs lda % 16 == 0,
+ * ldb % 16 == 0 and 16-byte aligned A and B; K and N may be any size. The reference is fp16-only
+ * (include/cell/compute/gemm.hpp:26-29); no counterpart there. */
+int tc_gemm_i8(const void* A, const void* B, const float* scale_a, const float* scale_b, void* C, int64_t M, int64_t N,
+               int64_t K, int64_t lda, int64_t ldb, int64_t ldc, int c_type, tc_stream_t stream);
+
+/* Matrix products grouped by expert. The rows of A are sorted by expert: expert e owns rows offsets[e] up to (not
+ * including) offsets[e+1], and  C[t,:] = A[t,:] B[e]^T  for its rows t. A [rows,K] (lda) and C [rows,N] (ldc) row-major,
+ * B [experts,N,K] with row stride ldb and expert stride stride_b (elements); A and B are of in_type (TC_F16 or TC_BF16),
+ * fp32 accumulation, C is rounded once to c_type (in_type or TC_F32). offsets is DEVICE memory, experts + 1 integers
+ * (int64 when offsets_are_int64 else int32), nondecreasing and within [0, rows]: the host never reads them, so sizes
+ * decided by a router on the device need no synchronisation. Empty experts are fine; rows before offsets[0] and from
+ * offsets[experts] on are not read into any result and their rows of C stay as they were. Offsets outside
+ * [0, rows] are clamped to it, a decreasing pair makes an empty expert, and either is reported through tc_device_status()
+ * (code 16). 1 <= experts <= 2048; rows may be 0. Needs lda, ldb, stride_b multiples of 16 bytes and 16-byte
+ * aligned A and B; N, K and ldc may be any size. One expert's products are the reference's `gemm`
+ * (examples/cpp/01_gemm/02_gemm_all_mem/gemm.hpp:92-155); the grouping has no counterpart there. */
+int tc_grouped_gemm(const void* A, const void* B, const void* offsets, int offsets_are_int64, void* C, int64_t rows,
+                    int64_t experts, int64_t N, int64_t K, int64_t lda, int64_t ldb, int64_t stride_b, int64_t ldc,
+                    int in_type, int c_type, tc_stream_t stream);
+
+/* tc_grouped_gemm on 8-bit integers: C[t,n] = scale_a[t] * scale_b[e,n] * sum_k A[t,k] B[e,n,k], arithmetic and types of
+ * C as tc_gemm_i8, rows and offsets as tc_grouped_gemm; scale_a fp32 [rows], scale_b fp32 [experts,N] contiguous.
+ * Needs lda, ldb and stride_b multiples of 16. It has no counterpart in the reference. */
+int tc_grouped_gemm_i8(const void* A, const void* B, const float* scale_a, const float* scale_b, const void* offsets,
+                       int offsets_are_int64, void* C, int64_t rows, int64_t experts, int64_t N, int64_t K, int64_t lda,
+                       int64_t ldb, int64_t stride_b, int64_t ldc, int c_type, tc_stream_t stream);
+
+/* Gradient of tc_grouped_gemm to A: dA[t,:] = dC[t,:] B[e] for the rows t of expert e. dC [rows,N] (lddc), dA [rows,K]
+ * (ldda); everything else, the rows outside all groups included, as there. Needs lddc, ldb, stride_b multiples of 16
+ * bytes. The reference has no backward pass; no counterpart there. */
+int tc_grouped_gemm_dgrad(const void* dC, const void* B, const void* offsets, int offsets_are_int64, void* dA,
+                          int64_t rows, int64_t experts, int64_t N, int64_t K, int64_t lddc, int64_t ldb,
+                          int64_t stride_b, int64_t ldda, int in_type, int da_type, tc_stream_t stream);
+
+/* Gradient of tc_grouped_gemm to B: dB[e] = sum over the rows t of expert e of dC[t,:]^T A[t,:], the whole of dB
+ * [experts,N,K] (row stride lddb, expert stride stride_db): an expert without rows gets zeros. Rows outside all groups
+ * take no part, whatever they hold. The sum runs over the rows in order, so the result does not change from run to run.
+ * Needs lddc and lda multiples of 16 bytes. The reference has no backward pass; no counterpart there. */
+int tc_grouped_gemm_wgrad(const void* dC, const void* A, const void* offsets, int offsets_are_int64, void* dB,
+                          int64_t rows, int64_t experts, int64_t N, int64_t K, int64_t lddc, int64_t lda, int64_t lddb,
+                          int64_t stride_db, int in_type, int db_type, tc_stream_t stream);
+
 /* E[b] (fp32 [M,P]) = fp16(A[b] * B[b]) * D[b] for b in [0,batch): A fp16 [M,K] row-major; B
  * column-major [K,N] stored as [N,K]; D column-major [N,P] stored as [P,N]. The intermediate A*B is
  * accumulated in fp32, rounded to fp16 and never leaves the chip.

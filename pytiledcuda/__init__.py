@@ -13,7 +13,13 @@ from tiledcuda_b200.pytiledcuda import (  # noqa: F401
     flash_attn,
     flash_attn_ex,
     gemm,
+    gemm_i8,
+    grouped_gemm,
+    grouped_gemm_dgrad,
+    grouped_gemm_i8,
+    grouped_gemm_wgrad,
     lstm_cell,
+    quantize_rows,
     scatter_nd,
     scatter_nd_add,
 )
@@ -25,7 +31,13 @@ __all__ = [
     "flash_attn",
     "flash_attn_ex",
     "gemm",
+    "gemm_i8",
+    "grouped_gemm",
+    "grouped_gemm_dgrad",
+    "grouped_gemm_i8",
+    "grouped_gemm_wgrad",
     "lstm_cell",
+    "quantize_rows",
     "scatter_nd",
     "scatter_nd_add",
 ]

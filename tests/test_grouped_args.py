@@ -1,0 +1,94 @@
+"""CPU tests of the argument checks of the scaled 8-bit and the expert-grouped products: every refusal is a status and a
+message before anything touches CUDA. Addresses are made up and never dereferenced."""
+import pytest
+import torch
+
+from tiledcuda_b200 import _lib, ops
+
+F32, F16, I32, BF16 = 0, 1, 2, 4
+BAD, UNSUPPORTED = -1, -2
+
+
+def quantize(l, x=64, q=64, s=64, rows=4, cols=8, ldx=8, ldq=8, ty=F16):
+    return l.tc_quantize_rows(x, q, s, rows, cols, ldx, ldq, ty, None)
+
+
+def i8(l, a=64, b=64, sa=64, sb=64, c=64, m=4, n=8, k=32, lda=32, ldb=32, ldc=8, ty=F16):
+    return l.tc_gemm_i8(a, b, sa, sb, c, m, n, k, lda, ldb, ldc, ty, None)
+
+
+def grouped(l, a=64, b=64, off=64, wide=0, c=64, rows=4, e=2, n=8, k=32, lda=32, ldb=32, sb=256, ldc=8, it=F16, ct=F16):
+    return l.tc_grouped_gemm(a, b, off, wide, c, rows, e, n, k, lda, ldb, sb, ldc, it, ct, None)
+
+
+def grouped_i8(l, a=64, b=64, sa=64, sb=64, off=64, wide=0, c=64, rows=4, e=2, n=8, k=32, lda=32, ldb=32, stride=256, ldc=8, ct=F16):
+    return l.tc_grouped_gemm_i8(a, b, sa, sb, off, wide, c, rows, e, n, k, lda, ldb, stride, ldc, ct, None)
+
+
+def dgrad(l, dc=64, b=64, off=64, wide=0, da=64, rows=4, e=2, n=8, k=32, lddc=8, ldb=32, sb=256, ldda=32, it=F16, ot=F16):
+    return l.tc_grouped_gemm_dgrad(dc, b, off, wide, da, rows, e, n, k, lddc, ldb, sb, ldda, it, ot, None)
+
+
+def wgrad(l, dc=64, a=64, off=64, wide=0, db=64, rows=4, e=2, n=8, k=32, lddc=8, lda=32, lddb=32, sdb=256, it=F16, ot=F16):
+    return l.tc_grouped_gemm_wgrad(dc, a, off, wide, db, rows, e, n, k, lddc, lda, lddb, sdb, it, ot, None)
+
+
+CASES = [
+    (quantize, dict(x=None), BAD, "null"), (quantize, dict(s=None), BAD, "null"), (quantize, dict(cols=0), BAD, "positive"),
+    (quantize, dict(rows=-1), BAD, "negative"), (quantize, dict(rows=1 << 31), BAD, "31 bits"), (quantize, dict(ldx=7), BAD, "leading dimension"),
+    (quantize, dict(ldq=7), BAD, "leading dimension"), (quantize, dict(ty=I32), BAD, "x_type"), (quantize, dict(x=65), BAD, "aligned"),
+    (i8, dict(a=None), BAD, "null"), (i8, dict(sa=None), BAD, "null"), (i8, dict(c=None), BAD, "null"), (i8, dict(m=-1), BAD, "negative"),
+    (i8, dict(n=0), BAD, "positive"), (i8, dict(k=0), BAD, "positive"), (i8, dict(lda=40), BAD, "row stride"), (i8, dict(ldb=24), BAD, "leading dimension"),
+    (i8, dict(ldc=7), BAD, "leading dimension"), (i8, dict(a=72), BAD, "aligned"), (i8, dict(c=65), BAD, "aligned"), (i8, dict(sb=66), BAD, "aligned"),
+    (i8, dict(ty=I32), BAD, "c_type"), (i8, dict(k=131072, lda=131072, ldb=131072), UNSUPPORTED, "overflow"), (i8, dict(n=1 << 31), BAD, "31 bits"),
+    (i8, dict(lda=1 << 40), BAD, "too large"),
+    (grouped, dict(off=None), BAD, "offsets"), (grouped, dict(off=66), BAD, "aligned"), (grouped, dict(off=68, wide=1), BAD, "aligned"),
+    (grouped, dict(e=0), BAD, "positive"), (grouped, dict(e=2049), UNSUPPORTED, "2048"), (grouped, dict(rows=-1), BAD, "negative"),
+    (grouped, dict(lda=36), BAD, "row stride"), (grouped, dict(ldb=36), BAD, "row stride"), (grouped, dict(sb=260), BAD, "expert stride"),
+    (grouped, dict(sb=16), BAD, "expert stride"), (grouped, dict(sb=0), BAD, "expert stride"), (grouped, dict(it=F32, ct=F32), BAD, "in_type"), (grouped, dict(ct=BF16), BAD, "input's type"),
+    (grouped, dict(b=72), BAD, "aligned"), (grouped, dict(ldc=0), BAD, "leading dimension"), (grouped, dict(sb=1 << 40), BAD, "too large"),
+    (grouped_i8, dict(off=None), BAD, "offsets"), (grouped_i8, dict(stride=264), BAD, "expert stride"), (grouped_i8, dict(lda=40), BAD, "row stride"),
+    (grouped_i8, dict(k=1 << 18, lda=1 << 18, ldb=1 << 18, stride=1 << 21), UNSUPPORTED, "overflow"), (grouped_i8, dict(sa=None), BAD, "null"),
+    (dgrad, dict(lddc=12), BAD, "row stride"), (dgrad, dict(ldda=31), BAD, "leading dimension"), (dgrad, dict(dc=None), BAD, "null"),
+    (dgrad, dict(ot=BF16), BAD, "input's type"), (dgrad, dict(e=2049), UNSUPPORTED, "2048"), (dgrad, dict(off=None), BAD, "offsets"),
+    (wgrad, dict(lddc=12), BAD, "row stride"), (wgrad, dict(lda=36), BAD, "row stride"), (wgrad, dict(db=None), BAD, "null"), (wgrad, dict(db=None, rows=0), BAD, "null"),
+    (wgrad, dict(lddb=31), BAD, "leading dimension"), (wgrad, dict(sdb=8), BAD, "expert stride"), (wgrad, dict(it=I32, ot=I32), BAD, "in_type"),
+    (wgrad, dict(off=None), BAD, "offsets"),
+]
+
+
+@pytest.mark.parametrize("call,change,status,needle", CASES)
+def test_refusals(call, change, status, needle):
+    lib = _lib.load()
+    assert call(lib, **change) == status
+    assert needle in lib.tc_last_error().decode()
+
+
+def test_no_rows_is_no_work():
+    lib = _lib.load()
+    assert quantize(lib, x=None, q=None, s=None, rows=0) == 0
+    assert i8(lib, a=None, c=None, sa=None, m=0) == 0
+    assert grouped(lib, a=None, c=None, rows=0) == 0
+    assert grouped_i8(lib, a=None, c=None, sa=None, rows=0) == 0
+    assert dgrad(lib, dc=None, da=None, rows=0) == 0
+
+
+def test_python_route_refuses_cpu_tensors_and_wrong_types():
+    a, b, c = torch.zeros(4, 16, dtype=torch.float16), torch.zeros(2, 8, 16, dtype=torch.float16), torch.zeros(4, 8, dtype=torch.float16)
+    off = torch.tensor([0, 2, 4], dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.grouped_gemm(a, b, off, c)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.grouped_gemm_dgrad(c, b, off, a)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.grouped_gemm_wgrad(c, a, off, b)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.quantize_rows(a, a.to(torch.int8), torch.zeros(4))
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.gemm_i8(a.to(torch.int8), b[0].to(torch.int8), torch.zeros(4), torch.zeros(8), c)
+    with pytest.raises(ValueError, match="3-D"):
+        ops.grouped_gemm(a, b[0], off, c)
+    with pytest.raises(TypeError):
+        ops.grouped_gemm(None, b, off, c)
+    with pytest.raises(TypeError):
+        ops.quantize_rows([1.0], None, None)

@@ -26,6 +26,24 @@ SIGNATURES = {
     "tc_gemm_tile_plan": (ctypes.c_int, [c_i64, c_i64, c_i64, ctypes.c_int]),
     "tc_gemm_host_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64]),
     "tc_gemm_f16_f32_host": (ctypes.c_int, [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp]),
+    "tc_quantize_rows": (ctypes.c_int, [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, ctypes.c_int, c_vp]),
+    "tc_gemm_i8": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, ctypes.c_int, c_vp]),
+    "tc_grouped_gemm": (
+        ctypes.c_int,
+        [c_vp, c_vp, c_vp, ctypes.c_int, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, ctypes.c_int, ctypes.c_int, c_vp],
+    ),
+    "tc_grouped_gemm_i8": (
+        ctypes.c_int,
+        [c_vp, c_vp, c_vp, c_vp, c_vp, ctypes.c_int, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, ctypes.c_int, c_vp],
+    ),
+    "tc_grouped_gemm_dgrad": (
+        ctypes.c_int,
+        [c_vp, c_vp, c_vp, ctypes.c_int, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, ctypes.c_int, ctypes.c_int, c_vp],
+    ),
+    "tc_grouped_gemm_wgrad": (
+        ctypes.c_int,
+        [c_vp, c_vp, c_vp, ctypes.c_int, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, ctypes.c_int, ctypes.c_int, c_vp],
+    ),
     "tc_b2b_gemm_f16": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp]),
     "tc_flash_attn_fwd_f16": (
         ctypes.c_int,

@@ -9,6 +9,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <initializer_list>
 #include <vector>
 
@@ -206,6 +207,120 @@ void lstm_cell_op(const at::Tensor& W, const at::Tensor& U, const c10::optional<
                                         h_out.data_ptr(), c_out.data_ptr<float>(), batch, input, hidden, stream_of(x)));
 }
 
+// ---- scaled 8-bit and expert-grouped products -------------------------------------------------------------------
+int type_code(const at::Tensor& t) {
+    return t.scalar_type() == at::kFloat ? TC_F32 : t.scalar_type() == at::kHalf ? TC_F16 : TC_BF16;
+}
+bool is_half(const at::Tensor& t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; }
+
+// A CUDA tensor of this shape whose last dimension is dense; other strides are the caller's.
+void need_rows(const char* op, const char* name, const at::Tensor& t, at::IntArrayRef shape, bool type_ok) {
+    TORCH_CHECK(t.is_cuda(), op, ": ", name, " must be a CUDA tensor");
+    TORCH_CHECK(type_ok, op, ": ", name, " may not be ", t.scalar_type());
+    TORCH_CHECK(t.sizes() == shape, op, ": ", name, " must be ", shape, ", got ", t.sizes());
+    TORCH_CHECK(t.size(-1) <= 1 || t.stride(-1) == 1, op, ": ", name, " must have unit inner stride");
+}
+
+// Stride of a dimension; that of a dimension of one element is never stepped over and may be anything, so it is
+// replaced by the dense one, rounded up to what the kernels' loads are granular in.
+int64_t ld(const at::Tensor& t, int64_t dim, int64_t granule = 1) {
+    if (t.size(dim) > 1) return t.stride(dim);
+    const int64_t inner = dim + 2 == t.dim() ? t.size(dim + 1) : t.size(dim + 1) * ld(t, dim + 1, granule);
+    return (std::max<int64_t>(1, inner) + granule - 1) / granule * granule;
+}
+
+int wide_offsets(const char* op, const at::Tensor& offsets, int64_t experts) {
+    need_rows(op, "offsets", offsets, {experts + 1}, offsets.scalar_type() == at::kInt || offsets.scalar_type() == at::kLong);
+    return offsets.scalar_type() == at::kLong ? 1 : 0;
+}
+
+void quantize_rows_op(const at::Tensor& x, at::Tensor& q, at::Tensor& scale) {
+    const char* op = "quantize_rows";
+    TORCH_CHECK(x.dim() == 2, op, ": x must be 2-D");
+    need_rows(op, "x", x, x.sizes(), x.scalar_type() == at::kFloat || is_half(x));
+    need_rows(op, "q", q, x.sizes(), q.scalar_type() == at::kChar);
+    need_rows(op, "scale", scale, {x.size(0)}, scale.scalar_type() == at::kFloat);
+    same_device(op, x, {&q, &scale});
+    c10::cuda::CUDAGuard guard(x.device());
+    check(op, tc_quantize_rows(x.data_ptr(), q.data_ptr(), scale.data_ptr<float>(), x.size(0), x.size(1), ld(x, 0), ld(q, 0), type_code(x),
+                               stream_of(x)));
+}
+
+void gemm_i8_op(const at::Tensor& A, const at::Tensor& B, const at::Tensor& scale_a, const at::Tensor& scale_b, at::Tensor& C) {
+    const char* op = "gemm_i8";
+    TORCH_CHECK(A.dim() == 2 && B.dim() == 2, op, ": A and B must be 2-D");
+    const int64_t m = A.size(0), k = A.size(1), n = B.size(0);
+    need_rows(op, "A", A, {m, k}, A.scalar_type() == at::kChar);
+    need_rows(op, "B", B, {n, k}, B.scalar_type() == at::kChar);
+    need_rows(op, "scale_a", scale_a, {m}, scale_a.scalar_type() == at::kFloat);
+    need_rows(op, "scale_b", scale_b, {n}, scale_b.scalar_type() == at::kFloat);
+    need_rows(op, "C", C, {m, n}, C.scalar_type() == at::kFloat || is_half(C));
+    same_device(op, A, {&B, &scale_a, &scale_b, &C});
+    c10::cuda::CUDAGuard guard(A.device());
+    check(op, tc_gemm_i8(A.data_ptr(), B.data_ptr(), scale_a.data_ptr<float>(), scale_b.data_ptr<float>(), C.data_ptr(), m, n, k, ld(A, 0, 16),
+                         ld(B, 0, 16), ld(C, 0), type_code(C), stream_of(A)));
+}
+
+void grouped_gemm_op(const at::Tensor& A, const at::Tensor& B, const at::Tensor& offsets, at::Tensor& C) {
+    const char* op = "grouped_gemm";
+    TORCH_CHECK(A.dim() == 2 && B.dim() == 3, op, ": A must be 2-D and B 3-D");
+    const int64_t t = A.size(0), k = A.size(1), e = B.size(0), n = B.size(1);
+    need_rows(op, "A", A, {t, k}, is_half(A));
+    need_rows(op, "B", B, {e, n, k}, B.scalar_type() == A.scalar_type());
+    need_rows(op, "C", C, {t, n}, C.scalar_type() == A.scalar_type() || C.scalar_type() == at::kFloat);
+    const int wide = wide_offsets(op, offsets, e);
+    same_device(op, A, {&B, &offsets, &C});
+    c10::cuda::CUDAGuard guard(A.device());
+    check(op, tc_grouped_gemm(A.data_ptr(), B.data_ptr(), offsets.data_ptr(), wide, C.data_ptr(), t, e, n, k, ld(A, 0, 8), ld(B, 1, 8),
+                              ld(B, 0, 8), ld(C, 0), type_code(A), type_code(C), stream_of(A)));
+}
+
+void grouped_gemm_i8_op(const at::Tensor& A, const at::Tensor& B, const at::Tensor& scale_a, const at::Tensor& scale_b,
+                        const at::Tensor& offsets, at::Tensor& C) {
+    const char* op = "grouped_gemm_i8";
+    TORCH_CHECK(A.dim() == 2 && B.dim() == 3, op, ": A must be 2-D and B 3-D");
+    const int64_t t = A.size(0), k = A.size(1), e = B.size(0), n = B.size(1);
+    need_rows(op, "A", A, {t, k}, A.scalar_type() == at::kChar);
+    need_rows(op, "B", B, {e, n, k}, B.scalar_type() == at::kChar);
+    need_rows(op, "scale_a", scale_a, {t}, scale_a.scalar_type() == at::kFloat);
+    need_rows(op, "scale_b", scale_b, {e, n}, scale_b.scalar_type() == at::kFloat);
+    TORCH_CHECK(scale_b.is_contiguous(), op, ": scale_b must be contiguous");
+    need_rows(op, "C", C, {t, n}, C.scalar_type() == at::kFloat || is_half(C));
+    const int wide = wide_offsets(op, offsets, e);
+    same_device(op, A, {&B, &scale_a, &scale_b, &offsets, &C});
+    c10::cuda::CUDAGuard guard(A.device());
+    check(op, tc_grouped_gemm_i8(A.data_ptr(), B.data_ptr(), scale_a.data_ptr<float>(), scale_b.data_ptr<float>(), offsets.data_ptr(), wide,
+                                 C.data_ptr(), t, e, n, k, ld(A, 0, 16), ld(B, 1, 16), ld(B, 0, 16), ld(C, 0), type_code(C), stream_of(A)));
+}
+
+void grouped_gemm_dgrad_op(const at::Tensor& dC, const at::Tensor& B, const at::Tensor& offsets, at::Tensor& dA) {
+    const char* op = "grouped_gemm_dgrad";
+    TORCH_CHECK(dC.dim() == 2 && B.dim() == 3, op, ": dC must be 2-D and B 3-D");
+    const int64_t t = dC.size(0), n = dC.size(1), e = B.size(0), k = B.size(2);
+    need_rows(op, "dC", dC, {t, n}, is_half(dC));
+    need_rows(op, "B", B, {e, n, k}, B.scalar_type() == dC.scalar_type());
+    need_rows(op, "dA", dA, {t, k}, dA.scalar_type() == dC.scalar_type() || dA.scalar_type() == at::kFloat);
+    const int wide = wide_offsets(op, offsets, e);
+    same_device(op, dC, {&B, &offsets, &dA});
+    c10::cuda::CUDAGuard guard(dC.device());
+    check(op, tc_grouped_gemm_dgrad(dC.data_ptr(), B.data_ptr(), offsets.data_ptr(), wide, dA.data_ptr(), t, e, n, k, ld(dC, 0, 8), ld(B, 1, 8),
+                                    ld(B, 0, 8), ld(dA, 0), type_code(dC), type_code(dA), stream_of(dC)));
+}
+
+void grouped_gemm_wgrad_op(const at::Tensor& dC, const at::Tensor& A, const at::Tensor& offsets, at::Tensor& dB) {
+    const char* op = "grouped_gemm_wgrad";
+    TORCH_CHECK(dC.dim() == 2 && A.dim() == 2 && dB.dim() == 3, op, ": dC and A must be 2-D and dB 3-D");
+    const int64_t t = dC.size(0), n = dC.size(1), e = dB.size(0), k = A.size(1);
+    need_rows(op, "dC", dC, {t, n}, is_half(dC));
+    need_rows(op, "A", A, {t, k}, A.scalar_type() == dC.scalar_type());
+    need_rows(op, "dB", dB, {e, n, k}, dB.scalar_type() == dC.scalar_type() || dB.scalar_type() == at::kFloat);
+    const int wide = wide_offsets(op, offsets, e);
+    same_device(op, dC, {&A, &offsets, &dB});
+    c10::cuda::CUDAGuard guard(dC.device());
+    check(op, tc_grouped_gemm_wgrad(dC.data_ptr(), A.data_ptr(), offsets.data_ptr(), wide, dB.data_ptr(), t, e, n, k, ld(dC, 0, 8), ld(A, 0, 8),
+                                    ld(dB, 1), ld(dB, 0), type_code(dC), type_code(dB), stream_of(dC)));
+}
+
 }  // namespace
 
 TORCH_LIBRARY(tiledcuda, m) {
@@ -218,6 +333,12 @@ TORCH_LIBRARY(tiledcuda, m) {
     m.def("back2back_gemm(Tensor A, Tensor B, Tensor D, Tensor(a!) E) -> ()");
     m.def("lstm_cell(Tensor W, Tensor U, Tensor? bias, Tensor x, Tensor h_prev, Tensor c_prev, Tensor(a!) h_out, "
           "Tensor(b!) c_out) -> ()");
+    m.def("quantize_rows(Tensor x, Tensor(a!) q, Tensor(b!) scale) -> ()");
+    m.def("gemm_i8(Tensor A, Tensor B, Tensor scale_a, Tensor scale_b, Tensor(a!) C) -> ()");
+    m.def("grouped_gemm(Tensor A, Tensor B, Tensor offsets, Tensor(a!) C) -> ()");
+    m.def("grouped_gemm_i8(Tensor A, Tensor B, Tensor scale_a, Tensor scale_b, Tensor offsets, Tensor(a!) C) -> ()");
+    m.def("grouped_gemm_dgrad(Tensor dC, Tensor B, Tensor offsets, Tensor(a!) dA) -> ()");
+    m.def("grouped_gemm_wgrad(Tensor dC, Tensor A, Tensor offsets, Tensor(a!) dB) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(tiledcuda, CUDA, m) {
@@ -229,4 +350,10 @@ TORCH_LIBRARY_IMPL(tiledcuda, CUDA, m) {
     m.impl("gemm", &gemm_op);
     m.impl("back2back_gemm", &back2back_gemm_op);
     m.impl("lstm_cell", &lstm_cell_op);
+    m.impl("quantize_rows", &quantize_rows_op);
+    m.impl("gemm_i8", &gemm_i8_op);
+    m.impl("grouped_gemm", &grouped_gemm_op);
+    m.impl("grouped_gemm_i8", &grouped_gemm_i8_op);
+    m.impl("grouped_gemm_dgrad", &grouped_gemm_dgrad_op);
+    m.impl("grouped_gemm_wgrad", &grouped_gemm_wgrad_op);
 }

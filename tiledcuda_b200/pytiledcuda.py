@@ -62,6 +62,36 @@ def lstm_cell(W, U, bias, x, h_prev, c_prev, h_out, c_out):
     torch.ops.tiledcuda.lstm_cell(W, U, bias, x, h_prev, c_prev, h_out, c_out)
 
 
+def quantize_rows(x, q, scale):
+    """Rows of x to 8-bit integers with one fp32 scale per row."""
+    torch.ops.tiledcuda.quantize_rows(x, q, scale)
+
+
+def gemm_i8(A, B, scale_a, scale_b, C):
+    """C = (A @ B.T) * scale_a[:, None] * scale_b[None, :] on 8-bit integers A [M, K], B [N, K]."""
+    torch.ops.tiledcuda.gemm_i8(A, B, scale_a, scale_b, C)
+
+
+def grouped_gemm(A, B, offsets, C):
+    """C[t] = A[t] @ B[e].T for the rows offsets[e] <= t < offsets[e + 1] of expert e."""
+    torch.ops.tiledcuda.grouped_gemm(A, B, offsets, C)
+
+
+def grouped_gemm_i8(A, B, scale_a, scale_b, offsets, C):
+    """grouped_gemm on 8-bit integers with scales scale_a [T] and scale_b [E, N]."""
+    torch.ops.tiledcuda.grouped_gemm_i8(A, B, scale_a, scale_b, offsets, C)
+
+
+def grouped_gemm_dgrad(dC, B, offsets, dA):
+    """Gradient of grouped_gemm to A."""
+    torch.ops.tiledcuda.grouped_gemm_dgrad(dC, B, offsets, dA)
+
+
+def grouped_gemm_wgrad(dC, A, offsets, dB):
+    """Gradient of grouped_gemm to B."""
+    torch.ops.tiledcuda.grouped_gemm_wgrad(dC, A, offsets, dB)
+
+
 class TiledFlashAttention:
     """query [m,k], key [k,n] (already K^T, as the reference test passes it), value [n,p]; one head, no scale."""
 
