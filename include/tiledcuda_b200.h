@@ -115,7 +115,7 @@ int tc_gemm_i8(const void* A, const void* B, const float* scale_a, const float* 
  * decided by a router on the device need no synchronisation. Empty experts are fine; rows before offsets[0] and from
  * offsets[experts] on are not read into any result and their rows of C stay as they were. Offsets outside
  * [0, rows] are clamped to it, a decreasing pair makes an empty expert, and either is reported through tc_device_status()
- * (code 16). 1 <= experts <= 2048; rows may be 0. Needs lda, ldb, stride_b multiples of 16 bytes and 16-byte
+ * (code 16). 1 <= experts <= 1024; rows may be 0. Needs lda, ldb, stride_b multiples of 16 bytes and 16-byte
  * aligned A and B; N, K and ldc may be any size. One expert's products are the reference's `gemm`
  * (examples/cpp/01_gemm/02_gemm_all_mem/gemm.hpp:92-155); the grouping has no counterpart there. */
 int tc_grouped_gemm(const void* A, const void* B, const void* offsets, int offsets_are_int64, void* C, int64_t rows,

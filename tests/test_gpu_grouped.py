@@ -379,7 +379,7 @@ def test_grouped_no_rows(cuda_ops, clean_status):
                              torch.ones(3, 24, device=DEV), off, torch.empty(0, 24, device=DEV))
 
 
-@pytest.mark.parametrize("experts", [1, 33, 1000, 2048])
+@pytest.mark.parametrize("experts", [1, 33, 1000, 1024])
 def test_many_experts_most_of_them_empty(cuda_ops, clean_status, experts):
     sizes = [(3 * e + 1) % 7 if e % 17 == 0 else 0 for e in range(experts)]
     n, k, total = 48, 40, sum(sizes)

@@ -43,14 +43,14 @@ CASES = [
     (i8, dict(ty=I32), BAD, "c_type"), (i8, dict(k=131072, lda=131072, ldb=131072), UNSUPPORTED, "overflow"), (i8, dict(n=1 << 31), BAD, "31 bits"),
     (i8, dict(lda=1 << 40), BAD, "too large"),
     (grouped, dict(off=None), BAD, "offsets"), (grouped, dict(off=66), BAD, "aligned"), (grouped, dict(off=68, wide=1), BAD, "aligned"),
-    (grouped, dict(e=0), BAD, "positive"), (grouped, dict(e=2049), UNSUPPORTED, "2048"), (grouped, dict(rows=-1), BAD, "negative"),
+    (grouped, dict(e=0), BAD, "positive"), (grouped, dict(e=1025), UNSUPPORTED, "1024"), (grouped, dict(rows=-1), BAD, "negative"),
     (grouped, dict(lda=36), BAD, "row stride"), (grouped, dict(ldb=36), BAD, "row stride"), (grouped, dict(sb=260), BAD, "expert stride"),
     (grouped, dict(sb=16), BAD, "expert stride"), (grouped, dict(sb=0), BAD, "expert stride"), (grouped, dict(it=F32, ct=F32), BAD, "in_type"), (grouped, dict(ct=BF16), BAD, "input's type"),
     (grouped, dict(b=72), BAD, "aligned"), (grouped, dict(ldc=0), BAD, "leading dimension"), (grouped, dict(sb=1 << 40), BAD, "too large"),
     (grouped_i8, dict(off=None), BAD, "offsets"), (grouped_i8, dict(stride=264), BAD, "expert stride"), (grouped_i8, dict(lda=40), BAD, "row stride"),
     (grouped_i8, dict(k=1 << 18, lda=1 << 18, ldb=1 << 18, stride=1 << 21), UNSUPPORTED, "overflow"), (grouped_i8, dict(sa=None), BAD, "null"),
     (dgrad, dict(lddc=12), BAD, "row stride"), (dgrad, dict(ldda=31), BAD, "leading dimension"), (dgrad, dict(dc=None), BAD, "null"),
-    (dgrad, dict(ot=BF16), BAD, "input's type"), (dgrad, dict(e=2049), UNSUPPORTED, "2048"), (dgrad, dict(off=None), BAD, "offsets"),
+    (dgrad, dict(ot=BF16), BAD, "input's type"), (dgrad, dict(e=1025), UNSUPPORTED, "1024"), (dgrad, dict(off=None), BAD, "offsets"),
     (wgrad, dict(lddc=12), BAD, "row stride"), (wgrad, dict(lda=36), BAD, "row stride"), (wgrad, dict(db=None), BAD, "null"), (wgrad, dict(db=None, rows=0), BAD, "null"),
     (wgrad, dict(lddb=31), BAD, "leading dimension"), (wgrad, dict(sdb=8), BAD, "expert stride"), (wgrad, dict(it=I32, ot=I32), BAD, "in_type"),
     (wgrad, dict(off=None), BAD, "offsets"),

@@ -1,101 +1,8 @@
-// Matrix products grouped by expert, and the scaled 8-bit product (one group): one thread per output element.
-#include <cuda_bf16.h>
-
-#include "host.h"
-#include "sm100.cuh"
+// Entry points of the products grouped by expert and of the scaled 8-bit product (one group): argument checks and the
+// choice of the kernel.
+#include "grouped.h"
 
 namespace tcb {
-
-enum GroupedMode { kForward, kForwardI8, kDgrad, kWgrad };
-
-struct GroupedParams {
-    const void* p;          // fwd: B, dgrad: B, wgrad: A
-    const void* q;          // fwd: A, dgrad: dC, wgrad: dC
-    const float* scale_a;
-    const float* scale_b;
-    const void* offsets;    // null: one group of all rows
-    int offsets_are_int64;
-    void* out;
-    int64_t rows, experts, N, K, ldp, stride_p, ldq, ldo, stride_o;
-    int in_type, out_type;
-    uint32_t* status;
-};
-
-__device__ __forceinline__ float load_half(const void* p, int64_t i, int type) {
-    return type == TC_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]) : __half2float(static_cast<const __half*>(p)[i]);
-}
-
-__device__ __forceinline__ void store_out(void* p, int64_t i, float v, int type) {
-    if (type == TC_F32) static_cast<float*>(p)[i] = v;
-    else if (type == TC_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
-    else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-}
-
-// Row range of a group, clamped into the tensor; *bad is set when an offset lies outside or the pair decreases.
-__device__ __forceinline__ void group_rows(const GroupedParams& p, int e, int64_t& first, int64_t& last, bool& bad) {
-    if (p.offsets == nullptr) {
-        first = 0;
-        last = p.rows;
-        return;
-    }
-    const int64_t a = p.offsets_are_int64 ? static_cast<const int64_t*>(p.offsets)[e] : static_cast<const int32_t*>(p.offsets)[e];
-    const int64_t b = p.offsets_are_int64 ? static_cast<const int64_t*>(p.offsets)[e + 1] : static_cast<const int32_t*>(p.offsets)[e + 1];
-    bad |= a < 0 || b > p.rows || b < a;
-    first = min(max(a, static_cast<int64_t>(0)), p.rows);
-    last = max(first, min(max(b, static_cast<int64_t>(0)), p.rows));
-}
-
-template <int kMode>
-__global__ void __launch_bounds__(256) grouped_kernel(const GroupedParams p) {
-    bool bad = false;
-    for (int64_t e = blockIdx.z; e < p.experts; e += gridDim.z) {
-        int64_t first = 0, last = 0;
-        group_rows(p, static_cast<int>(e), first, last, bad);
-        const int64_t out_rows = kMode == kWgrad ? p.N : last - first;
-        const int64_t out_cols = kMode == kForward || kMode == kForwardI8 ? p.N : p.K;
-        for (int64_t r = blockIdx.y * 16 + threadIdx.y; r < out_rows; r += gridDim.y * 16) {
-            for (int64_t c = static_cast<int64_t>(blockIdx.x) * 16 + threadIdx.x; c < out_cols; c += static_cast<int64_t>(gridDim.x) * 16) {
-                if (kMode == kForwardI8) {
-                    const int8_t* a = static_cast<const int8_t*>(p.q) + (first + r) * p.ldq;
-                    const int8_t* b = static_cast<const int8_t*>(p.p) + e * p.stride_p + c * p.ldp;
-                    int acc = 0;
-                    for (int64_t k = 0; k < p.K; ++k) acc += static_cast<int>(a[k]) * static_cast<int>(b[k]);
-                    const float v = static_cast<float>(acc) * p.scale_a[first + r] * p.scale_b[e * p.N + c];
-                    store_out(p.out, (first + r) * p.ldo + c, v, p.out_type);
-                } else {
-                    float acc = 0.f;
-                    if (kMode == kForward) {
-                        for (int64_t k = 0; k < p.K; ++k)
-                            acc = fmaf(load_half(p.q, (first + r) * p.ldq + k, p.in_type), load_half(p.p, e * p.stride_p + c * p.ldp + k, p.in_type), acc);
-                    } else if (kMode == kDgrad) {
-                        for (int64_t n = 0; n < p.N; ++n)
-                            acc = fmaf(load_half(p.q, (first + r) * p.ldq + n, p.in_type), load_half(p.p, e * p.stride_p + n * p.ldp + c, p.in_type), acc);
-                    } else {
-                        for (int64_t t = first; t < last; ++t)
-                            acc = fmaf(load_half(p.q, t * p.ldq + r, p.in_type), load_half(p.p, t * p.ldp + c, p.in_type), acc);
-                    }
-                    store_out(p.out, (kMode == kWgrad ? e * p.stride_o + r * p.ldo : (first + r) * p.ldo) + c, acc, p.out_type);
-                }
-            }
-        }
-    }
-    if (bad) atomicMax(p.status, static_cast<uint32_t>(kDevIndexOutOfRange));
-}
-
-template <int kMode>
-static int launch_grouped(GroupedParams& p, cudaStream_t stream) {
-    const DeviceInfo* dev = nullptr;
-    if (int rc = current_device(&dev)) return rc;
-    p.status = dev->status_word;
-    const int64_t out_cols = kMode == kForward || kMode == kForwardI8 ? p.N : p.K;
-    const int64_t out_rows = kMode == kWgrad ? p.N : p.rows;
-    const dim3 grid(static_cast<unsigned>(min((out_cols + 15) / 16, static_cast<int64_t>(1024))),
-                    static_cast<unsigned>(max(static_cast<int64_t>(1), min((out_rows + 15) / 16, static_cast<int64_t>(1024)))),
-                    static_cast<unsigned>(min(p.experts, static_cast<int64_t>(1024))));
-    grouped_kernel<kMode><<<grid, dim3(16, 16), 0, stream>>>(p);
-    TCB_CUDA(cudaGetLastError());
-    return TC_OK;
-}
 
 static bool half_type(int t) { return t == TC_F16 || t == TC_BF16; }
 static bool any_type(int t) { return t == TC_F32 || half_type(t); }
@@ -107,7 +14,7 @@ static int check_sizes(const char* op, int64_t rows, int64_t experts, int64_t N,
     TCB_REQUIRE(experts > 0 && N > 0 && K > 0, "%s: experts, N and K must be positive (got %lld, %lld, %lld)", op, (long long)experts,
                 (long long)N, (long long)K);
     TCB_REQUIRE(rows < (1ll << 31) && N < (1ll << 31) && K < (1ll << 31), "%s: a dimension does not fit in 31 bits", op);
-    if (experts > 2048) return fail(TC_ERR_UNSUPPORTED, "%s: %lld experts, at most 2048 are supported", op, (long long)experts);
+    if (experts > kMaxExperts) return fail(TC_ERR_UNSUPPORTED, "%s: %lld experts, at most %d are supported", op, (long long)experts, kMaxExperts);
     return TC_OK;
 }
 
@@ -154,6 +61,12 @@ static int check_i8(const char* op, int64_t K, int c_type, const float* scale_a,
     return TC_OK;
 }
 
+static int launch_grouped(const GroupedProblem& g, tc_stream_t stream) {
+    const DeviceInfo* dev = nullptr;
+    if (int rc = current_device(&dev)) return rc;
+    return launch_grouped_pair(g, dev, static_cast<cudaStream_t>(stream));
+}
+
 #define TCB_TRY(expr)             \
     do {                          \
         if (int _rc = (expr)) return _rc; \
@@ -171,8 +84,7 @@ extern "C" int tc_gemm_i8(const void* A, const void* B, const float* scale_a, co
     TCB_TRY(check_input(op, "A", A, lda, K, 1));
     TCB_TRY(check_input(op, "B", B, ldb, K, 1));
     TCB_TRY(check_output(op, "C", C, ldc, N, c_type));
-    GroupedParams p{B, A, scale_a, scale_b, nullptr, 0, C, M, 1, N, K, ldb, 0, lda, ldc, 0, 0, c_type, nullptr};
-    return launch_grouped<kForwardI8>(p, static_cast<cudaStream_t>(stream));
+    return launch_grouped({B, A, scale_b, scale_a, nullptr, 0, C, M, 1, N, K, ldb, 0, lda, ldc, 0, kTypeI8, c_type, false, false}, stream);
 }
 
 extern "C" int tc_grouped_gemm_i8(const void* A, const void* B, const float* scale_a, const float* scale_b, const void* offsets,
@@ -188,8 +100,8 @@ extern "C" int tc_grouped_gemm_i8(const void* A, const void* B, const float* sca
     TCB_TRY(check_input(op, "B", B, ldb, K, 1));
     TCB_TRY(check_stack(op, "B", stride_b, K, experts, 1));
     TCB_TRY(check_output(op, "C", C, ldc, N, c_type));
-    GroupedParams p{B, A, scale_a, scale_b, offsets, offsets_are_int64, C, rows, experts, N, K, ldb, stride_b, lda, ldc, 0, 0, c_type, nullptr};
-    return launch_grouped<kForwardI8>(p, static_cast<cudaStream_t>(stream));
+    return launch_grouped({B, A, scale_b, scale_a, offsets, offsets_are_int64, C, rows, experts, N, K, ldb, stride_b, lda, ldc, 0, kTypeI8, c_type,
+                           false, false}, stream);
 }
 
 extern "C" int tc_grouped_gemm(const void* A, const void* B, const void* offsets, int offsets_are_int64, void* C, int64_t rows,
@@ -205,8 +117,8 @@ extern "C" int tc_grouped_gemm(const void* A, const void* B, const void* offsets
     TCB_TRY(check_input(op, "B", B, ldb, K, 2));
     TCB_TRY(check_stack(op, "B", stride_b, K, experts, 2));
     TCB_TRY(check_output(op, "C", C, ldc, N, c_type));
-    GroupedParams p{B, A, nullptr, nullptr, offsets, offsets_are_int64, C, rows, experts, N, K, ldb, stride_b, lda, ldc, 0, in_type, c_type, nullptr};
-    return launch_grouped<kForward>(p, static_cast<cudaStream_t>(stream));
+    return launch_grouped({B, A, nullptr, nullptr, offsets, offsets_are_int64, C, rows, experts, N, K, ldb, stride_b, lda, ldc, 0, in_type, c_type,
+                           false, false}, stream);
 }
 
 extern "C" int tc_grouped_gemm_dgrad(const void* dC, const void* B, const void* offsets, int offsets_are_int64, void* dA,
@@ -222,8 +134,8 @@ extern "C" int tc_grouped_gemm_dgrad(const void* dC, const void* B, const void* 
     TCB_TRY(check_input(op, "B", B, ldb, K, 2));
     TCB_TRY(check_stack(op, "B", stride_b, K, experts, 2));
     TCB_TRY(check_output(op, "dA", dA, ldda, K, da_type));
-    GroupedParams p{B, dC, nullptr, nullptr, offsets, offsets_are_int64, dA, rows, experts, N, K, ldb, stride_b, lddc, ldda, 0, in_type, da_type, nullptr};
-    return launch_grouped<kDgrad>(p, static_cast<cudaStream_t>(stream));
+    return launch_grouped({B, dC, nullptr, nullptr, offsets, offsets_are_int64, dA, rows, experts, K, N, ldb, stride_b, lddc, ldda, 0, in_type, da_type,
+                           true, false}, stream);
 }
 
 extern "C" int tc_grouped_gemm_wgrad(const void* dC, const void* A, const void* offsets, int offsets_are_int64, void* dB,
@@ -240,6 +152,13 @@ extern "C" int tc_grouped_gemm_wgrad(const void* dC, const void* A, const void* 
     }
     TCB_TRY(check_output(op, "dB", dB, lddb, K, db_type));
     TCB_REQUIRE(experts == 1 || stride_db >= K, "%s: expert stride of dB smaller than a row", op);
-    GroupedParams p{A, dC, nullptr, nullptr, offsets, offsets_are_int64, dB, rows, experts, N, K, lda, 0, lddc, lddb, stride_db, in_type, db_type, nullptr};
-    return launch_grouped<kWgrad>(p, static_cast<cudaStream_t>(stream));
+    if (rows == 0) {   // nothing to sum over, and no tensors to describe to TMA
+        const size_t es = static_cast<size_t>(type_bytes(db_type));
+        for (int64_t e = 0; e < experts; ++e)
+            TCB_CUDA(cudaMemset2DAsync(static_cast<uint8_t*>(dB) + static_cast<size_t>(e * stride_db) * es, static_cast<size_t>(lddb) * es, 0,
+                                       static_cast<size_t>(K) * es, static_cast<size_t>(N), static_cast<cudaStream_t>(stream)));
+        return TC_OK;
+    }
+    return launch_grouped({A, dC, nullptr, nullptr, offsets, offsets_are_int64, dB, rows, experts, K, N, lda, 0, lddc, lddb, stride_db, in_type, db_type,
+                           true, true}, stream);
 }

@@ -1,0 +1,374 @@
+// Grouped products on CTA pairs: tiles of 256 output columns (128 per CTA) by up to 256 rows, tcgen05.mma.cta_group::2
+// with M = 256 (output columns) and N = the tile's rows rounded up to 32. See grouped.h for the common form.
+//   warp 0      TMA producer (both CTAs): per stage 256 bytes of x for 128 columns of P and half of the tile's rows of Q,
+//               landing in the issuing CTA's shared memory and completing on the leader's full barrier;
+//   warp 1      TMEM owner; in the leader also the MMA issuer;
+//   warps 2..5  epilogue (both CTAs): accumulator columns -> scaled -> converted -> shared memory -> rows of the output;
+//   warp 6      wgrad only: the last x block of a group holds rows of the next group, which have to count as zero
+//               whatever they hold (NaN included), in both operands. The K step of the MMA is 16 rows, so up to 15 rows
+//               of each operand tile are overwritten with zeros before the MMAs read them.
+// Persistent over tiles; accumulators are double-buffered in TMEM. Which tiles there are follows from the offsets, which
+// every CTA reads from device memory into a table at the start.
+#include "grouped.cuh"
+
+namespace tcb {
+
+constexpr int kGpCols = 128;              // output columns per CTA
+constexpr int kGpRows = 256;              // most rows per tile
+constexpr int kGpStages = 3;
+constexpr int kGpOperand = 128 * 256;     // bytes of one operand per stage and CTA: 128 columns / rows x 256 bytes of x
+constexpr int kGpChunk = kGpOperand / 2;  // 128 bytes of x (x contiguous), or 64 columns / rows (those contiguous)
+constexpr int kGpStageBytes = 2 * kGpOperand;
+constexpr int kGpStaging = 4 * 4096;
+constexpr int kGpScales = 4 * 128;
+constexpr int kGpBars = 256;
+constexpr int kGpSmem = kGpStages * kGpStageBytes + kGpStaging + kGpScales + kGpBars + static_cast<int>(sizeof(GroupTable)) + 1024;
+static_assert(kGpSmem <= 232448, "shared memory of one CTA");
+
+__device__ __forceinline__ void umma_i8_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t"
+        "}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorMap* m, uint32_t bar_cluster_addr, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+template <bool kI8, bool kPCols, bool kRaggedX>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kRaggedX ? 224 : 192, 1)
+grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q,
+                    const __grid_constant__ CUtensorMap tmap_q32, const GroupedArgs a) {
+    constexpr int kBlockX = kI8 ? 256 : 128;   // x elements per stage
+    constexpr int kStepX = kBlockX / 8;        // per MMA
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = align_smem_1024(smem_raw);
+    uint8_t* smem_p = smem;
+    uint8_t* smem_q = smem + kGpStages * kGpOperand;
+    uint8_t* staging = smem + kGpStages * kGpStageBytes;
+    float* scales = reinterpret_cast<float*>(staging + kGpStaging);
+    uint64_t* bar_full = reinterpret_cast<uint64_t*>(staging + kGpStaging + kGpScales);   // used in the leader
+    uint64_t* bar_empty = bar_full + kGpStages;          // one per CTA
+    uint64_t* bar_acc_full = bar_empty + kGpStages;      // one per CTA
+    uint64_t* bar_acc_empty = bar_acc_full + 2;          // used in the leader
+    uint64_t* bar_tail_full = bar_acc_empty + 2;         // one per CTA: a stage whose last rows have to be cleared has landed
+    uint64_t* bar_tail_ready = bar_tail_full + kGpStages;   // used in the leader: both CTAs have cleared them
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_tail_ready + kGpStages);
+    volatile uint32_t* abort_word = tmem_slot + 1;
+    GroupTable* table = reinterpret_cast<GroupTable*>(reinterpret_cast<uint8_t*>(bar_full) + kGpBars);
+
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+    const int lane = threadIdx.x & 31;
+    const uint32_t rank = __shfl_sync(0xffffffffu, cluster_ctarank(), 0);   // 0 = leader
+    const int pair = blockIdx.x >> 1;
+    const int num_pairs = gridDim.x >> 1;
+    const int col_tiles = (a.cols + 2 * kGpCols - 1) / (2 * kGpCols);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kGpStages; ++s) {
+            mbar_init(&bar_full[s], 1);
+            mbar_init(&bar_empty[s], 1);
+            mbar_init(&bar_tail_full[s], 1);
+            mbar_init(&bar_tail_ready[s], 2);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bar_acc_full[i], 1);
+            mbar_init(&bar_acc_empty[i], 8);   // four epilogue warps in each CTA of the pair
+        }
+        *abort_word = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(tmem_slot, 512);
+        tmem_relinquish_pair();
+    }
+    grid_launch_dependents();
+    grid_dependency_wait();   // the offsets may come from the kernel before this one
+    if (warp == 0) build_group_table(table, a, kRaggedX ? (a.other + a.tile_rows - 1) / a.tile_rows : -1, blockIdx.x == 0);
+    tc_fence_before_sync();
+    cluster_sync_all();   // barriers of both CTAs are initialised before anyone signals across the pair
+    tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot;
+    const int num_tiles = table->tiles_before[a.experts] * col_tiles;
+
+    if (warp == 0) {
+        // ---------------- TMA producer (both CTAs) ----------------
+        const bool leader = elect_one_sync();
+        if (leader) {
+            tma_prefetch_desc(&tmap_p);
+            tma_prefetch_desc(&tmap_q);
+        }
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
+            const GroupTile t = group_tile<kRaggedX>(table, a, tile, col_tiles, 2 * kGpCols);
+            const int blocks = (t.x_len + kBlockX - 1) / kBlockX;
+            const int col = t.col0 + static_cast<int>(rank) * kGpCols;
+            const int half = t.width >> 1;                              // this CTA's rows of Q
+            const int row = t.row0 + static_cast<int>(rank) * half;
+            for (int kb = 0; kb < blocks; ++kb) {
+                if (!mbar_wait_warp(&bar_empty[stage], phase ^ 1u, abort_word, kDevTimeoutProducer)) {
+                    ok = false;
+                    break;
+                }
+                const int x = kb * kBlockX;
+                const int chunks = t.x_len - x > kBlockX / 2 ? 2 : 1;   // 128-byte pieces of x
+                const int q_boxes = (half + 31) >> 5;
+                const bool whole_q = t.width == kGpRows;
+                const bool two_rows = half > 64;                         // wgrad: 64-row pieces of Q
+                const bool tail = kRaggedX && kb == blocks - 1 && (t.x_len & 15) != 0;
+                const uint32_t p_bytes = kPCols ? kGpOperand : chunks * kGpChunk;
+                const uint32_t q_bytes = kRaggedX ? (two_rows ? kGpOperand : kGpChunk) : chunks * (whole_q ? kGpChunk : q_boxes * 4096);
+                uint64_t* bar = tail ? &bar_tail_full[stage] : &bar_full[stage];
+                // full counts the bytes of both CTAs, in the leader; a tail counts its own in each
+                const uint32_t bar_addr = map_to_cta(smem_u32(bar), tail ? rank : 0);
+                uint8_t* dst_p = smem_p + stage * kGpOperand;
+                uint8_t* dst_q = smem_q + stage * kGpOperand;
+                if (leader) {
+                    if (tail) {
+                        mbar_arrive_expect_tx(bar, p_bytes + q_bytes);
+                        if (rank == 0) mbar_arrive(&bar_full[stage]);
+                    } else if (rank == 0) {
+                        mbar_arrive_expect_tx(bar, 2 * (p_bytes + q_bytes));
+                    }
+                    if (kPCols) {
+                        const int y = kRaggedX ? t.x0 + x : x;
+                        const int z = kRaggedX ? 0 : t.e;
+                        tma_load_3d_pair(dst_p, &tmap_p, bar_addr, col, y, z);
+                        tma_load_3d_pair(dst_p + kGpChunk, &tmap_p, bar_addr, col + 64, y, z);
+                    } else {
+                        for (int c = 0; c < chunks; ++c) tma_load_3d_pair(dst_p + c * kGpChunk, &tmap_p, bar_addr, x + c * (kBlockX / 2), col, t.e);
+                    }
+                    if (kRaggedX) {
+                        tma_load_2d_pair(dst_q, &tmap_q, bar_addr, row, t.x0 + x);
+                        if (two_rows) tma_load_2d_pair(dst_q + kGpChunk, &tmap_q, bar_addr, row + 64, t.x0 + x);
+                    } else if (whole_q) {
+                        for (int c = 0; c < chunks; ++c) tma_load_2d_pair(dst_q + c * kGpChunk, &tmap_q, bar_addr, x + c * (kBlockX / 2), row);
+                    } else {
+                        for (int c = 0; c < chunks; ++c)
+                            for (int b = 0; b < q_boxes; ++b)
+                                tma_load_2d_pair(dst_q + c * kGpChunk + b * 4096, &tmap_q32, bar_addr, x + c * (kBlockX / 2), row + b * 32);
+                    }
+                }
+                if (++stage == kGpStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ---------------- MMA issuer (leader CTA only) ----------------
+        if (lane == 0 && rank == 0) {
+            const uint32_t desc_hi = smem_desc_hi_sw128(1024);
+            const uint32_t p_lo0 = smem_desc_lo(smem_u32(smem_p), kPCols ? kGpChunk : 16);
+            const uint32_t q_lo0 = smem_desc_lo(smem_u32(smem_q), kRaggedX ? kGpChunk : 16);
+            int stage = 0;
+            uint32_t phase = 0;
+            int acc = 0;
+            uint32_t acc_phase = 0;
+            uint32_t tail_phase = 0;   // one bit per stage
+            bool ok = true;
+            for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
+                const GroupTile t = group_tile<kRaggedX>(table, a, tile, col_tiles, 2 * kGpCols);
+                const int blocks = (t.x_len + kBlockX - 1) / kBlockX;
+                const uint32_t idesc = a.idesc | (static_cast<uint32_t>(t.width >> 3) << 17);
+                if (!mbar_wait(&bar_acc_empty[acc], acc_phase ^ 1u, abort_word, kDevTimeoutMma)) break;
+                tc_fence_after_sync();
+                const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kGpRows);
+                for (int kb = 0; kb < blocks; ++kb) {
+                    if (!mbar_wait(&bar_full[stage], phase, abort_word, kDevTimeoutMma)) {
+                        ok = false;
+                        break;
+                    }
+                    const int rest = t.x_len - kb * kBlockX;
+                    if (kRaggedX && rest <= kBlockX && (rest & 15) != 0) {
+                        if (!mbar_wait_cluster(&bar_tail_ready[stage], (tail_phase >> stage) & 1u, abort_word, kDevTimeoutMma)) {
+                            ok = false;
+                            break;
+                        }
+                        tail_phase ^= 1u << stage;
+                    }
+                    tc_fence_after_sync();
+                    const uint32_t p_lo = p_lo0 + static_cast<uint32_t>(stage) * (kGpOperand >> 4);
+                    const uint32_t q_lo = q_lo0 + static_cast<uint32_t>(stage) * (kGpOperand >> 4);
+                    const int steps = min(8, (rest + kStepX - 1) / kStepX);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        if (k < steps) {
+                            // x contiguous: 32 bytes on in the swizzled row, the next chunk after four; else 16 rows of x on
+                            const uint32_t off_p = kPCols ? k * (2048u >> 4) : static_cast<uint32_t>(((k >> 2) * kGpChunk + (k & 3) * 32) >> 4);
+                            const uint32_t off_q = kRaggedX ? k * (2048u >> 4) : static_cast<uint32_t>(((k >> 2) * kGpChunk + (k & 3) * 32) >> 4);
+                            const uint64_t dp = smem_desc_join(p_lo + off_p, desc_hi), dq = smem_desc_join(q_lo + off_q, desc_hi);
+                            if (kI8) umma_i8_ss_pair(d_tmem, dp, dq, idesc, (kb | k) != 0);
+                            else umma_f16_ss_pair(d_tmem, dp, dq, idesc, (kb | k) != 0);
+                        }
+                    }
+                    umma_commit_pair_both(smem_u32(&bar_empty[stage]));
+                    if (++stage == kGpStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                umma_commit_pair_both(smem_u32(&bar_acc_full[acc]));
+                if (++acc == 2) {
+                    acc = 0;
+                    acc_phase ^= 1u;
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp < 6) {
+        // ---------------- epilogue (both CTAs) ----------------
+        const int quarter = warp & 3;
+        uint8_t* stage = staging + quarter * 4096;
+        float* row_scales = scales + quarter * 32;
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        for (int tile = pair; tile < num_tiles; tile += num_pairs) {
+            const GroupTile t = group_tile<kRaggedX>(table, a, tile, col_tiles, 2 * kGpCols);
+            const int col = t.col0 + static_cast<int>(rank) * kGpCols + quarter * 32;
+            const int cols = a.cols - col;     // columns of the output from this warp's first on
+            float sp = 1.f;
+            if (kI8 && lane < cols) sp = a.scale_p[static_cast<int64_t>(t.e) * a.cols + col + lane];
+            if (!mbar_wait_warp(&bar_acc_full[acc], acc_phase, abort_word, kDevTimeoutEpilogue)) break;
+            tc_fence_after_sync();
+            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * kGpRows);
+            if (cols > 0) {
+                for (int j0 = 0; j0 < t.rows; j0 += 32) {
+                    uint32_t r[32];
+                    float v[32];
+                    if (kI8) {
+                        const int row = j0 + lane;
+                        const float sq = row < t.rows ? a.scale_q[t.row0 + row] : 0.f;
+                        __syncwarp();
+                        row_scales[lane] = sq;
+                    }
+                    tmem_ld_x32(taddr + static_cast<uint32_t>(j0), r);
+                    tmem_ld_wait();
+                    if (kI8) {
+                        __syncwarp();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = __int2float_rn(static_cast<int>(r[j])) * row_scales[j] * sp;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = kRaggedX && t.x_len == 0 ? 0.f : __uint_as_float(r[j]);
+                    }
+                    const int64_t index = (kRaggedX ? t.e * a.stride_o : 0) + static_cast<int64_t>(t.row0 + j0) * a.ldo + col;
+                    store_block(v, stage, a, index, t.rows - j0, cols, lane);
+                }
+            }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&bar_acc_empty[acc]), 0));
+            if (++acc == 2) {
+                acc = 0;
+                acc_phase ^= 1u;
+            }
+        }
+    } else if (kRaggedX) {
+        // ---------------- clears the foreign rows of a group's last x block (both CTAs) ----------------
+        int blocks_before = 0;
+        uint32_t tail_phase = 0;
+        for (int tile = pair; tile < num_tiles; tile += num_pairs) {
+            const GroupTile t = group_tile<kRaggedX>(table, a, tile, col_tiles, 2 * kGpCols);
+            const int blocks = (t.x_len + kBlockX - 1) / kBlockX;
+            if ((t.x_len & 15) != 0) {
+                const int s = (blocks_before + blocks - 1) % kGpStages;
+                if (!mbar_wait_warp(&bar_tail_full[s], (tail_phase >> s) & 1u, abort_word, kDevTimeoutMma)) break;
+                tail_phase ^= 1u << s;
+                const int first = t.x_len - (blocks - 1) * kBlockX;
+                const int n = ((first + 15) & ~15) - first;      // rows of 128 bytes in each of the four 64-wide pieces
+                uint8_t* p = smem_p + s * kGpOperand;
+                uint8_t* q = smem_q + s * kGpOperand;
+                for (int i = lane; i < n * 8; i += 32) {
+                    const int at = (first + (i >> 3)) * 128 + (i & 7) * 16;
+                    *reinterpret_cast<uint4*>(p + at) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(p + kGpChunk + at) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(q + at) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(q + kGpChunk + at) = make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&bar_tail_ready[s]), 0));
+            }
+            blocks_before += blocks;
+        }
+    }
+
+    // ---------------- teardown: neither CTA frees TMEM or exits while its peer may still touch it ----------------
+    __syncwarp();
+    tc_fence_before_sync();
+    cluster_sync_all();
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc_pair(tmem_base, 512);
+    }
+    if (threadIdx.x == 0 && *abort_word != 0) atomicMax(a.status, *abort_word);
+}
+
+template <bool kI8, bool kPCols, bool kRaggedX>
+static int launch_variant(const CUtensorMap& tp, const CUtensorMap& tq, const CUtensorMap& tq32, const GroupedArgs& a, int pairs,
+                          const DeviceInfo* dev, cudaStream_t stream) {
+    auto kernel = grouped_pair_kernel<kI8, kPCols, kRaggedX>;
+    static OncePerDevice once;
+    if (int rc = raise_smem_limit_once(once, dev->device, kernel, kGpSmem)) return rc;
+    TCB_CUDA(launch_overlapped(kernel, dim3(2 * pairs), dim3(kRaggedX ? 224 : 192), kGpSmem, stream, tp, tq, tq32, a));
+    return TC_OK;
+}
+
+int launch_grouped_pair(const GroupedProblem& g, const DeviceInfo* dev, cudaStream_t stream) {
+    const bool i8 = g.in_type == kTypeI8;
+    const int es = i8 ? 1 : 2;
+    const uint32_t chunk_x = 128 / es;
+    GroupedArgs a = grouped_args(g, dev);
+    a.tile_rows = kGpRows;
+    // M = 256: tcgen05 instruction descriptor, see make_idesc_f16_f32; kind::i8 counts D format 2 (s32), A and B format 1 (s8)
+    a.idesc = i8 ? (2u << 4) | (1u << 7) | (1u << 10) | (16u << 24)
+                 : make_idesc_f16_f32(2 * kGpCols, 0, g.p_c_contiguous, g.ragged_x) | (g.in_type == TC_BF16 ? kIdescBf16Inputs : 0u);
+    auto encode = [&](CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
+        return i8 ? encode_tmap_i8_sw128(out, base, rank, dims, strides, box)
+                  : encode_tmap_f16_sw128(out, base, rank, dims, strides, box, g.in_type == TC_BF16);
+    };
+    CUtensorMap tp, tq, tq32;
+    const uint64_t token_rows = static_cast<uint64_t>(g.token_rows);
+    {
+        const bool stack = !g.ragged_x;   // P is B [experts, rows, row length], or A [token_rows, cols]
+        const uint64_t inner = static_cast<uint64_t>(g.p_c_contiguous ? g.cols : g.other);
+        const uint64_t outer = stack ? static_cast<uint64_t>(g.p_c_contiguous ? g.other : g.cols) : token_rows;
+        const uint64_t dims[3] = {inner, outer, stack ? static_cast<uint64_t>(g.experts) : 1};
+        const uint64_t strides[2] = {static_cast<uint64_t>(g.ldp) * es, static_cast<uint64_t>(stack && g.experts > 1 ? g.stride_p : g.ldp) * es};
+        const uint32_t box[3] = {chunk_x, 128, 1};
+        if (int rc = encode(&tp, g.p, 3, dims, strides, box)) return rc;
+    }
+    {
+        const uint64_t dims[2] = {static_cast<uint64_t>(g.other), token_rows};
+        const uint64_t strides[1] = {static_cast<uint64_t>(g.ldq) * es};
+        const uint32_t box[2] = {chunk_x, 128};
+        const uint32_t box32[2] = {chunk_x, 32};
+        if (int rc = encode(&tq, g.q, 2, dims, strides, box)) return rc;
+        if (int rc = encode(&tq32, g.q, 2, dims, strides, box32)) return rc;
+    }
+    const int64_t col_tiles = (g.cols + 2 * kGpCols - 1) / (2 * kGpCols);
+    const int64_t most_row_tiles = g.ragged_x ? g.experts * ((g.other + kGpRows - 1) / kGpRows)
+                                              : g.token_rows / kGpRows + (g.experts < g.token_rows ? g.experts : g.token_rows);
+    if (most_row_tiles * col_tiles >= (1ll << 31)) return fail(TC_ERR_UNSUPPORTED, "grouped product: too many output tiles");
+    const int64_t max_pairs = dev->sm_count / 2;
+    const int pairs = static_cast<int>(most_row_tiles * col_tiles < max_pairs ? most_row_tiles * col_tiles : max_pairs);
+    if (i8) return launch_variant<true, false, false>(tp, tq, tq32, a, pairs, dev, stream);
+    if (g.ragged_x) return launch_variant<false, true, true>(tp, tq, tq32, a, pairs, dev, stream);
+    if (g.p_c_contiguous) return launch_variant<false, true, false>(tp, tq, tq32, a, pairs, dev, stream);
+    return launch_variant<false, false, false>(tp, tq, tq32, a, pairs, dev, stream);
+}
+
+}  // namespace tcb

@@ -65,8 +65,8 @@ static int load_encode() {
     return TC_OK;
 }
 
-int encode_tmap_f16_sw128(CUtensorMap* out, const void* base, int rank, const uint64_t* dims,
-                          const uint64_t* strides_bytes, const uint32_t* box, bool bf16) {
+static int encode_tmap_sw128(CUtensorMap* out, const void* base, int rank, const uint64_t* dims,
+                             const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapDataType type) {
     if (int rc = load_encode()) return rc;
     cuuint64_t gdim[5];
     cuuint64_t gstride[5];
@@ -78,7 +78,7 @@ int encode_tmap_f16_sw128(CUtensorMap* out, const void* base, int rank, const ui
         estride[i] = 1;
         if (i + 1 < rank) gstride[i] = strides_bytes[i];
     }
-    CUresult r = g_encode(out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, static_cast<cuuint32_t>(rank),
+    CUresult r = g_encode(out, type, static_cast<cuuint32_t>(rank),
                           const_cast<void*>(base), gdim, gstride, bdim, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -88,6 +88,16 @@ int encode_tmap_f16_sw128(CUtensorMap* out, const void* base, int rank, const ui
                     static_cast<int>(r), rank, (unsigned long long)dims[0], (unsigned long long)(rank > 1 ? dims[1] : 1),
                     box[0], rank > 1 ? box[1] : 1u);
     return TC_OK;
+}
+
+int encode_tmap_f16_sw128(CUtensorMap* out, const void* base, int rank, const uint64_t* dims,
+                          const uint64_t* strides_bytes, const uint32_t* box, bool bf16) {
+    return encode_tmap_sw128(out, base, rank, dims, strides_bytes, box, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
+}
+
+int encode_tmap_i8_sw128(CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
+                         const uint32_t* box) {
+    return encode_tmap_sw128(out, base, rank, dims, strides_bytes, box, CU_TENSOR_MAP_DATA_TYPE_UINT8);
 }
 
 int encode_tmap_f32_sw128(CUtensorMap* out, const void* base, uint64_t cols, uint64_t rows, uint64_t row_stride_bytes,

@@ -131,6 +131,14 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
     return mbar_wait_slow(bar, parity, abort_word, code);
 }
 
+// mbar_wait_cluster: one thread, for a barrier that threads of another CTA of the cluster arrive on after writing
+// memory that this thread's work reads: the wait acquires at cluster scope.
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_word, uint32_t code) {
+    const bool ok = mbar_wait(bar, parity, abort_word, code);
+    asm volatile("fence.acq_rel.cluster;" ::: "memory");
+    return ok;
+}
+
 // mbar_wait_warp: a whole converged warp; every lane polls (so every lane acquires the phase) and the
 // warp leaves together, which keeps a timeout from leaving part of a warp behind before a
 // warp-collective instruction (tcgen05.ld / st, votes).
