@@ -1,6 +1,7 @@
 // Entry points of the products grouped by expert and of the scaled 8-bit product (one group): argument checks and the
 // choice of the kernel.
 #include "grouped.h"
+#include "sm100.cuh"
 
 namespace tcb {
 
@@ -61,10 +62,69 @@ static int check_i8(const char* op, int64_t K, int c_type, const float* scale_a,
     return TC_OK;
 }
 
+uint32_t grouped_idesc(const GroupedProblem& g, int m) {
+    if (g.in_type == kTypeI8) return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(m >> 4) << 24);
+    return make_idesc_f16_f32(m, 0, g.p_c_contiguous, g.ragged_x) | (g.in_type == TC_BF16 ? kIdescBf16Inputs : 0u);
+}
+
+static int encode_operand(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box,
+                          int in_type) {
+    if (in_type == kTypeI8) return encode_tmap_i8_sw128(map, base, rank, dims, strides, box);
+    return encode_tmap_f16_sw128(map, base, rank, dims, strides, box, in_type == TC_BF16);
+}
+
+int grouped_map_p(CUtensorMap* map, const GroupedProblem& g, int box_rows) {
+    // B [experts, rows, row length], or for wgrad A [token_rows, cols]
+    const uint64_t es = g.in_type == kTypeI8 ? 1 : 2;
+    const int64_t inner = g.p_c_contiguous ? g.cols : g.other;
+    const int64_t outer = g.ragged_x ? g.token_rows : g.p_c_contiguous ? g.other : g.cols;
+    const bool stack = !g.ragged_x && g.experts > 1;
+    const uint64_t dims[3] = {static_cast<uint64_t>(inner), static_cast<uint64_t>(outer), stack ? static_cast<uint64_t>(g.experts) : 1};
+    const uint64_t strides[2] = {static_cast<uint64_t>(g.ldp) * es, static_cast<uint64_t>(stack ? g.stride_p : g.ldp) * es};
+    const uint32_t box[3] = {static_cast<uint32_t>(128 / es), static_cast<uint32_t>(box_rows), 1};
+    return encode_operand(map, g.p, 3, dims, strides, box, g.in_type);
+}
+
+int grouped_map_q(CUtensorMap* map, const GroupedProblem& g, int box_rows) {
+    const uint64_t es = g.in_type == kTypeI8 ? 1 : 2;
+    const uint64_t dims[2] = {static_cast<uint64_t>(g.other), static_cast<uint64_t>(g.token_rows)};
+    const uint64_t strides[1] = {static_cast<uint64_t>(g.ldq) * es};
+    const uint32_t box[2] = {static_cast<uint32_t>(128 / es), static_cast<uint32_t>(box_rows)};
+    return encode_operand(map, g.q, 2, dims, strides, box, g.in_type);
+}
+
+#ifdef TCB_TUNE
+int g_force_pair = -1, g_force_rows = 0, g_force_splits = 0;
+extern "C" void tc_tune(int pair, int rows, int splits) { g_force_pair = pair; g_force_rows = rows; g_force_splits = splits; }
+#endif
+
+static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+static GroupedPlan grouped_plan(const GroupedProblem& g, int sm_count) {
+    GroupedPlan p;
+    p.pair = true;
+    p.tile_rows = 256;
+    p.splits = 1;
+#ifdef TCB_TUNE
+    if (g_force_pair >= 0 && !(g.ragged_x && g_force_rows < 64)) { p.pair = g_force_pair; p.tile_rows = g_force_rows; p.splits = g_force_splits; }
+#endif
+    const int64_t row_tiles = g.ragged_x ? g.experts * ceil_div(g.other, p.tile_rows)
+                              : g.offsets == nullptr ? ceil_div(g.token_rows, p.tile_rows)
+                                         : g.token_rows / p.tile_rows + (g.experts < g.token_rows ? g.experts : g.token_rows);
+    p.tiles = row_tiles * ceil_div(g.cols, p.pair ? 256 : 128);
+    return p;
+}
+
 static int launch_grouped(const GroupedProblem& g, tc_stream_t stream) {
     const DeviceInfo* dev = nullptr;
     if (int rc = current_device(&dev)) return rc;
-    return launch_grouped_pair(g, dev, static_cast<cudaStream_t>(stream));
+    const GroupedPlan plan = grouped_plan(g, dev->sm_count);
+    // tile numbers are 32-bit, also for offsets that give every expert all rows
+    if (g.experts * ceil_div(g.ragged_x ? g.other : g.token_rows, plan.tile_rows) * ceil_div(g.cols, 128) * plan.splits >= (1ll << 31))
+        return fail(TC_ERR_UNSUPPORTED, "grouped product: too many output tiles (%lld experts, %lld rows, %lld columns)", (long long)g.experts,
+                    (long long)g.token_rows, (long long)g.cols);
+    auto s = static_cast<cudaStream_t>(stream);
+    return plan.pair ? launch_grouped_pair(g, plan, dev, s) : launch_grouped_split(g, plan, dev, s);
 }
 
 #define TCB_TRY(expr)             \

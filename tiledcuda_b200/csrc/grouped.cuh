@@ -16,50 +16,60 @@ struct GroupTable {
     int tiles_before[kMaxExperts + 1];
 };
 
-// Executed by one whole warp. Offsets are clamped into [0, token_rows] and a decreasing pair makes an empty group, so
-// that whatever they hold no access leaves the tensors; `report` lets one CTA of the grid record that.
-// fixed_tiles >= 0: every group has that many row tiles (wgrad).
-__device__ __forceinline__ void build_group_table(GroupTable* t, const GroupedArgs& a, int fixed_tiles, bool report) {
-    const int lane = threadIdx.x & 31;
-    if (a.offsets == nullptr) {
-        if (lane == 0) {
-            t->first[0] = 0;
-            t->len[0] = a.token_rows;
-            t->tiles_before[0] = 0;
-            t->tiles_before[1] = fixed_tiles >= 0 ? fixed_tiles : (a.token_rows + a.tile_rows - 1) / a.tile_rows;
+// Row range of group e. Offsets are clamped into [0, token_rows] and a decreasing pair makes an empty group, so that
+// whatever they hold no access leaves the tensors; `bad` tells that this was needed.
+__device__ __forceinline__ void group_range(const GroupedArgs& a, int e, int& first, int& len, bool& bad) {
+    int64_t lo = 0, hi = a.token_rows;
+    if (a.offsets != nullptr) {
+        if (a.offsets_are_int64) {
+            lo = static_cast<const int64_t*>(a.offsets)[e];
+            hi = static_cast<const int64_t*>(a.offsets)[e + 1];
+        } else {
+            lo = static_cast<const int32_t*>(a.offsets)[e];
+            hi = static_cast<const int32_t*>(a.offsets)[e + 1];
         }
-        __syncwarp();
-        return;
     }
+    const int64_t rows = a.token_rows;
+    bad |= lo < 0 || hi > rows || hi < lo;
+    lo = min(max(lo, static_cast<int64_t>(0)), rows);
+    hi = max(lo, min(max(hi, static_cast<int64_t>(0)), rows));
+    first = static_cast<int>(lo);
+    len = static_cast<int>(hi - lo);
+}
+
+// Row tiles of a group: its rows cut evenly, or (wgrad) the same for every group.
+template <bool kRaggedX>
+__device__ __forceinline__ int group_row_tiles(const GroupedArgs& a, int len) {
+    return ((kRaggedX ? a.other : len) + a.tile_rows - 1) / a.tile_rows;
+}
+
+__device__ __forceinline__ int warp_inclusive_sum(int v) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += up;
+    }
+    return v;
+}
+
+// Executed by one whole warp; `report` lets one CTA of the grid record bad offsets.
+template <bool kRaggedX>
+__device__ __forceinline__ void build_group_table(GroupTable* t, const GroupedArgs& a, bool report) {
+    const int lane = threadIdx.x & 31;
     int base = 0;
     bool bad = false;
     for (int e0 = 0; e0 < a.experts; e0 += 32) {
         const int e = e0 + lane;
         int tiles = 0;
         if (e < a.experts) {
-            int64_t lo, hi;
-            if (a.offsets_are_int64) {
-                lo = static_cast<const int64_t*>(a.offsets)[e];
-                hi = static_cast<const int64_t*>(a.offsets)[e + 1];
-            } else {
-                lo = static_cast<const int32_t*>(a.offsets)[e];
-                hi = static_cast<const int32_t*>(a.offsets)[e + 1];
-            }
-            const int64_t rows = a.token_rows;
-            bad |= lo < 0 || hi > rows || hi < lo;
-            lo = min(max(lo, static_cast<int64_t>(0)), rows);
-            hi = max(lo, min(max(hi, static_cast<int64_t>(0)), rows));
-            const int len = static_cast<int>(hi - lo);
-            t->first[e] = static_cast<int>(lo);
+            int first, len;
+            group_range(a, e, first, len, bad);
+            t->first[e] = first;
             t->len[e] = len;
-            tiles = fixed_tiles >= 0 ? fixed_tiles : (len + a.tile_rows - 1) / a.tile_rows;
+            tiles = group_row_tiles<kRaggedX>(a, len);
         }
-        int sum = tiles;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int up = __shfl_up_sync(0xffffffffu, sum, d);
-            if (lane >= d) sum += up;
-        }
+        const int sum = warp_inclusive_sum(tiles);
         if (e < a.experts) t->tiles_before[e] = base + sum - tiles;
         base += __shfl_sync(0xffffffffu, sum, 31);
     }
@@ -69,10 +79,32 @@ __device__ __forceinline__ void build_group_table(GroupTable* t, const GroupedAr
 }
 
 // One output tile: rows [row0, row0 + rows) of the output (of group e's slice for wgrad), columns from col0 on, summed over
-// x in [x0, x0 + x_len). `width` is rows rounded up to 32, the N extent of its MMAs.
+// x in [x0, x0 + x_len). `width` is rows rounded up to 32 (16 where tiles have 16), the N extent of its MMAs.
 struct GroupTile {
     int e, row0, rows, width, col0, x0, x_len;
 };
+
+template <bool kRaggedX>
+__device__ __forceinline__ GroupTile make_group_tile(const GroupedArgs& a, int e, int first, int len, int rt, int row_tiles, int col0) {
+    GroupTile g;
+    g.e = e;
+    g.col0 = col0;
+    if (kRaggedX) {
+        g.row0 = rt * a.tile_rows;
+        g.rows = min(a.tile_rows, a.other - g.row0);
+        g.x0 = first;
+        g.x_len = len;
+    } else {
+        // the rows of a group spread evenly over its tiles, in steps of 32
+        const int step = min(a.tile_rows, ((len + row_tiles - 1) / row_tiles + 31) & ~31);
+        g.row0 = first + rt * step;
+        g.rows = min(step, len - rt * step);
+        g.x0 = 0;
+        g.x_len = a.other;
+    }
+    g.width = min(a.tile_rows, (g.rows + 31) & ~31);
+    return g;
+}
 
 // The tiles of a group are walked in bands of kBandCols column tiles, row tiles outermost inside a band, so that the CTAs
 // in flight share operands through L2.
@@ -87,8 +119,6 @@ __device__ __forceinline__ GroupTile group_tile(const GroupTable* t, const Group
         if (t->tiles_before[mid] <= row_tile_all) lo = mid;
         else hi = mid - 1;
     }
-    GroupTile g;
-    g.e = lo;
     const int before = t->tiles_before[lo];
     const int row_tiles = t->tiles_before[lo + 1] - before;
     const int local = tile - before * col_tiles;
@@ -98,79 +128,141 @@ __device__ __forceinline__ GroupTile group_tile(const GroupTable* t, const Group
     const int in_band = local - band * per_band;
     const int rt = in_band / band_cols;
     const int ct = band * kBandCols + in_band - rt * band_cols;
-    g.col0 = ct * tile_cols;
-    if (kRaggedX) {
-        g.row0 = rt * a.tile_rows;
-        g.rows = min(a.tile_rows, a.other - g.row0);
-        g.x0 = t->first[lo];
-        g.x_len = t->len[lo];
-    } else {
-        // the rows of a group spread evenly over its tiles, in steps of 32
-        const int len = t->len[lo];
-        const int step = ((len + row_tiles - 1) / row_tiles + 31) & ~31;
-        g.row0 = t->first[lo] + rt * step;
-        g.rows = min(step, len - rt * step);
-        g.x0 = 0;
-        g.x_len = a.other;
-    }
-    g.width = (g.rows + 31) & ~31;
-    return g;
+    return make_group_tile<kRaggedX>(a, lo, t->first[lo], t->len[lo], rt, row_tiles, ct * tile_cols);
 }
 
 __device__ __forceinline__ uint16_t to_half_bits(float v, int type) {
     return type == TC_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
 }
 
-// 32 x 32 block of the output, one column per lane and one row per register, through `stage` (4 KiB of this warp) to
-// out[row, col] for row < rows and column < cols: rows leave as 64-byte (16-bit types) or 128-byte pieces.
-__device__ __forceinline__ void store_block(const float (&v)[32], uint8_t* stage, const GroupedArgs& a, int64_t out_index, int rows,
-                                            int cols, int lane) {
-    __syncwarp();   // the previous block has left the staging area
-    if (a.out_type == TC_F32) {
-        float* s = reinterpret_cast<float*>(stage);
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi, int type) {
+    if (type == TC_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return pack_half2(lo, hi);
+}
+
+// 16 TMEM lanes by 32 columns: register 4 q + 2 i + b of a thread is lane 8 i + lane / 4, column 8 q + 2 (lane % 4) + b,
+// i.e. four 16 x 8 blocks, each in the accumulator fragment layout of the warp-level MMAs.
+__device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+
+// Four 8 x 8 blocks of 16-bit values, each stored transposed: lane l gives the address of row l % 8 of block l / 8.
+__device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// Drains the part of an output tile that one warp owns: 32 output columns (TMEM lanes, from column `col` of the output on)
+// by the tile's rows (TMEM columns), scaled, converted and stored; of the rows the 32 from `first` on, then `step` on. `staging` is 2 KiB and `row_scales` 32 floats of
+// shared memory of this warp. `zero`: the accumulator holds nothing, the sum is empty.
+//   16-bit results on 16-byte rows: tcgen05.ld in fragment layout, packed along rows, transposed by stmatrix into
+//     [row][column] and stored as 64-byte row pieces. One warp's 32 x 32 block costs 4 stmatrix instead of 32 stores of
+//     2 bytes a lane; the block after it is loaded meanwhile.
+//   everything else: one column per lane, each row of the block one coalesced store of 32 elements.
+template <bool kI8, bool kRaggedX>
+__device__ __forceinline__ void drain_tile(uint32_t taddr, const GroupTile& t, const GroupedArgs& a, int col, uint8_t* staging,
+                                           float* row_scales, bool zero, int lane, int first, int step) {
+    const int cols = a.cols - col;
+    if (cols <= 0 || first >= t.rows) return;
+    const int64_t out0 = (kRaggedX ? t.e * a.stride_o : 0) + static_cast<int64_t>(t.row0) * a.ldo + col;
+    const float* scale_p = kI8 ? a.scale_p + static_cast<int64_t>(t.e) * a.cols + col : nullptr;
+    if (a.out_type != TC_F32 && a.vector_out) {
+        float sp[4];
+        if (kI8) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) s[j * 32 + lane] = v[j];
-        __syncwarp();
-        float* out = static_cast<float*>(a.out) + out_index;
-        const int piece = lane & 7;
+            for (int m = 0; m < 4; ++m) {
+                const int c = 8 * m + (lane >> 2);
+                sp[m] = c < cols ? scale_p[c] : 0.f;
+            }
+        }
+        const uint32_t stage = smem_u32(staging);
+        // rows of 64 bytes, their 16-byte pieces exchanged so that neither side meets a bank twice
+        const int sr = lane & 7, sm = lane >> 3;
+        const uint32_t st_addr = stage + static_cast<uint32_t>(sr * 64 + ((sm ^ (sr >> 1)) & 3) * 16);
+        const int lr = lane >> 2, lp = lane & 3;
+        const uint8_t* ld_addr = staging + lr * 64 + ((lp ^ (lr >> 1)) & 3) * 16;
+        uint16_t* out = static_cast<uint16_t*>(a.out) + out0 + lr * a.ldo + lp * 8;
+        const int piece_cols = cols - lp * 8;
+        uint32_t r[2][16];
+        tmem_ld_16x256b_x4(taddr + static_cast<uint32_t>(first), r[0]);
+        tmem_ld_16x256b_x4(taddr + static_cast<uint32_t>(first) + (16u << 16), r[1]);
+        for (int j0 = first; j0 < t.rows; j0 += step) {
+            if (kI8) row_scales[lane] = j0 + lane < t.rows ? a.scale_q[t.row0 + j0 + lane] : 0.f;
+            tmem_ld_wait();
+            __syncwarp();   // row_scales are there; the staging area has been read
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int r = i * 4 + (lane >> 3);
-            if (r >= rows) break;
-            const float4 x = *reinterpret_cast<const float4*>(s + r * 32 + piece * 4);
-            float* dst = out + r * a.ldo + piece * 4;
-            if (a.vector_out && piece * 4 + 4 <= cols) {
-                *reinterpret_cast<float4*>(dst) = x;
-            } else {
-                const float e[4] = {x.x, x.y, x.z, x.w};
+            for (int q = 0; q < 4; ++q) {
+                uint32_t h[4];
+                float2 sq = make_float2(1.f, 1.f);
+                if (kI8) sq = *reinterpret_cast<const float2*>(row_scales + 8 * q + 2 * (lane & 3));
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (piece * 4 + j < cols) dst[j] = e[j];
+                for (int m = 0; m < 4; ++m) {
+                    const uint32_t u0 = r[m >> 1][4 * q + 2 * (m & 1)], u1 = r[m >> 1][4 * q + 2 * (m & 1) + 1];
+                    float lo, hi;
+                    if (kI8) {
+                        lo = __int2float_rn(static_cast<int>(u0)) * sq.x * sp[m];
+                        hi = __int2float_rn(static_cast<int>(u1)) * sq.y * sp[m];
+                    } else {
+                        lo = kRaggedX && zero ? 0.f : __uint_as_float(u0);
+                        hi = kRaggedX && zero ? 0.f : __uint_as_float(u1);
+                    }
+                    h[m] = pack_pair(lo, hi, a.out_type);
+                }
+                stmatrix_x4_trans(st_addr + static_cast<uint32_t>(q) * 512, h[0], h[1], h[2], h[3]);
+            }
+            if (j0 + step < t.rows) {
+                tmem_ld_16x256b_x4(taddr + static_cast<uint32_t>(j0 + step), r[0]);
+                tmem_ld_16x256b_x4(taddr + static_cast<uint32_t>(j0 + step) + (16u << 16), r[1]);
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint4 x = *reinterpret_cast<const uint4*>(ld_addr + i * 512);
+                uint16_t* dst = out + static_cast<int64_t>(j0 + i * 8) * a.ldo;
+                if (j0 + i * 8 + lr < t.rows) {
+                    if (piece_cols >= 8) {
+                        *reinterpret_cast<uint4*>(dst) = x;
+                    } else {
+                        const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (j < piece_cols) dst[j] = static_cast<uint16_t>(e[j >> 1] >> ((j & 1) * 16));
+                    }
+                }
             }
         }
     } else {
-        uint16_t* s = reinterpret_cast<uint16_t*>(stage);
+        const float sp = kI8 && lane < cols ? scale_p[lane] : 0.f;
+        for (int j0 = first; j0 < t.rows; j0 += step) {
+            uint32_t r[32];
+            if (kI8) {
+                __syncwarp();
+                row_scales[lane] = j0 + lane < t.rows ? a.scale_q[t.row0 + j0 + lane] : 0.f;
+                __syncwarp();
+            }
+            tmem_ld_x32(taddr + static_cast<uint32_t>(j0), r);
+            tmem_ld_wait();
+            if (lane >= cols) continue;
+            const int64_t at = out0 + static_cast<int64_t>(j0) * a.ldo + lane;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) s[j * 32 + lane] = to_half_bits(v[j], a.out_type);
-        __syncwarp();
-        uint16_t* out = static_cast<uint16_t*>(a.out) + out_index;
-        const int piece = lane & 3;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = i * 8 + (lane >> 2);
-            if (r >= rows) break;
-            const uint4 x = *reinterpret_cast<const uint4*>(s + r * 32 + piece * 8);
-            uint16_t* dst = out + r * a.ldo + piece * 8;
-            if (a.vector_out && piece * 8 + 8 <= cols) {
-                *reinterpret_cast<uint4*>(dst) = x;
-            } else {
-                const uint32_t e[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (piece * 8 + j < cols) dst[j] = static_cast<uint16_t>(e[j >> 1] >> ((j & 1) * 16));
+            for (int j = 0; j < 32; ++j) {
+                if (j0 + j < t.rows) {
+                    const float v = kI8 ? __int2float_rn(static_cast<int>(r[j])) * row_scales[j] * sp : kRaggedX && zero ? 0.f : __uint_as_float(r[j]);
+                    if (a.out_type == TC_F32) static_cast<float*>(a.out)[at + j * a.ldo] = v;
+                    else static_cast<uint16_t*>(a.out)[at + j * a.ldo] = to_half_bits(v, a.out_type);
+                }
             }
         }
     }
+    __syncwarp();
 }
 
 }  // namespace tcb

@@ -54,8 +54,7 @@ struct GroupedArgs {
     uint32_t* status;
 };
 
-// Fills everything but tile_rows.
-inline GroupedArgs grouped_args(const GroupedProblem& g, const DeviceInfo* dev) {
+inline GroupedArgs grouped_args(const GroupedProblem& g, int tile_rows, const DeviceInfo* dev) {
     GroupedArgs a;
     a.offsets = g.offsets;
     a.scale_p = g.scale_p;
@@ -68,7 +67,7 @@ inline GroupedArgs grouped_args(const GroupedProblem& g, const DeviceInfo* dev) 
     a.experts = static_cast<int>(g.experts);
     a.cols = static_cast<int>(g.cols);
     a.other = static_cast<int>(g.other);
-    a.tile_rows = 0;
+    a.tile_rows = tile_rows;
     a.out_type = g.out_type;
     const int es = g.out_type == TC_F32 ? 4 : 2;
     a.vector_out = aligned16(g.out) && (g.ldo * es) % 16 == 0 && (g.stride_o * es) % 16 == 0;
@@ -77,6 +76,23 @@ inline GroupedArgs grouped_args(const GroupedProblem& g, const DeviceInfo* dev) 
     return a;
 }
 
-int launch_grouped_pair(const GroupedProblem& g, const DeviceInfo* dev, cudaStream_t stream);
+// tcgen05 instruction descriptor without its N field, for M rows of the MMA (sm100.cuh: make_idesc_f16_f32). For kind::i8
+// the format fields count otherwise: D 2 = s32, A and B 1 = s8.
+uint32_t grouped_idesc(const GroupedProblem& g, int m);
+
+// Tensor maps of the operands, 128-byte swizzle: 128 bytes of the contiguous dimension by box_rows of the other one.
+int grouped_map_p(CUtensorMap* map, const GroupedProblem& g, int box_rows);
+int grouped_map_q(CUtensorMap* map, const GroupedProblem& g, int box_rows);
+
+// Which kernel runs a problem.
+struct GroupedPlan {
+    bool pair;        // grouped_pair.cu, else grouped_split.cu
+    int tile_rows;    // most rows of an output tile
+    int splits;       // pieces of x per tile (split kernel)
+    int64_t tiles;    // bound on the number of output tiles
+};
+
+int launch_grouped_pair(const GroupedProblem& g, const GroupedPlan& plan, const DeviceInfo* dev, cudaStream_t stream);
+int launch_grouped_split(const GroupedProblem& g, const GroupedPlan& plan, const DeviceInfo* dev, cudaStream_t stream);
 
 }  // namespace tcb

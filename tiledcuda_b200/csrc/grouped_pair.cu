@@ -3,8 +3,11 @@
 //   warp 0      TMA producer (both CTAs): per stage 256 bytes of x for 128 columns of P and half of the tile's rows of Q,
 //               landing in the issuing CTA's shared memory and completing on the leader's full barrier;
 //   warp 1      TMEM owner; in the leader also the MMA issuer;
-//   warps 2..5  epilogue (both CTAs): accumulator columns -> scaled -> converted -> shared memory -> rows of the output;
-//   warp 6      wgrad only: the last x block of a group holds rows of the next group, which have to count as zero
+//   warps 2..9  epilogue (both CTAs), two per TMEM lane quarter: accumulator -> scaled -> converted -> shared memory -> rows
+//               of the output. Four warps took 6500 cycles for a 128 x 256 accumulator, more than the MMAs of a short sum;
+//   warp 10     works out the CTA's tiles, 16 at a time (one per lane), into a ring in shared memory: a search and three
+//               divisions, about 1000 cycles, which the MMA issuer would otherwise spend between any two tiles;
+//   warp 11     wgrad only: the last x block of a group holds rows of the next group, which have to count as zero
 //               whatever they hold (NaN included), in both operands. The K step of the MMA is 16 rows, so up to 15 rows
 //               of each operand tile are overwritten with zeros before the MMAs read them.
 // Persistent over tiles; accumulators are double-buffered in TMEM. Which tiles there are follows from the offsets, which
@@ -19,11 +22,42 @@ constexpr int kGpStages = 3;
 constexpr int kGpOperand = 128 * 256;     // bytes of one operand per stage and CTA: 128 columns / rows x 256 bytes of x
 constexpr int kGpChunk = kGpOperand / 2;  // 128 bytes of x (x contiguous), or 64 columns / rows (those contiguous)
 constexpr int kGpStageBytes = 2 * kGpOperand;
-constexpr int kGpStaging = 4 * 4096;
-constexpr int kGpScales = 4 * 128;
+constexpr int kGpEpilogueWarps = 8;
+constexpr int kGpStaging = kGpEpilogueWarps * 2048;
+constexpr int kGpScales = kGpEpilogueWarps * 128;
+constexpr int kGpBatch = 16;              // tiles worked out at a time; the ring holds two batches
+constexpr int kGpTiles = 2 * kGpBatch * static_cast<int>(sizeof(GroupTile));
 constexpr int kGpBars = 256;
-constexpr int kGpSmem = kGpStages * kGpStageBytes + kGpStaging + kGpScales + kGpBars + static_cast<int>(sizeof(GroupTable)) + 1024;
+constexpr int kGpSmem = kGpStages * kGpStageBytes + kGpStaging + kGpScales + kGpTiles + kGpBars + static_cast<int>(sizeof(GroupTable)) + 1024;
 static_assert(kGpSmem <= 232448, "shared memory of one CTA");
+
+// A role's walk through the CTA's tiles. One thread or one converged warp each.
+struct TileCursor {
+    const GroupTile* ring;
+    uint64_t* bar_full;     // [2]: a batch has been written
+    uint64_t* bar_empty;    // [2]: every role has read the last tile of a batch
+    volatile uint32_t* abort_word;
+    int i;
+
+    // false at the end, or when a wait ran out. kWarp: all lanes call it, lane 0 arrives.
+    template <bool kWarp>
+    __device__ __forceinline__ bool next(GroupTile& t) {
+        const int half = (i / kGpBatch) & 1;
+        if (i % kGpBatch == 0) {
+            const uint32_t parity = static_cast<uint32_t>(i / (2 * kGpBatch)) & 1u;
+            const bool ok = kWarp ? mbar_wait_warp(&bar_full[half], parity, abort_word, kDevTimeoutMma)
+                                  : mbar_wait(&bar_full[half], parity, abort_word, kDevTimeoutMma);
+            if (!ok) return false;
+        }
+        t = ring[i % (2 * kGpBatch)];
+        if (i % kGpBatch == kGpBatch - 1) {
+            if (kWarp) __syncwarp();
+            if (!kWarp || (threadIdx.x & 31) == 0) mbar_arrive(&bar_empty[half]);
+        }
+        ++i;
+        return t.rows > 0;
+    }
+};
 
 __device__ __forceinline__ void umma_i8_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, bool accumulate) {
     asm volatile(
@@ -44,7 +78,7 @@ __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorM
 }
 
 template <bool kI8, bool kPCols, bool kRaggedX>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kRaggedX ? 224 : 192, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kRaggedX ? 384 : 352, 1)
 grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q,
                     const __grid_constant__ CUtensorMap tmap_q32, const GroupedArgs a) {
     constexpr int kBlockX = kI8 ? 256 : 128;   // x elements per stage
@@ -55,13 +89,16 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
     uint8_t* smem_q = smem + kGpStages * kGpOperand;
     uint8_t* staging = smem + kGpStages * kGpStageBytes;
     float* scales = reinterpret_cast<float*>(staging + kGpStaging);
-    uint64_t* bar_full = reinterpret_cast<uint64_t*>(staging + kGpStaging + kGpScales);   // used in the leader
+    GroupTile* tile_ring = reinterpret_cast<GroupTile*>(staging + kGpStaging + kGpScales);
+    uint64_t* bar_full = reinterpret_cast<uint64_t*>(staging + kGpStaging + kGpScales + kGpTiles);   // used in the leader
     uint64_t* bar_empty = bar_full + kGpStages;          // one per CTA
     uint64_t* bar_acc_full = bar_empty + kGpStages;      // one per CTA
     uint64_t* bar_acc_empty = bar_acc_full + 2;          // used in the leader
     uint64_t* bar_tail_full = bar_acc_empty + 2;         // one per CTA: a stage whose last rows have to be cleared has landed
     uint64_t* bar_tail_ready = bar_tail_full + kGpStages;   // used in the leader: both CTAs have cleared them
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_tail_ready + kGpStages);
+    uint64_t* bar_tiles_full = bar_tail_ready + kGpStages;  // one per CTA
+    uint64_t* bar_tiles_empty = bar_tiles_full + 2;         // one per CTA
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_tiles_empty + 2);
     volatile uint32_t* abort_word = tmem_slot + 1;
     GroupTable* table = reinterpret_cast<GroupTable*>(reinterpret_cast<uint8_t*>(bar_full) + kGpBars);
 
@@ -81,7 +118,9 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar_acc_full[i], 1);
-            mbar_init(&bar_acc_empty[i], 8);   // four epilogue warps in each CTA of the pair
+            mbar_init(&bar_acc_empty[i], 2 * kGpEpilogueWarps);   // of both CTAs
+            mbar_init(&bar_tiles_full[i], 1);
+            mbar_init(&bar_tiles_empty[i], 1 + kGpEpilogueWarps + (rank == 0 ? 1 : 0) + (kRaggedX ? 1 : 0));
         }
         *abort_word = 0;
         fence_barrier_init();
@@ -92,12 +131,13 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
     }
     grid_launch_dependents();
     grid_dependency_wait();   // the offsets may come from the kernel before this one
-    if (warp == 0) build_group_table(table, a, kRaggedX ? (a.other + a.tile_rows - 1) / a.tile_rows : -1, blockIdx.x == 0);
+    if (warp == 0) build_group_table<kRaggedX>(table, a, blockIdx.x == 0);
     tc_fence_before_sync();
     cluster_sync_all();   // barriers of both CTAs are initialised before anyone signals across the pair
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
-    const int num_tiles = table->tiles_before[a.experts] * col_tiles;
+    TileCursor cursor{tile_ring, bar_tiles_full, bar_tiles_empty, abort_word, 0};
+    GroupTile t;
 
     if (warp == 0) {
         // ---------------- TMA producer (both CTAs) ----------------
@@ -109,8 +149,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
-        for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
-            const GroupTile t = group_tile<kRaggedX>(table, a, tile, col_tiles, 2 * kGpCols);
+        while (ok && cursor.next<true>(t)) {
             const int blocks = (t.x_len + kBlockX - 1) / kBlockX;
             const int col = t.col0 + static_cast<int>(rank) * kGpCols;
             const int half = t.width >> 1;                              // this CTA's rows of Q
@@ -178,15 +217,15 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
             uint32_t acc_phase = 0;
             uint32_t tail_phase = 0;   // one bit per stage
             bool ok = true;
-            for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
-                const GroupTile t = group_tile<kRaggedX>(table, a, tile, col_tiles, 2 * kGpCols);
+            while (ok && cursor.next<false>(t)) {
                 const int blocks = (t.x_len + kBlockX - 1) / kBlockX;
                 const uint32_t idesc = a.idesc | (static_cast<uint32_t>(t.width >> 3) << 17);
                 if (!mbar_wait(&bar_acc_empty[acc], acc_phase ^ 1u, abort_word, kDevTimeoutMma)) break;
                 tc_fence_after_sync();
                 const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kGpRows);
+                bool landed = false;   // the next stage was seen full while the MMAs of this one were being issued
                 for (int kb = 0; kb < blocks; ++kb) {
-                    if (!mbar_wait(&bar_full[stage], phase, abort_word, kDevTimeoutMma)) {
+                    if (!landed && !mbar_wait(&bar_full[stage], phase, abort_word, kDevTimeoutMma)) {
                         ok = false;
                         break;
                     }
@@ -202,8 +241,10 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
                     const uint32_t p_lo = p_lo0 + static_cast<uint32_t>(stage) * (kGpOperand >> 4);
                     const uint32_t q_lo = q_lo0 + static_cast<uint32_t>(stage) * (kGpOperand >> 4);
                     const int steps = min(8, (rest + kStepX - 1) / kStepX);
+                    const bool wraps = stage + 1 == kGpStages;
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
+                        if (k == 4) landed = kb + 1 < blocks && mbar_test(&bar_full[wraps ? 0 : stage + 1], wraps ? phase ^ 1u : phase);
                         if (k < steps) {
                             // x contiguous: 32 bytes on in the swizzled row, the next chunk after four; else 16 rows of x on
                             const uint32_t off_p = kPCols ? k * (2048u >> 4) : static_cast<uint32_t>(((k >> 2) * kGpChunk + (k & 3) * 32) >> 4);
@@ -228,46 +269,20 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
             }
         }
         __syncwarp();
-    } else if (warp < 6) {
+    } else if (warp < 2 + kGpEpilogueWarps) {
         // ---------------- epilogue (both CTAs) ----------------
         const int quarter = warp & 3;
-        uint8_t* stage = staging + quarter * 4096;
-        float* row_scales = scales + quarter * 32;
+        uint8_t* stage = staging + (warp - 2) * 2048;
+        float* row_scales = scales + (warp - 2) * 32;
+        const int row_part = (warp - 2) >> 2;   // which of every two 32-row blocks
         int acc = 0;
         uint32_t acc_phase = 0;
-        for (int tile = pair; tile < num_tiles; tile += num_pairs) {
-            const GroupTile t = group_tile<kRaggedX>(table, a, tile, col_tiles, 2 * kGpCols);
-            const int col = t.col0 + static_cast<int>(rank) * kGpCols + quarter * 32;
-            const int cols = a.cols - col;     // columns of the output from this warp's first on
-            float sp = 1.f;
-            if (kI8 && lane < cols) sp = a.scale_p[static_cast<int64_t>(t.e) * a.cols + col + lane];
+        while (cursor.next<true>(t)) {
             if (!mbar_wait_warp(&bar_acc_full[acc], acc_phase, abort_word, kDevTimeoutEpilogue)) break;
             tc_fence_after_sync();
             const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * kGpRows);
-            if (cols > 0) {
-                for (int j0 = 0; j0 < t.rows; j0 += 32) {
-                    uint32_t r[32];
-                    float v[32];
-                    if (kI8) {
-                        const int row = j0 + lane;
-                        const float sq = row < t.rows ? a.scale_q[t.row0 + row] : 0.f;
-                        __syncwarp();
-                        row_scales[lane] = sq;
-                    }
-                    tmem_ld_x32(taddr + static_cast<uint32_t>(j0), r);
-                    tmem_ld_wait();
-                    if (kI8) {
-                        __syncwarp();
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = __int2float_rn(static_cast<int>(r[j])) * row_scales[j] * sp;
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = kRaggedX && t.x_len == 0 ? 0.f : __uint_as_float(r[j]);
-                    }
-                    const int64_t index = (kRaggedX ? t.e * a.stride_o : 0) + static_cast<int64_t>(t.row0 + j0) * a.ldo + col;
-                    store_block(v, stage, a, index, t.rows - j0, cols, lane);
-                }
-            }
+            drain_tile<kI8, kRaggedX>(taddr, t, a, t.col0 + static_cast<int>(rank) * kGpCols + quarter * 32, stage, row_scales, t.x_len == 0, lane,
+                                      row_part * 32, 64);
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&bar_acc_empty[acc]), 0));
@@ -276,12 +291,27 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
                 acc_phase ^= 1u;
             }
         }
+    } else if (warp == 2 + kGpEpilogueWarps) {
+        // ---------------- which tiles (both CTAs) ----------------
+        const int num_tiles = table->tiles_before[a.experts] * col_tiles;
+        for (int batch = 0;; ++batch) {
+            const int half = batch & 1;
+            if (batch >= 2 && !mbar_wait_warp(&bar_tiles_empty[half], (static_cast<uint32_t>(batch >> 1) & 1u) ^ 1u, abort_word, kDevTimeoutMma)) break;
+            const int64_t tile = pair + static_cast<int64_t>(batch * kGpBatch + lane) * num_pairs;
+            if (lane < kGpBatch) {
+                GroupTile g = {};   // no rows: the end
+                if (tile < num_tiles) g = group_tile<kRaggedX>(table, a, static_cast<int>(tile), col_tiles, 2 * kGpCols);
+                tile_ring[half * kGpBatch + lane] = g;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar_tiles_full[half]);
+            if (pair + static_cast<int64_t>((batch + 1) * kGpBatch - 1) * num_pairs >= num_tiles) break;   // the end marker is out
+        }
     } else if (kRaggedX) {
         // ---------------- clears the foreign rows of a group's last x block (both CTAs) ----------------
         int blocks_before = 0;
         uint32_t tail_phase = 0;
-        for (int tile = pair; tile < num_tiles; tile += num_pairs) {
-            const GroupTile t = group_tile<kRaggedX>(table, a, tile, col_tiles, 2 * kGpCols);
+        while (cursor.next<true>(t)) {
             const int blocks = (t.x_len + kBlockX - 1) / kBlockX;
             if ((t.x_len & 15) != 0) {
                 const int s = (blocks_before + blocks - 1) % kGpStages;
@@ -323,48 +353,22 @@ static int launch_variant(const CUtensorMap& tp, const CUtensorMap& tq, const CU
     auto kernel = grouped_pair_kernel<kI8, kPCols, kRaggedX>;
     static OncePerDevice once;
     if (int rc = raise_smem_limit_once(once, dev->device, kernel, kGpSmem)) return rc;
-    TCB_CUDA(launch_overlapped(kernel, dim3(2 * pairs), dim3(kRaggedX ? 224 : 192), kGpSmem, stream, tp, tq, tq32, a));
+    TCB_CUDA(launch_overlapped(kernel, dim3(2 * pairs), dim3(kRaggedX ? 384 : 352), kGpSmem, stream, tp, tq, tq32, a));
     return TC_OK;
 }
 
-int launch_grouped_pair(const GroupedProblem& g, const DeviceInfo* dev, cudaStream_t stream) {
+int launch_grouped_pair(const GroupedProblem& g, const GroupedPlan& plan, const DeviceInfo* dev, cudaStream_t stream) {
     const bool i8 = g.in_type == kTypeI8;
-    const int es = i8 ? 1 : 2;
-    const uint32_t chunk_x = 128 / es;
-    GroupedArgs a = grouped_args(g, dev);
-    a.tile_rows = kGpRows;
-    // M = 256: tcgen05 instruction descriptor, see make_idesc_f16_f32; kind::i8 counts D format 2 (s32), A and B format 1 (s8)
-    a.idesc = i8 ? (2u << 4) | (1u << 7) | (1u << 10) | (16u << 24)
-                 : make_idesc_f16_f32(2 * kGpCols, 0, g.p_c_contiguous, g.ragged_x) | (g.in_type == TC_BF16 ? kIdescBf16Inputs : 0u);
-    auto encode = [&](CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
-        return i8 ? encode_tmap_i8_sw128(out, base, rank, dims, strides, box)
-                  : encode_tmap_f16_sw128(out, base, rank, dims, strides, box, g.in_type == TC_BF16);
-    };
+    GroupedArgs a = grouped_args(g, plan.tile_rows, dev);
+    a.idesc = grouped_idesc(g, 2 * kGpCols);
     CUtensorMap tp, tq, tq32;
-    const uint64_t token_rows = static_cast<uint64_t>(g.token_rows);
-    {
-        const bool stack = !g.ragged_x;   // P is B [experts, rows, row length], or A [token_rows, cols]
-        const uint64_t inner = static_cast<uint64_t>(g.p_c_contiguous ? g.cols : g.other);
-        const uint64_t outer = stack ? static_cast<uint64_t>(g.p_c_contiguous ? g.other : g.cols) : token_rows;
-        const uint64_t dims[3] = {inner, outer, stack ? static_cast<uint64_t>(g.experts) : 1};
-        const uint64_t strides[2] = {static_cast<uint64_t>(g.ldp) * es, static_cast<uint64_t>(stack && g.experts > 1 ? g.stride_p : g.ldp) * es};
-        const uint32_t box[3] = {chunk_x, 128, 1};
-        if (int rc = encode(&tp, g.p, 3, dims, strides, box)) return rc;
-    }
-    {
-        const uint64_t dims[2] = {static_cast<uint64_t>(g.other), token_rows};
-        const uint64_t strides[1] = {static_cast<uint64_t>(g.ldq) * es};
-        const uint32_t box[2] = {chunk_x, 128};
-        const uint32_t box32[2] = {chunk_x, 32};
-        if (int rc = encode(&tq, g.q, 2, dims, strides, box)) return rc;
-        if (int rc = encode(&tq32, g.q, 2, dims, strides, box32)) return rc;
-    }
-    const int64_t col_tiles = (g.cols + 2 * kGpCols - 1) / (2 * kGpCols);
-    const int64_t most_row_tiles = g.ragged_x ? g.experts * ((g.other + kGpRows - 1) / kGpRows)
-                                              : g.token_rows / kGpRows + (g.experts < g.token_rows ? g.experts : g.token_rows);
-    if (most_row_tiles * col_tiles >= (1ll << 31)) return fail(TC_ERR_UNSUPPORTED, "grouped product: too many output tiles");
+    if (int rc = grouped_map_p(&tp, g, 128)) return rc;
+    if (int rc = grouped_map_q(&tq, g, 128)) return rc;
+    tq32 = tq;
+    if (!g.ragged_x)
+        if (int rc = grouped_map_q(&tq32, g, 32)) return rc;
     const int64_t max_pairs = dev->sm_count / 2;
-    const int pairs = static_cast<int>(most_row_tiles * col_tiles < max_pairs ? most_row_tiles * col_tiles : max_pairs);
+    const int pairs = static_cast<int>(plan.tiles < max_pairs ? plan.tiles : max_pairs);
     if (i8) return launch_variant<true, false, false>(tp, tq, tq32, a, pairs, dev, stream);
     if (g.ragged_x) return launch_variant<false, true, true>(tp, tq, tq32, a, pairs, dev, stream);
     if (g.p_c_contiguous) return launch_variant<false, true, false>(tp, tq, tq32, a, pairs, dev, stream);
