@@ -53,8 +53,7 @@ __device__ __forceinline__ int warp_inclusive_sum(int v) {
     return v;
 }
 
-// Executed by one whole warp; `report` lets one CTA of the grid record bad offsets.
-template <bool kRaggedX>
+// Executed by one whole warp (forward and dgrad); `report` lets one CTA of the grid record bad offsets.
 __device__ __forceinline__ void build_group_table(GroupTable* t, const GroupedArgs& a, bool report) {
     const int lane = threadIdx.x & 31;
     int base = 0;
@@ -67,7 +66,7 @@ __device__ __forceinline__ void build_group_table(GroupTable* t, const GroupedAr
             group_range(a, e, first, len, bad);
             t->first[e] = first;
             t->len[e] = len;
-            tiles = group_row_tiles<kRaggedX>(a, len);
+            tiles = group_row_tiles<false>(a, len);
         }
         const int sum = warp_inclusive_sum(tiles);
         if (e < a.experts) t->tiles_before[e] = base + sum - tiles;
@@ -111,6 +110,17 @@ __device__ __forceinline__ GroupTile make_group_tile(const GroupedArgs& a, int e
 constexpr int kBandCols = 8;
 
 template <bool kRaggedX>
+__device__ __forceinline__ GroupTile banded_tile(const GroupedArgs& a, int e, int first, int len, int local, int row_tiles, int col_tiles,
+                                                 int tile_cols) {
+    const int per_band = kBandCols * row_tiles;
+    const int band = local / per_band;
+    const int band_cols = min(kBandCols, col_tiles - band * kBandCols);
+    const int in_band = local - band * per_band;
+    const int rt = in_band / band_cols;
+    const int ct = band * kBandCols + in_band - rt * band_cols;
+    return make_group_tile<kRaggedX>(a, e, first, len, rt, row_tiles, ct * tile_cols);
+}
+
 __device__ __forceinline__ GroupTile group_tile(const GroupTable* t, const GroupedArgs& a, int tile, int col_tiles, int tile_cols) {
     const int row_tile_all = tile / col_tiles;
     int lo = 0, hi = a.experts - 1;          // the last group with tiles_before <= row_tile_all
@@ -120,15 +130,7 @@ __device__ __forceinline__ GroupTile group_tile(const GroupTable* t, const Group
         else hi = mid - 1;
     }
     const int before = t->tiles_before[lo];
-    const int row_tiles = t->tiles_before[lo + 1] - before;
-    const int local = tile - before * col_tiles;
-    const int per_band = kBandCols * row_tiles;
-    const int band = local / per_band;
-    const int band_cols = min(kBandCols, col_tiles - band * kBandCols);
-    const int in_band = local - band * per_band;
-    const int rt = in_band / band_cols;
-    const int ct = band * kBandCols + in_band - rt * band_cols;
-    return make_group_tile<kRaggedX>(a, lo, t->first[lo], t->len[lo], rt, row_tiles, ct * tile_cols);
+    return banded_tile<false>(a, lo, t->first[lo], t->len[lo], tile - before * col_tiles, t->tiles_before[lo + 1] - before, col_tiles, tile_cols);
 }
 
 __device__ __forceinline__ uint16_t to_half_bits(float v, int type) {

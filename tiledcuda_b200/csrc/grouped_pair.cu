@@ -7,9 +7,10 @@
 //               of the output. Four warps took 6500 cycles for a 128 x 256 accumulator, more than the MMAs of a short sum;
 //   warp 10     works out the CTA's tiles, 16 at a time (one per lane), into a ring in shared memory: a search and three
 //               divisions, about 1000 cycles, which the MMA issuer would otherwise spend between any two tiles;
-//   warp 11     wgrad only: the last x block of a group holds rows of the next group, which have to count as zero
-//               whatever they hold (NaN included), in both operands. The K step of the MMA is 16 rows, so up to 15 rows
-//               of each operand tile are overwritten with zeros before the MMAs read them.
+//   warp 11     wgrad only: the last K step (16 rows of x) of a group may hold rows of the next group, which have to count as
+//               zero whatever they hold (NaN included), in both operands. Such a step has a buffer of its own, loaded when
+//               the producer starts the tile; this warp overwrites the foreign rows with zeros long before the MMA issuer
+//               comes to it. (Cleared in the ring instead, it held up every tile by about 1000 cycles.)
 // Persistent over tiles; accumulators are double-buffered in TMEM. Which tiles there are follows from the offsets, which
 // every CTA reads from device memory into a table at the start.
 #include "grouped.cuh"
@@ -23,13 +24,22 @@ constexpr int kGpOperand = 128 * 256;     // bytes of one operand per stage and 
 constexpr int kGpChunk = kGpOperand / 2;  // 128 bytes of x (x contiguous), or 64 columns / rows (those contiguous)
 constexpr int kGpStageBytes = 2 * kGpOperand;
 constexpr int kGpEpilogueWarps = 8;
-constexpr int kGpStaging = kGpEpilogueWarps * 2048;
-constexpr int kGpScales = kGpEpilogueWarps * 128;
 constexpr int kGpBatch = 16;              // tiles worked out at a time; the ring holds two batches
-constexpr int kGpTiles = 2 * kGpBatch * static_cast<int>(sizeof(GroupTile));
-constexpr int kGpBars = 256;
-constexpr int kGpSmem = kGpStages * kGpStageBytes + kGpStaging + kGpScales + kGpTiles + kGpBars + static_cast<int>(sizeof(GroupTable)) + 1024;
-static_assert(kGpSmem <= 232448, "shared memory of one CTA");
+constexpr int kGpTailPiece = 16 * 128;    // 16 rows of x for 64 columns / rows
+constexpr int kGpTailSlot = 4 * kGpTailPiece;
+
+// Shared memory behind the ring of operand stages.
+template <bool kI8, bool kRaggedX>
+struct PairSmem {
+    static constexpr int kTail = kGpStages * kGpStageBytes;                          // wgrad: two slots
+    static constexpr int kStaging = kTail + (kRaggedX ? 2 * kGpTailSlot : 0);
+    static constexpr int kScales = kStaging + kGpEpilogueWarps * 2048;
+    static constexpr int kTiles = kScales + (kI8 ? kGpEpilogueWarps * 128 : 0);
+    static constexpr int kBars = kTiles + 2 * kGpBatch * static_cast<int>(sizeof(GroupTile));
+    static constexpr int kTable = kBars + 256;                                        // forward, dgrad
+    static constexpr int kTotal = kTable + (kRaggedX ? 0 : static_cast<int>(sizeof(GroupTable))) + 1024;
+    static_assert(kTotal <= 232448, "shared memory of one CTA");
+};
 
 // A role's walk through the CTA's tiles. One thread or one converged warp each.
 struct TileCursor {
@@ -80,27 +90,31 @@ __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorM
 template <bool kI8, bool kPCols, bool kRaggedX>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kRaggedX ? 384 : 352, 1)
 grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q,
-                    const __grid_constant__ CUtensorMap tmap_q32, const GroupedArgs a) {
+                    const __grid_constant__ CUtensorMap tmap_p_small,
+                    const __grid_constant__ CUtensorMap tmap_q_small, const GroupedArgs a) {
     constexpr int kBlockX = kI8 ? 256 : 128;   // x elements per stage
     constexpr int kStepX = kBlockX / 8;        // per MMA
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = align_smem_1024(smem_raw);
     uint8_t* smem_p = smem;
     uint8_t* smem_q = smem + kGpStages * kGpOperand;
-    uint8_t* staging = smem + kGpStages * kGpStageBytes;
-    float* scales = reinterpret_cast<float*>(staging + kGpStaging);
-    GroupTile* tile_ring = reinterpret_cast<GroupTile*>(staging + kGpStaging + kGpScales);
-    uint64_t* bar_full = reinterpret_cast<uint64_t*>(staging + kGpStaging + kGpScales + kGpTiles);   // used in the leader
+    using S = PairSmem<kI8, kRaggedX>;
+    uint8_t* smem_tail = smem + S::kTail;
+    uint8_t* staging = smem + S::kStaging;
+    float* scales = reinterpret_cast<float*>(smem + S::kScales);
+    GroupTile* tile_ring = reinterpret_cast<GroupTile*>(smem + S::kTiles);
+    uint64_t* bar_full = reinterpret_cast<uint64_t*>(smem + S::kBars);   // used in the leader
     uint64_t* bar_empty = bar_full + kGpStages;          // one per CTA
     uint64_t* bar_acc_full = bar_empty + kGpStages;      // one per CTA
     uint64_t* bar_acc_empty = bar_acc_full + 2;          // used in the leader
-    uint64_t* bar_tail_full = bar_acc_empty + 2;         // one per CTA: a stage whose last rows have to be cleared has landed
-    uint64_t* bar_tail_ready = bar_tail_full + kGpStages;   // used in the leader: both CTAs have cleared them
-    uint64_t* bar_tiles_full = bar_tail_ready + kGpStages;  // one per CTA
-    uint64_t* bar_tiles_empty = bar_tiles_full + 2;         // one per CTA
+    uint64_t* bar_tail_full = bar_acc_empty + 2;         // one per CTA: its part of a last step has landed
+    uint64_t* bar_tail_ready = bar_tail_full + 2;        // used in the leader: both CTAs have cleared the foreign rows
+    uint64_t* bar_tail_empty = bar_tail_ready + 2;       // one per CTA
+    uint64_t* bar_tiles_full = bar_tail_empty + 2;       // one per CTA
+    uint64_t* bar_tiles_empty = bar_tiles_full + 2;      // one per CTA
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_tiles_empty + 2);
     volatile uint32_t* abort_word = tmem_slot + 1;
-    GroupTable* table = reinterpret_cast<GroupTable*>(reinterpret_cast<uint8_t*>(bar_full) + kGpBars);
+    GroupTable* table = reinterpret_cast<GroupTable*>(smem + S::kTable);
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int lane = threadIdx.x & 31;
@@ -113,10 +127,11 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
         for (int s = 0; s < kGpStages; ++s) {
             mbar_init(&bar_full[s], 1);
             mbar_init(&bar_empty[s], 1);
-            mbar_init(&bar_tail_full[s], 1);
-            mbar_init(&bar_tail_ready[s], 2);
         }
         for (int i = 0; i < 2; ++i) {
+            mbar_init(&bar_tail_full[i], 1);
+            mbar_init(&bar_tail_ready[i], 2);
+            mbar_init(&bar_tail_empty[i], 1);
             mbar_init(&bar_acc_full[i], 1);
             mbar_init(&bar_acc_empty[i], 2 * kGpEpilogueWarps);   // of both CTAs
             mbar_init(&bar_tiles_full[i], 1);
@@ -131,7 +146,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
     }
     grid_launch_dependents();
     grid_dependency_wait();   // the offsets may come from the kernel before this one
-    if (warp == 0) build_group_table<kRaggedX>(table, a, blockIdx.x == 0);
+    if (!kRaggedX && warp == 0) build_group_table(table, a, blockIdx.x == 0);
     tc_fence_before_sync();
     cluster_sync_all();   // barriers of both CTAs are initialised before anyone signals across the pair
     tc_fence_after_sync();
@@ -149,36 +164,44 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
+        int tails = 0;
         while (ok && cursor.next<true>(t)) {
-            const int blocks = (t.x_len + kBlockX - 1) / kBlockX;
+            const int x_len = kRaggedX ? t.x_len & ~15 : t.x_len;   // what the ring carries
+            const int blocks = (x_len + kBlockX - 1) / kBlockX;
             const int col = t.col0 + static_cast<int>(rank) * kGpCols;
             const int half = t.width >> 1;                              // this CTA's rows of Q
             const int row = t.row0 + static_cast<int>(rank) * half;
+            if (kRaggedX && x_len != t.x_len) {
+                const int slot = tails & 1;
+                if (!mbar_wait_warp(&bar_tail_empty[slot], (static_cast<uint32_t>(tails >> 1) & 1u) ^ 1u, abort_word, kDevTimeoutProducer)) break;
+                if (leader) {
+                    const uint32_t bar_addr = map_to_cta(smem_u32(&bar_tail_full[slot]), rank);
+                    uint8_t* dst = smem_tail + slot * kGpTailSlot;
+                    mbar_arrive_expect_tx(&bar_tail_full[slot], kGpTailSlot);
+                    for (int c = 0; c < 2; ++c) {
+                        tma_load_3d_pair(dst + c * kGpTailPiece, &tmap_p_small, bar_addr, col + c * 64, t.x0 + x_len, 0);
+                        tma_load_2d_pair(dst + (2 + c) * kGpTailPiece, &tmap_q_small, bar_addr, row + c * 64, t.x0 + x_len);
+                    }
+                }
+                ++tails;
+            }
             for (int kb = 0; kb < blocks; ++kb) {
                 if (!mbar_wait_warp(&bar_empty[stage], phase ^ 1u, abort_word, kDevTimeoutProducer)) {
                     ok = false;
                     break;
                 }
                 const int x = kb * kBlockX;
-                const int chunks = t.x_len - x > kBlockX / 2 ? 2 : 1;   // 128-byte pieces of x
+                const int chunks = x_len - x > kBlockX / 2 ? 2 : 1;      // 128-byte pieces of x
                 const int q_boxes = (half + 31) >> 5;
                 const bool whole_q = t.width == kGpRows;
                 const bool two_rows = half > 64;                         // wgrad: 64-row pieces of Q
-                const bool tail = kRaggedX && kb == blocks - 1 && (t.x_len & 15) != 0;
                 const uint32_t p_bytes = kPCols ? kGpOperand : chunks * kGpChunk;
                 const uint32_t q_bytes = kRaggedX ? (two_rows ? kGpOperand : kGpChunk) : chunks * (whole_q ? kGpChunk : q_boxes * 4096);
-                uint64_t* bar = tail ? &bar_tail_full[stage] : &bar_full[stage];
-                // full counts the bytes of both CTAs, in the leader; a tail counts its own in each
-                const uint32_t bar_addr = map_to_cta(smem_u32(bar), tail ? rank : 0);
+                const uint32_t bar_addr = map_to_cta(smem_u32(&bar_full[stage]), 0);   // counts the bytes of both CTAs
                 uint8_t* dst_p = smem_p + stage * kGpOperand;
                 uint8_t* dst_q = smem_q + stage * kGpOperand;
                 if (leader) {
-                    if (tail) {
-                        mbar_arrive_expect_tx(bar, p_bytes + q_bytes);
-                        if (rank == 0) mbar_arrive(&bar_full[stage]);
-                    } else if (rank == 0) {
-                        mbar_arrive_expect_tx(bar, 2 * (p_bytes + q_bytes));
-                    }
+                    if (rank == 0) mbar_arrive_expect_tx(&bar_full[stage], 2 * (p_bytes + q_bytes));
                     if (kPCols) {
                         const int y = kRaggedX ? t.x0 + x : x;
                         const int z = kRaggedX ? 0 : t.e;
@@ -195,7 +218,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
                     } else {
                         for (int c = 0; c < chunks; ++c)
                             for (int b = 0; b < q_boxes; ++b)
-                                tma_load_2d_pair(dst_q + c * kGpChunk + b * 4096, &tmap_q32, bar_addr, x + c * (kBlockX / 2), row + b * 32);
+                                tma_load_2d_pair(dst_q + c * kGpChunk + b * 4096, &tmap_q_small, bar_addr, x + c * (kBlockX / 2), row + b * 32);
                     }
                 }
                 if (++stage == kGpStages) {
@@ -215,10 +238,11 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
             uint32_t phase = 0;
             int acc = 0;
             uint32_t acc_phase = 0;
-            uint32_t tail_phase = 0;   // one bit per stage
+            int tails = 0;
             bool ok = true;
             while (ok && cursor.next<false>(t)) {
-                const int blocks = (t.x_len + kBlockX - 1) / kBlockX;
+                const int x_len = kRaggedX ? t.x_len & ~15 : t.x_len;
+                const int blocks = (x_len + kBlockX - 1) / kBlockX;
                 const uint32_t idesc = a.idesc | (static_cast<uint32_t>(t.width >> 3) << 17);
                 if (!mbar_wait(&bar_acc_empty[acc], acc_phase ^ 1u, abort_word, kDevTimeoutMma)) break;
                 tc_fence_after_sync();
@@ -229,14 +253,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
                         ok = false;
                         break;
                     }
-                    const int rest = t.x_len - kb * kBlockX;
-                    if (kRaggedX && rest <= kBlockX && (rest & 15) != 0) {
-                        if (!mbar_wait_cluster(&bar_tail_ready[stage], (tail_phase >> stage) & 1u, abort_word, kDevTimeoutMma)) {
-                            ok = false;
-                            break;
-                        }
-                        tail_phase ^= 1u << stage;
-                    }
+                    const int rest = x_len - kb * kBlockX;
                     tc_fence_after_sync();
                     const uint32_t p_lo = p_lo0 + static_cast<uint32_t>(stage) * (kGpOperand >> 4);
                     const uint32_t q_lo = q_lo0 + static_cast<uint32_t>(stage) * (kGpOperand >> 4);
@@ -261,6 +278,15 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
                     }
                 }
                 if (!ok) break;
+                if (kRaggedX && x_len != t.x_len) {
+                    const int slot = tails & 1;
+                    if (!mbar_wait_cluster(&bar_tail_ready[slot], static_cast<uint32_t>(tails >> 1) & 1u, abort_word, kDevTimeoutMma)) break;
+                    tc_fence_after_sync();
+                    const uint32_t lo = smem_desc_lo(smem_u32(smem_tail), kGpTailPiece) + static_cast<uint32_t>(slot) * (kGpTailSlot >> 4);
+                    umma_f16_ss_pair(d_tmem, smem_desc_join(lo, desc_hi), smem_desc_join(lo + (2 * kGpTailPiece >> 4), desc_hi), idesc, blocks > 0);
+                    umma_commit_pair_both(smem_u32(&bar_tail_empty[slot]));
+                    ++tails;
+                }
                 umma_commit_pair_both(smem_u32(&bar_acc_full[acc]));
                 if (++acc == 2) {
                     acc = 0;
@@ -293,46 +319,49 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
         }
     } else if (warp == 2 + kGpEpilogueWarps) {
         // ---------------- which tiles (both CTAs) ----------------
-        const int num_tiles = table->tiles_before[a.experts] * col_tiles;
+        const int row_tiles = group_row_tiles<kRaggedX>(a, 0);   // wgrad: of every group
+        const int num_tiles = (kRaggedX ? a.experts * row_tiles : table->tiles_before[a.experts]) * col_tiles;
+        bool bad = false;
         for (int batch = 0;; ++batch) {
             const int half = batch & 1;
             if (batch >= 2 && !mbar_wait_warp(&bar_tiles_empty[half], (static_cast<uint32_t>(batch >> 1) & 1u) ^ 1u, abort_word, kDevTimeoutMma)) break;
             const int64_t tile = pair + static_cast<int64_t>(batch * kGpBatch + lane) * num_pairs;
             if (lane < kGpBatch) {
                 GroupTile g = {};   // no rows: the end
-                if (tile < num_tiles) g = group_tile<kRaggedX>(table, a, static_cast<int>(tile), col_tiles, 2 * kGpCols);
+                if (tile < num_tiles) {
+                    if (kRaggedX) {
+                        const int per_group = row_tiles * col_tiles;
+                        const int e = static_cast<int>(tile) / per_group;
+                        int first, len;
+                        group_range(a, e, first, len, bad);
+                        g = banded_tile<true>(a, e, first, len, static_cast<int>(tile) - e * per_group, row_tiles, col_tiles, 2 * kGpCols);
+                    } else {
+                        g = group_tile(table, a, static_cast<int>(tile), col_tiles, 2 * kGpCols);
+                    }
+                }
                 tile_ring[half * kGpBatch + lane] = g;
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar_tiles_full[half]);
             if (pair + static_cast<int64_t>((batch + 1) * kGpBatch - 1) * num_pairs >= num_tiles) break;   // the end marker is out
         }
+        if (bad) atomicMax(a.status, static_cast<uint32_t>(kDevIndexOutOfRange));
     } else if (kRaggedX) {
-        // ---------------- clears the foreign rows of a group's last x block (both CTAs) ----------------
-        int blocks_before = 0;
-        uint32_t tail_phase = 0;
+        // ---------------- clears the foreign rows of last steps (both CTAs) ----------------
+        int tails = 0;
         while (cursor.next<true>(t)) {
-            const int blocks = (t.x_len + kBlockX - 1) / kBlockX;
-            if ((t.x_len & 15) != 0) {
-                const int s = (blocks_before + blocks - 1) % kGpStages;
-                if (!mbar_wait_warp(&bar_tail_full[s], (tail_phase >> s) & 1u, abort_word, kDevTimeoutMma)) break;
-                tail_phase ^= 1u << s;
-                const int first = t.x_len - (blocks - 1) * kBlockX;
-                const int n = ((first + 15) & ~15) - first;      // rows of 128 bytes in each of the four 64-wide pieces
-                uint8_t* p = smem_p + s * kGpOperand;
-                uint8_t* q = smem_q + s * kGpOperand;
-                for (int i = lane; i < n * 8; i += 32) {
-                    const int at = (first + (i >> 3)) * 128 + (i & 7) * 16;
-                    *reinterpret_cast<uint4*>(p + at) = make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4*>(p + kGpChunk + at) = make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4*>(q + at) = make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4*>(q + kGpChunk + at) = make_uint4(0, 0, 0, 0);
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&bar_tail_ready[s]), 0));
-            }
-            blocks_before += blocks;
+            const int first = t.x_len & 15;
+            if (first == 0) continue;
+            const int slot = tails & 1;
+            if (!mbar_wait_warp(&bar_tail_full[slot], static_cast<uint32_t>(tails >> 1) & 1u, abort_word, kDevTimeoutMma)) break;
+            ++tails;
+            uint8_t* p = smem_tail + slot * kGpTailSlot + first * 128;
+            for (int i = lane; i < (16 - first) * 8; i += 32)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4*>(p + c * kGpTailPiece + i * 16) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&bar_tail_ready[slot]), 0));
         }
     }
 
@@ -348,12 +377,13 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
 }
 
 template <bool kI8, bool kPCols, bool kRaggedX>
-static int launch_variant(const CUtensorMap& tp, const CUtensorMap& tq, const CUtensorMap& tq32, const GroupedArgs& a, int pairs,
-                          const DeviceInfo* dev, cudaStream_t stream) {
+static int launch_variant(const CUtensorMap& tp, const CUtensorMap& tq, const CUtensorMap& tp_small, const CUtensorMap& tq_small,
+                          const GroupedArgs& a, int pairs, const DeviceInfo* dev, cudaStream_t stream) {
     auto kernel = grouped_pair_kernel<kI8, kPCols, kRaggedX>;
+    constexpr int smem = PairSmem<kI8, kRaggedX>::kTotal;
     static OncePerDevice once;
-    if (int rc = raise_smem_limit_once(once, dev->device, kernel, kGpSmem)) return rc;
-    TCB_CUDA(launch_overlapped(kernel, dim3(2 * pairs), dim3(kRaggedX ? 384 : 352), kGpSmem, stream, tp, tq, tq32, a));
+    if (int rc = raise_smem_limit_once(once, dev->device, kernel, smem)) return rc;
+    TCB_CUDA(launch_overlapped(kernel, dim3(2 * pairs), dim3(kRaggedX ? 384 : 352), smem, stream, tp, tq, tp_small, tq_small, a));
     return TC_OK;
 }
 
@@ -361,18 +391,22 @@ int launch_grouped_pair(const GroupedProblem& g, const GroupedPlan& plan, const 
     const bool i8 = g.in_type == kTypeI8;
     GroupedArgs a = grouped_args(g, plan.tile_rows, dev);
     a.idesc = grouped_idesc(g, 2 * kGpCols);
-    CUtensorMap tp, tq, tq32;
+    // 128-row boxes; of Q also 32-row ones for tiles of fewer rows, or (wgrad) 16 rows of x of both for a group's last step
+    CUtensorMap tp, tq, tp_small, tq_small;
     if (int rc = grouped_map_p(&tp, g, 128)) return rc;
     if (int rc = grouped_map_q(&tq, g, 128)) return rc;
-    tq32 = tq;
-    if (!g.ragged_x)
-        if (int rc = grouped_map_q(&tq32, g, 32)) return rc;
+    if (int rc = grouped_map_q(&tq_small, g, g.ragged_x ? 16 : 32)) return rc;
+    if (g.ragged_x) {
+        if (int rc = grouped_map_p(&tp_small, g, 16)) return rc;
+    } else {
+        tp_small = tp;
+    }
     const int64_t max_pairs = dev->sm_count / 2;
     const int pairs = static_cast<int>(plan.tiles < max_pairs ? plan.tiles : max_pairs);
-    if (i8) return launch_variant<true, false, false>(tp, tq, tq32, a, pairs, dev, stream);
-    if (g.ragged_x) return launch_variant<false, true, true>(tp, tq, tq32, a, pairs, dev, stream);
-    if (g.p_c_contiguous) return launch_variant<false, true, false>(tp, tq, tq32, a, pairs, dev, stream);
-    return launch_variant<false, false, false>(tp, tq, tq32, a, pairs, dev, stream);
+    if (i8) return launch_variant<true, false, false>(tp, tq, tp_small, tq_small, a, pairs, dev, stream);
+    if (g.ragged_x) return launch_variant<false, true, true>(tp, tq, tp_small, tq_small, a, pairs, dev, stream);
+    if (g.p_c_contiguous) return launch_variant<false, true, false>(tp, tq, tp_small, tq_small, a, pairs, dev, stream);
+    return launch_variant<false, false, false>(tp, tq, tp_small, tq_small, a, pairs, dev, stream);
 }
 
 }  // namespace tcb
