@@ -93,25 +93,53 @@ int grouped_map_q(CUtensorMap* map, const GroupedProblem& g, int box_rows) {
     return encode_operand(map, g.q, 2, dims, strides, box, g.in_type);
 }
 
-#ifdef TCB_TUNE
-int g_force_pair = -1, g_force_rows = 0, g_force_splits = 0;
-extern "C" void tc_tune(int pair, int rows, int splits) { g_force_pair = pair; g_force_rows = rows; g_force_splits = splits; }
-#endif
-
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// The kernel and tile for a problem, from its sizes alone; of the offsets the host knows nothing, so the rule takes the
+// rows to be spread evenly. Times below in us: B200, CUDA graph replays, three sets of operands in turn.
+//  * Pair tiles (256 columns x up to 256 rows) once there are enough of them for the 74 pairs and the groups have 128
+//    rows or more to fill them: 32 experts x [4096,1024] with 4096 rows 59 against 69 in the split kernel, weight gradient
+//    of 16 x [2048,1024] 31 against 48. With 64 tiles the split kernel is ahead for one dense product (int8 2048^3 10.8
+//    against 12.2), the pair kernel where each group brings its own weights (8 x [2048,1024], 2048 rows: 18.4 against 19.3).
+//  * Else the split kernel. Where the weights' bytes count (few rows per group), a tile takes all rows of a group up to
+//    four times the even share, so that a popular expert's weights are read once: 16 x [2048,2048] with 512 rows 25
+//    with 128-row tiles against 30 with 32.
+//  * Tiles are halved while they still all run at once, one per SM: int8 1024^3 4.4 with 64 rows, 5.4 with 128; for long
+//    sums not below 64 rows, where cutting the sum does more: int8 300 x 1024 x 8192 9.4 with two pieces of 64-row
+//    tiles, 10.8 with 32-row tiles.
+//  * The sum is cut while SMs are idle and a piece keeps eight stages: int8 1 x 4096 x 4096 5.9 in four pieces, 6.7 in one.
+//    Clusters of eight only for a handful of tiles: a GPC holds two of them at most, and a weight gradient of 512 x 512
+//    from 4096 rows took 17.2 in eight pieces and 9.2 in four.
 static GroupedPlan grouped_plan(const GroupedProblem& g, int sm_count) {
+    const int64_t groups = g.offsets == nullptr ? 1 : g.ragged_x ? g.experts : (g.experts < g.token_rows ? g.experts : g.token_rows);
+    const int64_t share = ceil_div(g.token_rows, groups);               // rows of a group, spread evenly
+    const int64_t rows = g.ragged_x ? g.other : share;                   // extent of an output slice
+    const int64_t stages = ceil_div((g.ragged_x ? share : g.other) * (g.in_type == kTypeI8 ? 1 : 2), 128);   // of the split kernel
+    auto tiles = [&](int64_t tile_rows, int64_t tile_cols) { return groups * ceil_div(rows, tile_rows) * ceil_div(g.cols, tile_cols); };
     GroupedPlan p;
-    p.pair = true;
-    p.tile_rows = 256;
     p.splits = 1;
-#ifdef TCB_TUNE
-    if (g_force_pair >= 0 && !(g.ragged_x && g_force_rows < 64)) { p.pair = g_force_pair; p.tile_rows = g_force_rows; p.splits = g_force_splits; }
-#endif
-    const int64_t row_tiles = g.ragged_x ? g.experts * ceil_div(g.other, p.tile_rows)
-                              : g.offsets == nullptr ? ceil_div(g.token_rows, p.tile_rows)
-                                         : g.token_rows / p.tile_rows + (g.experts < g.token_rows ? g.experts : g.token_rows);
+    const bool own_weights = groups > 1 && !g.ragged_x;
+    p.pair = rows >= 128 && tiles(256, 256) >= (own_weights ? 64 : 100);
+    if (p.pair) {
+        p.tile_rows = 256;
+    } else {
+        const int64_t want = own_weights ? 4 * share : rows;
+        p.tile_rows = g.ragged_x ? 64 : 16;
+        while (p.tile_rows < 128 && p.tile_rows < want) p.tile_rows *= 2;
+        const int64_t least = g.ragged_x || stages > 16 ? 64 : 32;
+        while (p.tile_rows > least && tiles(p.tile_rows / 2, 128) <= sm_count && (!own_weights || share > 128 || p.tile_rows / 2 >= share))
+            p.tile_rows /= 2;
+        const int64_t n = tiles(p.tile_rows, 128);
+        const int64_t room = own_weights ? sm_count / 2 : sm_count;   // uneven groups make more tiles than counted here
+        while (p.splits < 8 && 2 * p.splits * n <= (p.splits == 4 ? 64 : room) && stages >= 16 * p.splits) p.splits *= 2;
+    }
+    // a bound on the output tiles for any offsets that do not overlap
+    const int64_t row_tiles = g.ragged_x ? groups * ceil_div(g.other, p.tile_rows)
+                              : g.offsets == nullptr ? ceil_div(g.token_rows, p.tile_rows) : g.token_rows / p.tile_rows + groups;
     p.tiles = row_tiles * ceil_div(g.cols, p.pair ? 256 : 128);
+    // The split kernel's CTAs get an SM each, and the ring of one, when they need no more: a few beyond the SMs, of which
+    // some will find no tile, do not change that (9 experts x [1001,776], 1333 rows: 152 CTAs 10.8 alone, 14.3 two to an SM).
+    p.alone = tiles(p.tile_rows, 128) * p.splits <= sm_count && 10 * p.tiles * p.splits <= 11 * sm_count;
     return p;
 }
 

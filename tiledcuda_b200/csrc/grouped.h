@@ -90,6 +90,7 @@ struct GroupedPlan {
     int tile_rows;    // most rows of an output tile
     int splits;       // pieces of x per tile (split kernel)
     int64_t tiles;    // bound on the number of output tiles
+    bool alone;       // one CTA per SM (split kernel)
 };
 
 int launch_grouped_pair(const GroupedProblem& g, const GroupedPlan& plan, const DeviceInfo* dev, cudaStream_t stream);

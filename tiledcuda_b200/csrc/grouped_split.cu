@@ -3,7 +3,7 @@
 //   warp 0      TMA producer: per stage 128 bytes of x for 128 columns of P and the tile's rows of Q;
 //   warp 1      TMEM owner and MMA issuer (M = 128, N = rows of the tile rounded up); for wgrad it also clears the rows
 //               of the next group in the last x block before the MMAs read them;
-//   warps 2..5  epilogue.
+//   warps 2..9  epilogue, two per TMEM lane quarter.
 // With one or a few rows per group the work is reading P once. Two CTAs fit on an SM, so that one streams while the other
 // starts or drains. Partial sums are added in rank order: the result does not change from run to run, no workspace and no
 // atomics are needed.
@@ -12,6 +12,8 @@
 namespace tcb {
 
 constexpr int kGsCols = 128;
+constexpr int kGsEpilogueWarps = 8;
+constexpr int kGsThreads = 64 + 32 * kGsEpilogueWarps;
 constexpr int kGsP = 128 * 128;                 // bytes of P per stage
 constexpr int kGsRing = 108 * 1024;             // bytes of the ring where two CTAs share an SM
 constexpr int kGsRingAlone = 216 * 1024;        // and where the grid leaves each its own
@@ -138,7 +140,7 @@ __device__ __forceinline__ GroupTile find_tile(const GroupedArgs& a, int tile, i
 }
 
 template <bool kI8, bool kPCols, bool kRaggedX>
-__global__ void __launch_bounds__(192, 2)
+__global__ void __launch_bounds__(kGsThreads, 2)
 grouped_split_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q, const GroupedArgs a,
                      int splits, int ring_bytes) {
     constexpr int kBlockX = kI8 ? 128 : 64;   // x elements per stage
@@ -269,8 +271,9 @@ grouped_split_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
     }
 
     // ---------------- epilogue ----------------
-    // warps 2..5 read the TMEM lanes of their quarter: one output column per thread
+    // a warp reads the TMEM lanes of its quarter, the two of a quarter take turns at blocks of 32 rows
     const int quarter = warp & 3;
+    const int part_of_rows = (warp - 2) >> 2;
     const bool drains = warp >= 2;
     const bool summed = block1 > block0;   // else this CTA's part is zero
     const bool ok = drains && t.rows > 0 && mbar_wait_warp(bar_acc, 0, abort_word, kDevTimeoutEpilogue);
@@ -278,13 +281,14 @@ grouped_split_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
     const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     const int64_t out0 = (kRaggedX ? t.e * a.stride_o : 0) + static_cast<int64_t>(t.row0) * a.ldo;
     if (splits == 1) {
-        if (ok) drain_tile<kI8, kRaggedX>(taddr, t, a, t.col0 + quarter * 32, ring + 4096 + quarter * 2048, scales + quarter * 32, !summed, lane, 0, 32);
+        if (ok) drain_tile<kI8, kRaggedX>(taddr, t, a, t.col0 + quarter * 32, ring + 4096 + (warp - 2) * 2048, scales + (warp - 2) * 32,
+                                          !summed, lane, part_of_rows * 32, 64);
     } else {
         // raw partial sums [row][column] into shared memory (every MMA of this CTA has read the ring), then rank s adds up and
         // writes its share of the rows
         uint32_t* part = reinterpret_cast<uint32_t*>(ring);
         if (ok) {
-            for (int j0 = 0; j0 < t.rows; j0 += 32) {
+            for (int j0 = part_of_rows * 32; j0 < t.rows; j0 += 64) {
                 uint32_t r[32];
                 tmem_ld_x32(taddr + static_cast<uint32_t>(j0), r);
                 tmem_ld_wait();
@@ -296,7 +300,7 @@ grouped_split_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
         __syncwarp();
         cluster_sync_all();
         if (ok) {
-            // a thread takes four columns of every fourth row of the share, two rows at a time
+            // a warp takes every eighth row of the share, two at a time, four columns a thread
             const int share = (t.rows + splits - 1) / splits;
             const int end = min(t.rows, (rank + 1) * share);
             const int my_col = t.col0 + lane * 4;
@@ -309,20 +313,20 @@ grouped_split_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
             }
             constexpr uint32_t kRow = kGsCols * 4;
             const uint32_t mine = smem_u32(part) + static_cast<uint32_t>(lane) * 16;
-            for (int row = rank * share + quarter; row < end; row += 8) {
+            for (int row = rank * share + warp - 2; row < end; row += 2 * kGsEpilogueWarps) {
                 float v[2][4];
-                const bool two = row + 4 < end;
+                const bool two = row + kGsEpilogueWarps < end;
                 // the second row, where there is none, is read from the first one's place
-                sum_partials<kI8, 2>(mine + static_cast<uint32_t>(row) * kRow, two ? 4 * kRow : 0, splits, v);
+                sum_partials<kI8, 2>(mine + static_cast<uint32_t>(row) * kRow, two ? kGsEpilogueWarps * kRow : 0, splits, v);
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     if (r == 1 && !two) break;
                     if (kI8) {
-                        const float sq = a.scale_q[t.row0 + row + 4 * r];
+                        const float sq = a.scale_q[t.row0 + row + kGsEpilogueWarps * r];
 #pragma unroll
                         for (int j = 0; j < 4; ++j) v[r][j] = v[r][j] * sq * sp4[j];
                     }
-                    if (cols > 0) store_four(a, out0 + (row + 4 * r) * a.ldo + my_col, v[r], cols);
+                    if (cols > 0) store_four(a, out0 + (row + kGsEpilogueWarps * r) * a.ldo + my_col, v[r], cols);
                 }
             }
         }
@@ -342,27 +346,27 @@ grouped_split_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
 }
 
 template <bool kI8, bool kPCols, bool kRaggedX>
-static int launch_variant(const CUtensorMap& tp, const CUtensorMap& tq, const GroupedArgs& a, int64_t tiles, int splits, const DeviceInfo* dev,
+static int launch_variant(const CUtensorMap& tp, const CUtensorMap& tq, const GroupedArgs& a, const GroupedPlan& plan, const DeviceInfo* dev,
                           cudaStream_t stream) {
     auto kernel = grouped_split_kernel<kI8, kPCols, kRaggedX>;
     static OncePerDevice once;
     if (int rc = raise_smem_limit_once(once, dev->device, kernel, gs_smem(kGsRingAlone))) return rc;
-    const int ring = tiles * splits <= dev->sm_count ? kGsRingAlone : kGsRing;
+    const int ring = plan.alone ? kGsRingAlone : kGsRing;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(tiles * splits));
-    cfg.blockDim = dim3(192);
+    cfg.gridDim = dim3(static_cast<unsigned>(plan.tiles * plan.splits));
+    cfg.blockDim = dim3(kGsThreads);
     cfg.dynamicSmemBytes = static_cast<size_t>(gs_smem(ring));
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = static_cast<unsigned>(splits);
+    attr[1].val.clusterDim.x = static_cast<unsigned>(plan.splits);
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = splits > 1 ? 2 : 1;
-    TCB_CUDA(cudaLaunchKernelEx(&cfg, kernel, tp, tq, a, splits, ring));
+    cfg.numAttrs = plan.splits > 1 ? 2 : 1;
+    TCB_CUDA(cudaLaunchKernelEx(&cfg, kernel, tp, tq, a, plan.splits, ring));
     return TC_OK;
 }
 
@@ -374,10 +378,10 @@ int launch_grouped_split(const GroupedProblem& g, const GroupedPlan& plan, const
     // P: 128 columns by 128 bytes of x, or (columns contiguous) 64 columns by 64 x; Q: the tile's rows alike
     if (int rc = grouped_map_p(&tp, g, g.p_c_contiguous ? 64 : 128)) return rc;
     if (int rc = grouped_map_q(&tq, g, g.ragged_x ? 64 : plan.tile_rows)) return rc;
-    if (i8) return launch_variant<true, false, false>(tp, tq, a, plan.tiles, plan.splits, dev, stream);
-    if (g.ragged_x) return launch_variant<false, true, true>(tp, tq, a, plan.tiles, plan.splits, dev, stream);
-    if (g.p_c_contiguous) return launch_variant<false, true, false>(tp, tq, a, plan.tiles, plan.splits, dev, stream);
-    return launch_variant<false, false, false>(tp, tq, a, plan.tiles, plan.splits, dev, stream);
+    if (i8) return launch_variant<true, false, false>(tp, tq, a, plan, dev, stream);
+    if (g.ragged_x) return launch_variant<false, true, true>(tp, tq, a, plan, dev, stream);
+    if (g.p_c_contiguous) return launch_variant<false, true, false>(tp, tq, a, plan, dev, stream);
+    return launch_variant<false, false, false>(tp, tq, a, plan, dev, stream);
 }
 
 }  // namespace tcb
