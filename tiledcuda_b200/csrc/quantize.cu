@@ -1,5 +1,7 @@
 // Rounding of rows to 8-bit integers with one scale per row: scale = max(amax / 127, 2^-126), q = x / scale to nearest,
-// ties to even. One block per row, the row read twice.
+// ties to even. Bound by memory: each element is read once (2 or 4 bytes) and written once (1 byte). A row stays in the
+// registers of the threads that own it between the maximum and the rounding; rows too long for that, or not on
+// 16-byte boundaries, are read a second time (out of L2).
 #include "host.h"
 #include "sm100.cuh"
 
@@ -8,57 +10,265 @@
 namespace tcb {
 
 constexpr int kQuantThreads = 256;
+constexpr int kQuantChunk = 16;   // consecutive elements of a thread: 16 bytes of q
 
-// x / scale rounded as the exact quotient would be. x * (1 / scale) is off by less than 2e-5 for quotients up to 127
-// (two roundings of 2^-24 each), so only a quotient within 1e-4 of a half can round the other way; there x is compared
-// with half * scale, a product of 9 and 24 significant bits that is exact in fp64.
-__device__ __forceinline__ float quantize_value(float x, float inv, float scale) {
-    const float t = x * inv;
-    float r = rintf(t);
-    if (fabsf(fabsf(t - r) - 0.5f) < 1e-4f) {
-        const float low = floorf(t);
-        const double border = (static_cast<double>(low) + 0.5) * static_cast<double>(scale);
-        const double xd = static_cast<double>(x);
-        if (xd > border) r = low + 1.f;
-        else if (xd < border) r = low;
-        else r = 2.f * rintf(0.5f * low + 0.25f);   // the even one of low and low + 1
-    }
-    return r;
+// x / scale rounded as the exact quotient would be. r, the rounded x * (1 / scale), is off by one at most, and only where the
+// quotient is within 1e-5 of a half-integer (the reciprocal's rounding times 127.5). e = x - r * scale tells: it comes out of one
+// fma, exact near |e| = scale / 2, where x and r * scale cancel to 24 bits (or is a half-step above it next to r = 1, where a
+// tie and a larger |e| lead to the same answer). r is right if |e| < scale / 2, and a tie goes to the even neighbour. Exact
+// ties are not rare: bf16 rows hold x = amax / 2 once in a few thousand elements.
+constexpr float kToInteger = 12582912.f;   // 1.5 * 2^23: added, it leaves the value rounded to an integer in the low mantissa bits
+
+__device__ __forceinline__ float settle(float r, float e, float half) {
+    const bool wrong = fabsf(e) > half || (fabsf(e) == half && (__float_as_uint(r + kToInteger) & 1u));
+    return wrong ? r + copysignf(1.f, e) : r;
 }
+
+__device__ __forceinline__ int8_t quantize_one(float x, float inv, float scale) {
+    const float r = fmaf(x, inv, kToInteger) - kToInteger;
+    return static_cast<int8_t>(settle(r, fmaf(-r, scale, x), 0.5f * scale));
+}
+
+// Loads of 16 elements as eight or sixteen words, their largest magnitude, and their values. Magnitudes compare as bit
+// patterns of |x| in fp32, infinities above every number and NaN above those.
+template <typename T>
+struct Chunk;
+template <>
+struct Chunk<float> {
+    static constexpr int kWords = 16;
+    static __device__ __forceinline__ uint32_t largest(const uint32_t (&w)[16]) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m = max(m, w[i] & 0x7fffffffu);
+        return m;
+    }
+    static __device__ __forceinline__ void values(const uint32_t (&w)[16], float (&v)[16]) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(w[i]);
+    }
+};
+template <>
+struct Chunk<__half> {
+    static constexpr int kWords = 8;
+    static __device__ __forceinline__ uint32_t largest(const uint32_t (&w)[8]) {
+        __half2 m = __habs2(*reinterpret_cast<const __half2*>(&w[0]));
+#pragma unroll
+        for (int i = 1; i < 8; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __half2*>(&w[i])));
+        return __float_as_uint(__half2float(__hmax_nan(__low2half(m), __high2half(m)))) & 0x7fffffffu;
+    }
+    static __device__ __forceinline__ void values(const uint32_t (&w)[8], float (&v)[16]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    }
+};
+template <>
+struct Chunk<__nv_bfloat16> {
+    static constexpr int kWords = 8;
+    static __device__ __forceinline__ uint32_t largest(const uint32_t (&w)[8]) {
+        __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[0]));
+#pragma unroll
+        for (int i = 1; i < 8; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[i])));
+        return __float_as_uint(__bfloat162float(__hmax_nan(__low2bfloat16(m), __high2bfloat16(m)))) & 0x7fffffffu;
+    }
+    static __device__ __forceinline__ void values(const uint32_t (&w)[8], float (&v)[16]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+};
 
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-template <typename T>
-__global__ void __launch_bounds__(kQuantThreads)
-quantize_rows_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scale_out, int64_t cols, int64_t ldx,
-                     int64_t ldq) {
-    const T* row = x + static_cast<int64_t>(blockIdx.x) * ldx;
-    int8_t* out = q + static_cast<int64_t>(blockIdx.x) * ldq;
-    __shared__ uint32_t warp_max[kQuantThreads / 32];
-    // the bit pattern of |x| orders like its value, infinities above every number and NaN above those
-    uint32_t m = 0;
-    for (int64_t c = threadIdx.x; c < cols; c += kQuantThreads) m = max(m, __float_as_uint(to_float(row[c])) & 0x7fffffffu);
-    m = __reduce_max_sync(0xffffffffu, m);
-    if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = m;
-    __syncthreads();
-    for (int w = 0; w < kQuantThreads / 32; ++w) m = max(m, warp_max[w]);
-    float scale = __fdiv_rn(__uint_as_float(m), 127.f);
+// Scale of a row from the bit pattern of its largest magnitude. `rounds`: the row is finite and not all of it rounds to 0.
+__device__ __forceinline__ void row_scale(uint32_t largest, float& scale, float& inv, bool& rounds) {
+    scale = __fdiv_rn(__uint_as_float(largest), 127.f);
     if (scale < 1.17549435e-38f) scale = 1.17549435e-38f;
-    const bool finite = m < 0x7f800000u;
-    const float inv = __fdiv_rn(1.f, scale);
-    for (int64_t c = threadIdx.x; c < cols; c += kQuantThreads)
-        out[c] = finite ? static_cast<int8_t>(quantize_value(to_float(row[c]), inv, scale)) : static_cast<int8_t>(0);
-    if (threadIdx.x == 0) scale_out[blockIdx.x] = scale;
+    inv = __fdiv_rn(1.f, scale);
+    rounds = largest < 0x7f800000u;
 }
 
 template <typename T>
-static int launch_quantize(const void* x, void* q, float* scale, int64_t rows, int64_t cols, int64_t ldx, int64_t ldq, cudaStream_t stream) {
-    quantize_rows_kernel<T><<<dim3(static_cast<unsigned>(rows)), kQuantThreads, 0, stream>>>(
-        static_cast<const T*>(x), static_cast<int8_t*>(q), scale, cols, ldx, ldq);
-    TCB_CUDA(cudaGetLastError());
+__device__ __forceinline__ uint4 quantize_chunk(const uint32_t (&w)[Chunk<T>::kWords], float inv, float scale, bool rounds) {
+    float v[kQuantChunk];
+    Chunk<T>::values(w, v);
+    const uint64_t inv2 = pack2(inv, inv), up = pack2(kToInteger, kToInteger), down = pack2(-kToInteger, -kToInteger);
+    const uint64_t minus_scale2 = pack2(-scale, -scale);
+    uint32_t b[kQuantChunk];
+    float far = 0.f;
+#pragma unroll
+    for (int i = 0; i < kQuantChunk; i += 2) {
+        const uint64_t x2 = pack2(v[i], v[i + 1]);
+        const uint64_t shifted = fma2(x2, inv2, up);
+        const uint64_t e2 = fma2(add2(shifted, down), minus_scale2, x2);
+        float s0, s1, e0, e1;
+        unpack2(shifted, s0, s1);
+        unpack2(e2, e0, e1);
+        b[i] = __float_as_uint(s0);
+        b[i + 1] = __float_as_uint(s1);
+        far = fmax3(far, fabsf(e0), fabsf(e1));
+    }
+    if (far >= 0.5f * scale) {
+#pragma unroll
+        for (int i = 0; i < kQuantChunk; ++i) {
+            const float r = __uint_as_float(b[i]) - kToInteger;
+            b[i] = __float_as_uint(settle(r, fmaf(-r, scale, v[i]), 0.5f * scale) + kToInteger);
+        }
+    }
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        o[i] = rounds ? __byte_perm(__byte_perm(b[4 * i], b[4 * i + 1], 0x0040), __byte_perm(b[4 * i + 2], b[4 * i + 3], 0x0040), 0x5410) : 0u;
+    return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+template <typename T, int kChunks>
+__device__ __forceinline__ void load_chunks(uint32_t (&w)[kChunks][Chunk<T>::kWords], const T* src, int whole, int thread, int threads, bool live) {
+    constexpr int kWords = Chunk<T>::kWords;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        const int chunk = c * threads + thread;
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[c][i] = 0;
+        if (live && chunk < whole) {
+            const uint4* p = reinterpret_cast<const uint4*>(src + static_cast<int64_t>(chunk) * kQuantChunk);
+#pragma unroll
+            for (int i = 0; i < kWords / 4; ++i) {
+                const uint4 u = __ldcs(p + i);
+                w[c][4 * i] = u.x;
+                w[c][4 * i + 1] = u.y;
+                w[c][4 * i + 2] = u.z;
+                w[c][4 * i + 3] = u.w;
+            }
+        }
+    }
+}
+
+// Rows on 16-byte boundaries (x and q), a row in the registers of `threads` threads (a power of two up to 1024), kChunks
+// chunks a thread; a block takes blockDim / threads rows at a time and loads the next ones before it rounds these. What is left
+// over behind the whole chunks of a row goes element by element.
+template <typename T, int kChunks>
+__global__ void __launch_bounds__(1024)
+quantize_rows_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scale_out, int rows, int cols, int64_t ldx,
+                     int64_t ldq, int threads) {
+    __shared__ uint32_t warp_max[2][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int thread = static_cast<int>(threadIdx.x) & (threads - 1);
+    const int per_block = static_cast<int>(blockDim.x) / threads;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * per_block;
+    const int whole = cols / kQuantChunk;
+    grid_launch_dependents();
+    grid_dependency_wait();
+    uint32_t w[kChunks][Chunk<T>::kWords];
+    int64_t row = static_cast<int64_t>(blockIdx.x) * per_block + static_cast<int>(threadIdx.x) / threads;
+    load_chunks<T, kChunks>(w, x + row * ldx, whole, thread, threads, row < rows);
+    int buffer = 0;
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * per_block; base < rows; base += step, row += step) {
+        const bool live = row < rows;
+        const T* src = x + row * ldx;
+        uint32_t m = 0;
+        if (live)
+            for (int i = whole * kQuantChunk + thread; i < cols; i += threads) m = max(m, __float_as_uint(to_float(src[i])) & 0x7fffffffu);
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) m = max(m, Chunk<T>::largest(w[c]));
+        uint32_t next[kChunks][Chunk<T>::kWords];
+        load_chunks<T, kChunks>(next, src + step * ldx, whole, thread, threads, row + step < rows);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1)
+            if (d < threads) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+        if (threads > 32) {
+            if (lane == 0) warp_max[buffer][warp] = m;
+            __syncthreads();
+            const int warps = threads >> 5;
+            m = __reduce_max_sync(0xffffffffu, lane < warps ? warp_max[buffer][(warp & ~(warps - 1)) + lane] : 0u);
+            buffer ^= 1;
+        }
+        if (live) {
+            float scale, inv;
+            bool rounds;
+            row_scale(m, scale, inv, rounds);
+            int8_t* dst = q + row * ldq;
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+                const int chunk = c * threads + thread;
+                if (chunk < whole) *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(chunk) * kQuantChunk) = quantize_chunk<T>(w[c], inv, scale, rounds);
+            }
+            for (int i = whole * kQuantChunk + thread; i < cols; i += threads)
+                dst[i] = rounds ? quantize_one(to_float(src[i]), inv, scale) : static_cast<int8_t>(0);
+            if (thread == 0) scale_out[row] = scale;
+        }
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+            for (int i = 0; i < Chunk<T>::kWords; ++i) w[c][i] = next[c][i];
+    }
+}
+
+// Any alignment and length: one block per row, element by element, the row read twice.
+template <typename T>
+__global__ void __launch_bounds__(1024)
+quantize_rows_any_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scale_out, int64_t cols, int64_t ldx,
+                         int64_t ldq) {
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const T* row = x + static_cast<int64_t>(blockIdx.x) * ldx;
+    int8_t* out = q + static_cast<int64_t>(blockIdx.x) * ldq;
+    __shared__ uint32_t warp_max[32];
+    uint32_t m = 0;
+#pragma unroll 8
+    for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) m = max(m, __float_as_uint(to_float(row[c])) & 0x7fffffffu);
+    m = __reduce_max_sync(0xffffffffu, m);
+    if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = m;
+    __syncthreads();
+    m = __reduce_max_sync(0xffffffffu, (threadIdx.x & 31) < blockDim.x / 32 ? warp_max[threadIdx.x & 31] : 0u);
+    float scale, inv;
+    bool rounds;
+    row_scale(m, scale, inv, rounds);
+#pragma unroll 4
+    for (int64_t c = threadIdx.x; c < cols; c += blockDim.x)
+        out[c] = rounds ? quantize_one(to_float(row[c]), inv, scale) : static_cast<int8_t>(0);
+    if (threadIdx.x == 0) scale_out[blockIdx.x] = scale;
+}
+
+template <typename T, int kChunks>
+static int launch_chunks(const T* x, int8_t* q, float* scale, int64_t rows, int64_t cols, int64_t ldx, int64_t ldq, int threads, int sm_count,
+                         cudaStream_t stream) {
+    const int block = threads > kQuantThreads ? threads : kQuantThreads;
+    const int64_t blocks = (rows * threads + block - 1) / block;
+    const int64_t resident = static_cast<int64_t>(sm_count) * (1024 / block);
+    TCB_CUDA(launch_overlapped(quantize_rows_kernel<T, kChunks>, dim3(static_cast<unsigned>(blocks < resident ? blocks : resident)), dim3(block), 0, stream, x, q, scale, static_cast<int>(rows), static_cast<int>(cols), ldx, ldq, threads));
     return TC_OK;
+}
+
+template <typename T>
+static int launch_quantize(const void* xv, void* qv, float* scale, int64_t rows, int64_t cols, int64_t ldx, int64_t ldq, int sm_count,
+                           cudaStream_t stream) {
+    const T* x = static_cast<const T*>(xv);
+    int8_t* q = static_cast<int8_t*>(qv);
+    const int64_t es = sizeof(T);
+    const int64_t chunks = (cols + kQuantChunk - 1) / kQuantChunk;
+    const bool granular = aligned16(x) && aligned16(q) && (ldx * es) % 16 == 0 && ldq % 16 == 0;
+    constexpr int kMost = sizeof(T) == 4 ? 1 : 2;   // chunks a thread can hold twice over in 64 registers
+    if (!granular || chunks > kMost * 1024) {
+        // more threads a row where the rows alone do not fill the SMs: 512 x 65536 fp16 62 us, 124 with 256 threads; 2000 x 4099 28 and 11
+        const int threads = cols > 4096 && rows < 8 * sm_count ? 1024 : kQuantThreads;
+        TCB_CUDA(launch_overlapped(quantize_rows_any_kernel<T>, dim3(static_cast<unsigned>(rows)), dim3(threads), 0, stream, x, q, scale, cols, ldx, ldq));
+        return TC_OK;
+    }
+    // Few rows: as many threads as chunks. Many rows: two chunks a thread, so that a thread has four loads in flight
+    // (8192 x 8192 fp16: 36.4 us, 5.5 TB/s; 46.8 before the next row's loads were issued ahead of the rounding).
+    const int per_thread = rows >= 1024 || chunks > 1024 ? kMost : 1;
+    int threads = 1;
+    while (threads < 1024 && static_cast<int64_t>(threads) * per_thread < chunks) threads *= 2;
+    if (per_thread == 2) return launch_chunks<T, kMost>(x, q, scale, rows, cols, ldx, ldq, threads, sm_count, stream);
+    return launch_chunks<T, 1>(x, q, scale, rows, cols, ldx, ldq, threads, sm_count, stream);
 }
 
 }  // namespace tcb
@@ -78,7 +288,7 @@ extern "C" int tc_quantize_rows(const void* x, void* q, float* scale, int64_t ro
     const DeviceInfo* dev = nullptr;
     if (int rc = current_device(&dev)) return rc;
     auto s = static_cast<cudaStream_t>(stream);
-    if (x_type == TC_F32) return launch_quantize<float>(x, q, scale, rows, cols, ldx, ldq, s);
-    if (x_type == TC_F16) return launch_quantize<__half>(x, q, scale, rows, cols, ldx, ldq, s);
-    return launch_quantize<__nv_bfloat16>(x, q, scale, rows, cols, ldx, ldq, s);
+    if (x_type == TC_F32) return launch_quantize<float>(x, q, scale, rows, cols, ldx, ldq, dev->sm_count, s);
+    if (x_type == TC_F16) return launch_quantize<__half>(x, q, scale, rows, cols, ldx, ldq, dev->sm_count, s);
+    return launch_quantize<__nv_bfloat16>(x, q, scale, rows, cols, ldx, ldq, dev->sm_count, s);
 }
