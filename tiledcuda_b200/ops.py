@@ -86,10 +86,19 @@ def gemm(a: torch.Tensor, b: torch.Tensor, c: torch.Tensor, max_sms: int = 0) ->
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 4}   # enum tc_type
 _HALVES = (torch.float16, torch.bfloat16)
+_INT8 = (torch.int8,)
+_FLOAT = (torch.float32,)
+_INTS = (torch.int32, torch.int64)
 
 
-def _need_rows(t: torch.Tensor, name: str, shape: tuple, dtypes, device: torch.device | None = None) -> None:
-    """A CUDA tensor of this shape whose last dimension is dense; other strides are the caller's."""
+def _need_rows(t: torch.Tensor, name: str, shape: tuple, dtypes, device: int) -> None:
+    """A CUDA tensor of this shape on this device whose last dimension is dense; other strides are the caller's.
+    device is -1 where the first operand of a call is not a CUDA tensor."""
+    try:   # the usual case, in as few attribute reads as it takes
+        if t.shape == shape and t.dtype in dtypes and t.get_device() == device >= 0 and (t.stride(-1) == 1 or shape[-1] <= 1):
+            return
+    except (AttributeError, TypeError):
+        pass
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if not t.is_cuda:
@@ -100,24 +109,36 @@ def _need_rows(t: torch.Tensor, name: str, shape: tuple, dtypes, device: torch.d
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name} must have unit inner stride")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the other operands are on {device}")
+    raise ValueError(f"{name} is on {t.device}, the other operands are on cuda:{device}")
 
 
-def _ndim(t: torch.Tensor, name: str, dim: int) -> None:
+def _shape(t: torch.Tensor, name: str, dim: int) -> torch.Size:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if t.dim() != dim:
         raise ValueError(f"{name} must be {dim}-D, got {list(t.shape)}")
+    return t.shape
 
 
-def _ld(t: torch.Tensor, dim: int = 0, granule: int = 1) -> int:
+def _ld(t: torch.Tensor, shape: tuple, dim: int = 0, granule: int = 1) -> int:
     """Stride of a dimension in elements. That of a dimension of one element is never stepped over and may be anything,
     so it is replaced by the dense one, rounded up to what the kernels' loads are granular in."""
-    if t.shape[dim] > 1:
+    if shape[dim] > 1:
         return t.stride(dim)
-    inner = t.shape[dim + 1] if dim + 2 == t.dim() else t.shape[dim + 1] * _ld(t, dim + 1, granule)
+    inner = shape[dim + 1] if dim + 2 == len(shape) else shape[dim + 1] * _ld(t, shape, dim + 1, granule)
     return -(-max(1, inner) // granule) * granule
+
+
+def _launch(name: str, device: int, *args) -> None:
+    """Calls the C entry point `name` on the current stream of `device` and raises if it fails."""
+    fn = getattr(_lib.load(), name)
+    if device == torch.cuda.current_device():
+        status = fn(*args, _raw_stream(device) if _raw_stream is not None else _stream())
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, _stream())
+    if status:
+        _lib.check(name, status)
 
 
 def quantize_rows(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> None:
@@ -127,15 +148,13 @@ def quantize_rows(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> None
     activations, one per output channel for a weight [N,K]. A row with an infinity or NaN gets that as its scale
     and q = 0. Row strides of x and q may exceed the row length.
     """
-    _ndim(x, "x", 2)
-    _need_rows(x, "x", x.shape, tuple(_TYPES))
-    _need_rows(q, "q", x.shape, (torch.int8,), x.device)
-    _need_rows(scale, "scale", x.shape[:1], (torch.float32,), x.device)
-    m, k = x.shape
-    lib = _lib.load()
-    with _on(x.device):
-        _lib.check("tc_quantize_rows",
-                   lib.tc_quantize_rows(_ptr(x), _ptr(q), _ptr(scale), m, k, _ld(x), _ld(q), _TYPES[x.dtype], _stream()))
+    shape = _shape(x, "x", 2)
+    m, k = shape
+    dev = x.get_device()
+    _need_rows(x, "x", shape, _TYPES, dev)
+    _need_rows(q, "q", shape, _INT8, dev)
+    _need_rows(scale, "scale", (m,), _FLOAT, dev)
+    _launch("tc_quantize_rows", dev, x.data_ptr(), q.data_ptr(), scale.data_ptr(), m, k, _ld(x, shape), _ld(q, shape), _TYPES[x.dtype])
 
 
 def gemm_i8(a: torch.Tensor, b: torch.Tensor, scale_a: torch.Tensor, scale_b: torch.Tensor, c: torch.Tensor) -> None:
@@ -145,24 +164,21 @@ def gemm_i8(a: torch.Tensor, b: torch.Tensor, scale_a: torch.Tensor, scale_b: to
     scaled in fp32 and rounded once. Row strides of a and b must be multiples of 16 bytes, K and N may be any size; M
     may be 0.
     """
-    _ndim(a, "a", 2)
-    _ndim(b, "b", 2)
-    m, k = a.shape
-    n = b.shape[0]
-    _need_rows(a, "a", (m, k), (torch.int8,))
-    _need_rows(b, "b", (n, k), (torch.int8,), a.device)
-    _need_rows(scale_a, "scale_a", (m,), (torch.float32,), a.device)
-    _need_rows(scale_b, "scale_b", (n,), (torch.float32,), a.device)
-    _need_rows(c, "c", (m, n), tuple(_TYPES), a.device)
-    lib = _lib.load()
-    with _on(a.device):
-        _lib.check("tc_gemm_i8",
-                   lib.tc_gemm_i8(_ptr(a), _ptr(b), _ptr(scale_a), _ptr(scale_b), _ptr(c), m, n, k, _ld(a, 0, 16), _ld(b, 0, 16),
-                                  _ld(c), _TYPES[c.dtype], _stream()))
+    sa, sb = _shape(a, "a", 2), _shape(b, "b", 2)
+    m, k = sa
+    n = sb[0]
+    dev = a.get_device()
+    _need_rows(a, "a", sa, _INT8, dev)
+    _need_rows(b, "b", (n, k), _INT8, dev)
+    _need_rows(scale_a, "scale_a", (m,), _FLOAT, dev)
+    _need_rows(scale_b, "scale_b", (n,), _FLOAT, dev)
+    _need_rows(c, "c", (m, n), _TYPES, dev)
+    _launch("tc_gemm_i8", dev, a.data_ptr(), b.data_ptr(), scale_a.data_ptr(), scale_b.data_ptr(), c.data_ptr(), m, n, k,
+            _ld(a, sa, 0, 16), _ld(b, sb, 0, 16), _ld(c, (m, n)), _TYPES[c.dtype])
 
 
-def _need_offsets(offsets: torch.Tensor, experts: int, device: torch.device) -> int:
-    _need_rows(offsets, "offsets", (experts + 1,), (torch.int32, torch.int64), device)
+def _need_offsets(offsets: torch.Tensor, experts: int, device: int) -> int:
+    _need_rows(offsets, "offsets", (experts + 1,), _INTS, device)
     return int(offsets.dtype == torch.int64)
 
 
@@ -173,19 +189,16 @@ def grouped_gemm(a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor, c: tor
     CUDA int32 / int64 tensor [E + 1], nondecreasing, within [0, T]; it is read on the device only. Experts may be
     empty; rows of c outside all groups stay as they were. Row strides of a and b must be multiples of 16 bytes.
     """
-    _ndim(a, "a", 2)
-    _ndim(b, "b", 3)
-    t, k = a.shape
-    e, n = b.shape[:2]
-    _need_rows(a, "a", (t, k), _HALVES)
-    _need_rows(b, "b", (e, n, k), (a.dtype,), a.device)
-    _need_rows(c, "c", (t, n), (a.dtype, torch.float32), a.device)
-    wide = _need_offsets(offsets, e, a.device)
-    lib = _lib.load()
-    with _on(a.device):
-        _lib.check("tc_grouped_gemm",
-                   lib.tc_grouped_gemm(_ptr(a), _ptr(b), _ptr(offsets), wide, _ptr(c), t, e, n, k, _ld(a, 0, 8), _ld(b, 1, 8),
-                                       _ld(b, 0, 8), _ld(c), _TYPES[a.dtype], _TYPES[c.dtype], _stream()))
+    sa, sb = _shape(a, "a", 2), _shape(b, "b", 3)
+    t, k = sa
+    e, n, _ = sb
+    dev = a.get_device()
+    _need_rows(a, "a", sa, _HALVES, dev)
+    _need_rows(b, "b", (e, n, k), (a.dtype,), dev)
+    _need_rows(c, "c", (t, n), (a.dtype, torch.float32), dev)
+    wide = _need_offsets(offsets, e, dev)
+    _launch("tc_grouped_gemm", dev, a.data_ptr(), b.data_ptr(), offsets.data_ptr(), wide, c.data_ptr(), t, e, n, k, _ld(a, sa, 0, 8),
+            _ld(b, sb, 1, 8), _ld(b, sb, 0, 8), _ld(c, (t, n)), _TYPES[a.dtype], _TYPES[c.dtype])
 
 
 def grouped_gemm_i8(a: torch.Tensor, b: torch.Tensor, scale_a: torch.Tensor, scale_b: torch.Tensor, offsets: torch.Tensor,
@@ -195,23 +208,20 @@ def grouped_gemm_i8(a: torch.Tensor, b: torch.Tensor, scale_a: torch.Tensor, sca
     scale_a fp32 [T], scale_b fp32 [E,N] contiguous, c [T,N] fp16, bf16 or fp32; sums as in gemm_i8, offsets and
     rows outside all groups as in grouped_gemm. Strides of a and b must be multiples of 16 bytes.
     """
-    _ndim(a, "a", 2)
-    _ndim(b, "b", 3)
-    t, k = a.shape
-    e, n = b.shape[:2]
-    _need_rows(a, "a", (t, k), (torch.int8,))
-    _need_rows(b, "b", (e, n, k), (torch.int8,), a.device)
-    _need_rows(scale_a, "scale_a", (t,), (torch.float32,), a.device)
-    _need_rows(scale_b, "scale_b", (e, n), (torch.float32,), a.device)
+    sa, sb = _shape(a, "a", 2), _shape(b, "b", 3)
+    t, k = sa
+    e, n, _ = sb
+    dev = a.get_device()
+    _need_rows(a, "a", sa, _INT8, dev)
+    _need_rows(b, "b", (e, n, k), _INT8, dev)
+    _need_rows(scale_a, "scale_a", (t,), _FLOAT, dev)
+    _need_rows(scale_b, "scale_b", (e, n), _FLOAT, dev)
     if not scale_b.is_contiguous():
         raise ValueError("scale_b must be contiguous")
-    _need_rows(c, "c", (t, n), tuple(_TYPES), a.device)
-    wide = _need_offsets(offsets, e, a.device)
-    lib = _lib.load()
-    with _on(a.device):
-        _lib.check("tc_grouped_gemm_i8",
-                   lib.tc_grouped_gemm_i8(_ptr(a), _ptr(b), _ptr(scale_a), _ptr(scale_b), _ptr(offsets), wide, _ptr(c), t, e, n, k,
-                                          _ld(a, 0, 16), _ld(b, 1, 16), _ld(b, 0, 16), _ld(c), _TYPES[c.dtype], _stream()))
+    _need_rows(c, "c", (t, n), _TYPES, dev)
+    wide = _need_offsets(offsets, e, dev)
+    _launch("tc_grouped_gemm_i8", dev, a.data_ptr(), b.data_ptr(), scale_a.data_ptr(), scale_b.data_ptr(), offsets.data_ptr(), wide,
+            c.data_ptr(), t, e, n, k, _ld(a, sa, 0, 16), _ld(b, sb, 1, 16), _ld(b, sb, 0, 16), _ld(c, (t, n)), _TYPES[c.dtype])
 
 
 def grouped_gemm_dgrad(dc: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor, da: torch.Tensor) -> None:
@@ -220,19 +230,16 @@ def grouped_gemm_dgrad(dc: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor,
     dc [T,N] and b [E,N,K] of one type (fp16 or bf16), da [T,K] of that type or fp32; offsets and the rows outside all
     groups as in grouped_gemm. Row strides of dc and b must be multiples of 16 bytes.
     """
-    _ndim(dc, "dc", 2)
-    _ndim(b, "b", 3)
-    t, n = dc.shape
-    e, k = b.shape[0], b.shape[2]
-    _need_rows(dc, "dc", (t, n), _HALVES)
-    _need_rows(b, "b", (e, n, k), (dc.dtype,), dc.device)
-    _need_rows(da, "da", (t, k), (dc.dtype, torch.float32), dc.device)
-    wide = _need_offsets(offsets, e, dc.device)
-    lib = _lib.load()
-    with _on(dc.device):
-        _lib.check("tc_grouped_gemm_dgrad",
-                   lib.tc_grouped_gemm_dgrad(_ptr(dc), _ptr(b), _ptr(offsets), wide, _ptr(da), t, e, n, k, _ld(dc, 0, 8),
-                                             _ld(b, 1, 8), _ld(b, 0, 8), _ld(da), _TYPES[dc.dtype], _TYPES[da.dtype], _stream()))
+    sc, sb = _shape(dc, "dc", 2), _shape(b, "b", 3)
+    t, n = sc
+    e, _, k = sb
+    dev = dc.get_device()
+    _need_rows(dc, "dc", sc, _HALVES, dev)
+    _need_rows(b, "b", (e, n, k), (dc.dtype,), dev)
+    _need_rows(da, "da", (t, k), (dc.dtype, torch.float32), dev)
+    wide = _need_offsets(offsets, e, dev)
+    _launch("tc_grouped_gemm_dgrad", dev, dc.data_ptr(), b.data_ptr(), offsets.data_ptr(), wide, da.data_ptr(), t, e, n, k,
+            _ld(dc, sc, 0, 8), _ld(b, sb, 1, 8), _ld(b, sb, 0, 8), _ld(da, (t, k)), _TYPES[dc.dtype], _TYPES[da.dtype])
 
 
 def grouped_gemm_wgrad(dc: torch.Tensor, a: torch.Tensor, offsets: torch.Tensor, db: torch.Tensor) -> None:
@@ -241,21 +248,17 @@ def grouped_gemm_wgrad(dc: torch.Tensor, a: torch.Tensor, offsets: torch.Tensor,
     dc [T,N] and a [T,K] of one type (fp16 or bf16), db [E,N,K] of that type or fp32, overwritten as a whole. Rows
     outside all groups take no part. Row strides of dc and a must be multiples of 16 bytes.
     """
-    _ndim(dc, "dc", 2)
-    _ndim(a, "a", 2)
-    _ndim(db, "db", 3)
-    t, n = dc.shape
-    k = a.shape[1]
-    e = db.shape[0]
-    _need_rows(dc, "dc", (t, n), _HALVES)
-    _need_rows(a, "a", (t, k), (dc.dtype,), dc.device)
-    _need_rows(db, "db", (e, n, k), (dc.dtype, torch.float32), dc.device)
-    wide = _need_offsets(offsets, e, dc.device)
-    lib = _lib.load()
-    with _on(dc.device):
-        _lib.check("tc_grouped_gemm_wgrad",
-                   lib.tc_grouped_gemm_wgrad(_ptr(dc), _ptr(a), _ptr(offsets), wide, _ptr(db), t, e, n, k, _ld(dc, 0, 8),
-                                             _ld(a, 0, 8), _ld(db, 1), _ld(db, 0), _TYPES[dc.dtype], _TYPES[db.dtype], _stream()))
+    sc, sa, sb = _shape(dc, "dc", 2), _shape(a, "a", 2), _shape(db, "db", 3)
+    t, n = sc
+    k = sa[1]
+    e = sb[0]
+    dev = dc.get_device()
+    _need_rows(dc, "dc", sc, _HALVES, dev)
+    _need_rows(a, "a", (t, k), (dc.dtype,), dev)
+    _need_rows(db, "db", (e, n, k), (dc.dtype, torch.float32), dev)
+    wide = _need_offsets(offsets, e, dev)
+    _launch("tc_grouped_gemm_wgrad", dev, dc.data_ptr(), a.data_ptr(), offsets.data_ptr(), wide, db.data_ptr(), t, e, n, k,
+            _ld(dc, sc, 0, 8), _ld(a, sa, 0, 8), _ld(db, sb, 1), _ld(db, sb, 0), _TYPES[dc.dtype], _TYPES[db.dtype])
 
 
 def gemm_host(a: torch.Tensor, b: torch.Tensor, c: torch.Tensor, workspace: torch.Tensor) -> None:
