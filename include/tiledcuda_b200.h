@@ -89,8 +89,8 @@ int tc_gemm_f16_f32_host(const void* hA, const void* hB, void* hC, int64_t M, in
 enum tc_type { TC_F32 = 0, TC_F16 = 1, TC_BF16 = 4 };
 
 /* Rounds each row (token, or output channel of a weight) of x to 8-bit integers with one fp32 scale:
- *   scale[r] = max(max_c |x[r,c]| / 127, 2^-126),   q[r,c] = x[r,c] / scale[r] rounded to nearest, ties to even,
- * so that q[r,c] * scale[r] stands for x[r,c] and |q| <= 127. The quotient is rounded as the exact one would be (the
+ *   scale[r] = max(max_c |x[r,c]| * (1/127), 2^-126),   q[r,c] = x[r,c] / scale[r] rounded to nearest, ties to even,
+ * with 1/127 and the product rounded to fp32, so that q[r,c] * scale[r] stands for x[r,c] and |q| <= 127. The quotient is rounded as the exact one would be (the
  * division leaves no rounding of its own). A row of zeros gives zeros; a row with an infinity or NaN gives
  * scale = inf or NaN and q = 0, so that what is computed from it is NaN. x is [rows, cols] of x_type (tc_type) with row
  * stride ldx, q int8 with row stride ldq, scale fp32 [rows]; no alignment is asked for beyond that of the types.

@@ -57,11 +57,9 @@ def offsets_of(sizes, start=0, dtype=torch.int32):
 
 # ------------------------------------------------------------------------------------------ quantize_rows
 def quantized(x):
-    """The definition: scale rounded to fp32 from the 64-bit quotient (torch divides fp32 by a number as a product with
-    its rounded reciprocal, which is off by a step at times), q's quotient in 64 bits, so that no near-tie rounds the
-    wrong way."""
-    amax = x.double().abs().amax(1)
-    scale = torch.maximum((amax / torch.full_like(amax, 127.0)).float(), torch.tensor(2.0 ** -126, device=x.device))
+    """The definition: scale a product in fp32, q's quotient in 64 bits, so that no near-tie rounds the wrong way."""
+    c = torch.tensor(1 / 127, dtype=F32, device=x.device)
+    scale = torch.maximum(x.float().abs().amax(1) * c, torch.tensor(2.0 ** -126, device=x.device))
     q = torch.round(x.double() / scale.double()[:, None])
     ok = torch.isfinite(scale)
     return torch.where(ok[:, None], q, torch.zeros_like(q)).to(torch.int8), scale
@@ -101,7 +99,7 @@ def test_quantize_rows_ties_go_to_the_even_integer(cuda_ops, clean_status):
         q = torch.empty(x.shape, dtype=torch.int8, device=DEV)
         scale = torch.empty(1, device=DEV)
         cuda_ops.quantize_rows(x, q, scale)
-        assert scale.item() == top / 127.0   # a power of two
+        assert scale.item() == top / 127   # a power of two: the rounding of 1/127 is lost in that of the product
         assert torch.equal(q[0, 1:].double(), torch.round(half.double())) and q[0, 0] == 127
 
 
@@ -109,7 +107,7 @@ def test_quantize_rows_next_to_a_tie(cuda_ops, clean_status):
     """fp32 values one to three steps around (j + 1/2) * scale for scales that are no power of two."""
     rows = []
     for top in (1.0, 3.3, 0.77, 1e-30, 5e30):
-        scale = torch.tensor(top, dtype=F32) / 127
+        scale = torch.tensor(top, dtype=F32) * torch.tensor(1 / 127, dtype=F32)
         at = ((torch.arange(-127, 127).double() + 0.5) * scale.double()).float()
         row = [torch.tensor([top], dtype=F32)]
         for steps in range(-3, 4):

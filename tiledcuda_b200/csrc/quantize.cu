@@ -1,5 +1,5 @@
-// Rounding of rows to 8-bit integers with one scale per row: scale = max(amax / 127, 2^-126), q = x / scale to nearest,
-// ties to even. Bound by memory: each element is read once (2 or 4 bytes) and written once (1 byte). A row stays in the
+// Rounding of rows to 8-bit integers with one scale per row: scale = max(amax * c, 2^-126) with c = 1 / 127 in fp32,
+// q = x / scale to nearest, ties to even. Bound by memory: each element is read once (2 or 4 bytes) and written once (1 byte). A row stays in the
 // registers of the threads that own it between the maximum and the rounding; rows too long for that, or not on
 // 16-byte boundaries, are read a second time (out of L2).
 #include "host.h"
@@ -89,7 +89,7 @@ __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162f
 
 // Scale of a row from the bit pattern of its largest magnitude. `rounds`: the row is finite and not all of it rounds to 0.
 __device__ __forceinline__ void row_scale(uint32_t largest, float& scale, float& inv, bool& rounds) {
-    scale = __fdiv_rn(__uint_as_float(largest), 127.f);
+    scale = __uint_as_float(largest) * (1.f / 127.f);
     if (scale < 1.17549435e-38f) scale = 1.17549435e-38f;
     inv = __fdiv_rn(1.f, scale);
     rounds = largest < 0x7f800000u;

@@ -144,7 +144,7 @@ def _launch(name: str, device: int, *args) -> None:
 def quantize_rows(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> None:
     """q (int8 [M,K]) and scale (fp32 [M]) such that q[m] * scale[m] stands for x[m] (fp16, bf16 or fp32 [M,K]).
 
-    scale = max(amax|x[m]| / 127, 2^-126); q = x / scale rounded to nearest, ties to even. One scale per token for
+    scale = max(amax|x[m]| * (1/127), 2^-126) in fp32; q = x / scale rounded to nearest, ties to even. One scale per token for
     activations, one per output channel for a weight [N,K]. A row with an infinity or NaN gets that as its scale
     and q = 0. Row strides of x and q may exceed the row length.
     """
