@@ -666,6 +666,46 @@ def test_torch_registry_and_python_package(cuda_ops, clean_status):
         pt.gemm_i8(qp, qb[0], s[:-1], sb[0], c1)
 
 
+def test_the_route_without_the_op_library(cuda_ops, clean_status, monkeypatch):
+    """Where libtiledcuda.so has not been built the calls go through ctypes, with the same result."""
+    g = gen(29)
+    sizes, n, k = [20, 0, 45], 136, 72
+    total, off = sum(sizes), offsets_of(sizes)
+    a, b, dc = halves(g, (total, k), BF16), halves(g, (3, n, k), BF16), halves(g, (total, n), BF16)
+    qb, sb = ints(g, (3, n, k)), torch.rand(3, n, generator=g, device=DEV)
+    results = []
+    for registered in (None, {}):
+        monkeypatch.setattr(cuda_ops, "_registered_ops", registered)
+        q = torch.zeros(total, 80, dtype=torch.int8, device=DEV)[:, :k]
+        s = torch.empty(total, device=DEV)
+        c1, c2, c3 = torch.empty(total, n, device=DEV), torch.empty(total, n, dtype=BF16, device=DEV), torch.empty(total, n, dtype=F16, device=DEV)
+        da, db = torch.empty(total, k, dtype=BF16, device=DEV), torch.empty(3, n, k, device=DEV)
+        cuda_ops.quantize_rows(a, q, s)
+        cuda_ops.gemm_i8(q, qb[0], s, sb[0], c1)
+        cuda_ops.grouped_gemm(a, b, off, c2)
+        cuda_ops.grouped_gemm_i8(q, qb, s, sb, off, c3)
+        cuda_ops.grouped_gemm_dgrad(dc, b, off, da)
+        cuda_ops.grouped_gemm_wgrad(dc, a, off, db)
+        assert bool(cuda_ops._registered_ops) == (registered is None)
+        results.append((q.clone(), s, c1, c2, c3, da, db))
+    assert all(torch.equal(x, y) for x, y in zip(*results))
+
+
+def test_operands_that_require_grad(cuda_ops, clean_status):
+    """Parameters may be operands as they are; the operators are not recorded and results require no grad."""
+    g = gen(30)
+    a, b = halves(g, (40, 64), F16).requires_grad_(), halves(g, (2, 72, 64), F16).requires_grad_()
+    off = offsets_of([15, 25])
+    c, db = torch.empty(40, 72, dtype=F16, device=DEV), torch.empty(2, 72, 64, dtype=F16, device=DEV)
+    cuda_ops.grouped_gemm(a, b, off, c)
+    cuda_ops.grouped_gemm_wgrad(c, a, off, db)
+    assert not c.requires_grad and not db.requires_grad
+    exact, s = plain_forward(a.detach(), b.detach(), [15, 25], 0)
+    assert_within(c, exact, product_error(s, 64))
+    b.grad = db
+    assert b.grad is db
+
+
 def test_refusals_on_device_tensors(cuda_ops):
     """Wrong types, shapes and strides raise before anything is launched."""
     from tiledcuda_b200 import _lib

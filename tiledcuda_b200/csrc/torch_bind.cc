@@ -357,3 +357,10 @@ TORCH_LIBRARY_IMPL(tiledcuda, CUDA, m) {
     m.impl("grouped_gemm_dgrad", &grouped_gemm_dgrad_op);
     m.impl("grouped_gemm_wgrad", &grouped_gemm_wgrad_op);
 }
+
+// The grouped and 8-bit products take no part in autograd (their gradients are operators of their own): parameters that
+// require grad may be operands, and the call goes straight to the kernel.
+TORCH_LIBRARY_IMPL(tiledcuda, Autograd, m) {
+    for (const char* op : {"quantize_rows", "gemm_i8", "grouped_gemm", "grouped_gemm_i8", "grouped_gemm_dgrad", "grouped_gemm_wgrad"})
+        m.impl(op, torch::CppFunction::makeFallthrough());
+}
