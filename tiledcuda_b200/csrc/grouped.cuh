@@ -162,6 +162,33 @@ __device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uin
     asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+// What a warp needs of the scales of its part of an 8-bit tile: those of its columns, and of the first 32 rows it takes. Loaded
+// while the accumulator is still being computed: read from memory when they are needed, they cost each block of 32 rows a trip
+// to L2.
+struct TileScales {
+    float p[4];   // columns 8 m + lane / 4 where 16-bit results leave as rows; else p[0] is column `lane`
+    float q;      // row first + lane
+};
+
+__device__ __forceinline__ bool leaves_by_rows(const GroupedArgs& a) { return a.out_type != TC_F32 && a.vector_out; }
+
+template <bool kI8>
+__device__ __forceinline__ TileScales load_scales(const GroupTile& t, const GroupedArgs& a, int col, int lane, int first) {
+    TileScales s = {};
+    if (kI8) {
+        const int cols = a.cols - col;
+        const float* scale_p = a.scale_p + static_cast<int64_t>(t.e) * a.cols + col;
+        const bool by_rows = leaves_by_rows(a);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            const int c = by_rows ? 8 * m + (lane >> 2) : lane;
+            s.p[m] = c < cols && (by_rows || m == 0) ? scale_p[c] : 0.f;
+        }
+        s.q = first + lane < t.rows ? a.scale_q[t.row0 + first + lane] : 0.f;
+    }
+    return s;
+}
+
 // Drains the part of an output tile that one warp owns: 32 output columns (TMEM lanes, from column `col` of the output on)
 // by the tile's rows (TMEM columns), scaled, converted and stored; of the rows the 32 from `first` on, then `step` on. `staging` is 2 KiB and `row_scales` 32 floats of
 // shared memory of this warp. `zero`: the accumulator holds nothing, the sum is empty.
@@ -171,20 +198,12 @@ __device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uin
 //   everything else: one column per lane, each row of the block one coalesced store of 32 elements.
 template <bool kI8, bool kRaggedX>
 __device__ __forceinline__ void drain_tile(uint32_t taddr, const GroupTile& t, const GroupedArgs& a, int col, uint8_t* staging,
-                                           float* row_scales, bool zero, int lane, int first, int step) {
+                                           float* row_scales, TileScales scales, bool zero, int lane, int first, int step) {
     const int cols = a.cols - col;
     if (cols <= 0 || first >= t.rows) return;
     const int64_t out0 = (kRaggedX ? t.e * a.stride_o : 0) + static_cast<int64_t>(t.row0) * a.ldo + col;
-    const float* scale_p = kI8 ? a.scale_p + static_cast<int64_t>(t.e) * a.cols + col : nullptr;
-    if (a.out_type != TC_F32 && a.vector_out) {
-        float sp[4];
-        if (kI8) {
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const int c = 8 * m + (lane >> 2);
-                sp[m] = c < cols ? scale_p[c] : 0.f;
-            }
-        }
+    const float* scale_q = kI8 ? a.scale_q + t.row0 : nullptr;
+    if (leaves_by_rows(a)) {
         const uint32_t stage = smem_u32(staging);
         // rows of 64 bytes, their 16-byte pieces exchanged so that neither side meets a bank twice
         const int sr = lane & 7, sm = lane >> 3;
@@ -197,21 +216,24 @@ __device__ __forceinline__ void drain_tile(uint32_t taddr, const GroupTile& t, c
         tmem_ld_16x256b_x4(taddr + static_cast<uint32_t>(first), r[0]);
         tmem_ld_16x256b_x4(taddr + static_cast<uint32_t>(first) + (16u << 16), r[1]);
         for (int j0 = first; j0 < t.rows; j0 += step) {
-            if (kI8) row_scales[lane] = j0 + lane < t.rows ? a.scale_q[t.row0 + j0 + lane] : 0.f;
+            if (kI8) {
+                row_scales[lane] = scales.q;
+                scales.q = j0 + step + lane < t.rows ? scale_q[j0 + step + lane] : 0.f;
+            }
             tmem_ld_wait();
             __syncwarp();   // row_scales are there; the staging area has been read
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 uint32_t h[4];
-                float2 sq = make_float2(1.f, 1.f);
-                if (kI8) sq = *reinterpret_cast<const float2*>(row_scales + 8 * q + 2 * (lane & 3));
+                uint64_t sq2 = 0;
+                if (kI8) sq2 = *reinterpret_cast<const uint64_t*>(row_scales + 8 * q + 2 * (lane & 3));
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
                     const uint32_t u0 = r[m >> 1][4 * q + 2 * (m & 1)], u1 = r[m >> 1][4 * q + 2 * (m & 1) + 1];
                     float lo, hi;
                     if (kI8) {
-                        lo = __int2float_rn(static_cast<int>(u0)) * sq.x * sp[m];
-                        hi = __int2float_rn(static_cast<int>(u1)) * sq.y * sp[m];
+                        const uint64_t v = mul2(pack2(__int2float_rn(static_cast<int>(u0)), __int2float_rn(static_cast<int>(u1))), sq2);
+                        unpack2(mul2(v, pack2(scales.p[m], scales.p[m])), lo, hi);
                     } else {
                         lo = kRaggedX && zero ? 0.f : __uint_as_float(u0);
                         hi = kRaggedX && zero ? 0.f : __uint_as_float(u1);
@@ -242,12 +264,12 @@ __device__ __forceinline__ void drain_tile(uint32_t taddr, const GroupTile& t, c
             }
         }
     } else {
-        const float sp = kI8 && lane < cols ? scale_p[lane] : 0.f;
         for (int j0 = first; j0 < t.rows; j0 += step) {
             uint32_t r[32];
             if (kI8) {
                 __syncwarp();
-                row_scales[lane] = j0 + lane < t.rows ? a.scale_q[t.row0 + j0 + lane] : 0.f;
+                row_scales[lane] = scales.q;
+                scales.q = j0 + step + lane < t.rows ? scale_q[j0 + step + lane] : 0.f;
                 __syncwarp();
             }
             tmem_ld_x32(taddr + static_cast<uint32_t>(j0), r);
@@ -257,7 +279,7 @@ __device__ __forceinline__ void drain_tile(uint32_t taddr, const GroupTile& t, c
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
                 if (j0 + j < t.rows) {
-                    const float v = kI8 ? __int2float_rn(static_cast<int>(r[j])) * row_scales[j] * sp : kRaggedX && zero ? 0.f : __uint_as_float(r[j]);
+                    const float v = kI8 ? __int2float_rn(static_cast<int>(r[j])) * row_scales[j] * scales.p[0] : kRaggedX && zero ? 0.f : __uint_as_float(r[j]);
                     if (a.out_type == TC_F32) static_cast<float*>(a.out)[at + j * a.ldo] = v;
                     else static_cast<uint16_t*>(a.out)[at + j * a.ldo] = to_half_bits(v, a.out_type);
                 }

@@ -304,11 +304,12 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
         int acc = 0;
         uint32_t acc_phase = 0;
         while (cursor.next<true>(t)) {
+            const int col = t.col0 + static_cast<int>(rank) * kGpCols + quarter * 32;
+            const TileScales tile_scales = load_scales<kI8>(t, a, col, lane, row_part * 32);
             if (!mbar_wait_warp(&bar_acc_full[acc], acc_phase, abort_word, kDevTimeoutEpilogue)) break;
             tc_fence_after_sync();
             const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * kGpRows);
-            drain_tile<kI8, kRaggedX>(taddr, t, a, t.col0 + static_cast<int>(rank) * kGpCols + quarter * 32, stage, row_scales, t.x_len == 0, lane,
-                                      row_part * 32, 64);
+            drain_tile<kI8, kRaggedX>(taddr, t, a, col, stage, row_scales, tile_scales, t.x_len == 0, lane, row_part * 32, 64);
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&bar_acc_empty[acc]), 0));

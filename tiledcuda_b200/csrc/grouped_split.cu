@@ -177,6 +177,10 @@ grouped_split_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
         tmem_alloc(tmem_slot, tmem_cols);
         tmem_relinquish();
     }
+    if (threadIdx.x == 0) {
+        tma_prefetch_desc(&tmap_p);
+        tma_prefetch_desc(&tmap_q);
+    }
     grid_launch_dependents();
     grid_dependency_wait();   // the offsets may come from the kernel before this one
     if (warp == 0) {
@@ -276,13 +280,15 @@ grouped_split_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
     const int part_of_rows = (warp - 2) >> 2;
     const bool drains = warp >= 2;
     const bool summed = block1 > block0;   // else this CTA's part is zero
+    TileScales tile_scales = {};
+    if (kI8 && drains && t.rows > 0 && splits == 1) tile_scales = load_scales<kI8>(t, a, t.col0 + quarter * 32, lane, part_of_rows * 32);
     const bool ok = drains && t.rows > 0 && mbar_wait_warp(bar_acc, 0, abort_word, kDevTimeoutEpilogue);
     if (ok) tc_fence_after_sync();
     const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     const int64_t out0 = (kRaggedX ? t.e * a.stride_o : 0) + static_cast<int64_t>(t.row0) * a.ldo;
     if (splits == 1) {
         if (ok) drain_tile<kI8, kRaggedX>(taddr, t, a, t.col0 + quarter * 32, ring + 4096 + (warp - 2) * 2048, scales + (warp - 2) * 32,
-                                          !summed, lane, part_of_rows * 32, 64);
+                                          tile_scales, !summed, lane, part_of_rows * 32, 64);
     } else {
         // raw partial sums [row][column] into shared memory (every MMA of this CTA has read the ring), then rank s adds up and
         // writes its share of the rows
