@@ -102,7 +102,7 @@ int tc_quantize_rows(const void* x, void* q, float* scale, int64_t rows, int64_t
  * [K,N] of tc_gemm_f16_f32), scales fp32 [M] and [N] (one per token and per output channel), C of c_type (tc_type)
  * with row stride ldc. The sum over K is exact (32-bit integers; K <= 131071, so that it cannot overflow for any
  * 8-bit values), then (float(sum) * scale_a) * scale_b in fp32 is rounded once to c_type. M may be 0. Needs lda % 16 == 0,
- * ldb % 16 == 0 and 16-byte aligned A and B; K and N may be any size. The reference is fp16-only
+ * ldb % 16 == 0 and 16-byte aligned A and B; K and N may be any size. C must not overlap A or B. The reference is fp16-only
  * (include/cell/compute/gemm.hpp:26-29); no counterpart there. */
 int tc_gemm_i8(const void* A, const void* B, const float* scale_a, const float* scale_b, void* C, int64_t M, int64_t N,
                int64_t K, int64_t lda, int64_t ldb, int64_t ldc, int c_type, tc_stream_t stream);
@@ -115,8 +115,10 @@ int tc_gemm_i8(const void* A, const void* B, const float* scale_a, const float* 
  * decided by a router on the device need no synchronisation. Empty experts are fine; rows before offsets[0] and from
  * offsets[experts] on are not read into any result and their rows of C stay as they were. Offsets outside
  * [0, rows] are clamped to it, a decreasing pair makes an empty expert, and either is reported through tc_device_status()
- * (code 16). 1 <= experts <= 1024; rows may be 0. Needs lda, ldb, stride_b multiples of 16 bytes and 16-byte
- * aligned A and B; N, K and ldc may be any size. One expert's products are the reference's `gemm`
+ * (code 16). 1 <= experts <= 1024; K <= 2^27; rows may be 0. Needs lda, ldb, stride_b multiples of 16 bytes and 16-byte
+ * aligned A and B; N, K and ldc may be any size. C must not overlap A or B. No workspace is used and nothing is kept
+ * between calls, so calls on several streams may overlap and a call may be captured into a graph (after a first one on
+ * the device) and replayed with other offsets. One expert's products are the reference's `gemm`
  * (examples/cpp/01_gemm/02_gemm_all_mem/gemm.hpp:92-155); the grouping has no counterpart there. */
 int tc_grouped_gemm(const void* A, const void* B, const void* offsets, int offsets_are_int64, void* C, int64_t rows,
                     int64_t experts, int64_t N, int64_t K, int64_t lda, int64_t ldb, int64_t stride_b, int64_t ldc,
@@ -130,14 +132,14 @@ int tc_grouped_gemm_i8(const void* A, const void* B, const float* scale_a, const
                        int64_t ldb, int64_t stride_b, int64_t ldc, int c_type, tc_stream_t stream);
 
 /* Gradient of tc_grouped_gemm to A: dA[t,:] = dC[t,:] B[e] for the rows t of expert e. dC [rows,N] (lddc), dA [rows,K]
- * (ldda); everything else, the rows outside all groups included, as there. Needs lddc, ldb, stride_b multiples of 16
+ * (ldda), N <= 2^27; everything else, the rows outside all groups included, as there. Needs lddc, ldb, stride_b multiples of 16
  * bytes. The reference has no backward pass; no counterpart there. */
 int tc_grouped_gemm_dgrad(const void* dC, const void* B, const void* offsets, int offsets_are_int64, void* dA,
                           int64_t rows, int64_t experts, int64_t N, int64_t K, int64_t lddc, int64_t ldb,
                           int64_t stride_b, int64_t ldda, int in_type, int da_type, tc_stream_t stream);
 
 /* Gradient of tc_grouped_gemm to B: dB[e] = sum over the rows t of expert e of dC[t,:]^T A[t,:], the whole of dB
- * [experts,N,K] (row stride lddb, expert stride stride_db): an expert without rows gets zeros. Rows outside all groups
+ * [experts,N,K] (row stride lddb, expert stride stride_db): an expert without rows gets zeros. rows <= 2^27. Rows outside all groups
  * take no part, whatever they hold. The sum runs over the rows in order, so the result does not change from run to run.
  * Needs lddc and lda multiples of 16 bytes. The reference has no backward pass; no counterpart there. */
 int tc_grouped_gemm_wgrad(const void* dC, const void* A, const void* offsets, int offsets_are_int64, void* dB,

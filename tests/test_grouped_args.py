@@ -13,23 +13,23 @@ def quantize(l, x=64, q=64, s=64, rows=4, cols=8, ldx=8, ldq=8, ty=F16):
     return l.tc_quantize_rows(x, q, s, rows, cols, ldx, ldq, ty, None)
 
 
-def i8(l, a=64, b=64, sa=64, sb=64, c=64, m=4, n=8, k=32, lda=32, ldb=32, ldc=8, ty=F16):
+def i8(l, a=64, b=64, sa=64, sb=64, c=4096, m=4, n=8, k=32, lda=32, ldb=32, ldc=8, ty=F16):
     return l.tc_gemm_i8(a, b, sa, sb, c, m, n, k, lda, ldb, ldc, ty, None)
 
 
-def grouped(l, a=64, b=64, off=64, wide=0, c=64, rows=4, e=2, n=8, k=32, lda=32, ldb=32, sb=256, ldc=8, it=F16, ct=F16):
+def grouped(l, a=64, b=64, off=64, wide=0, c=4096, rows=4, e=2, n=8, k=32, lda=32, ldb=32, sb=256, ldc=8, it=F16, ct=F16):
     return l.tc_grouped_gemm(a, b, off, wide, c, rows, e, n, k, lda, ldb, sb, ldc, it, ct, None)
 
 
-def grouped_i8(l, a=64, b=64, sa=64, sb=64, off=64, wide=0, c=64, rows=4, e=2, n=8, k=32, lda=32, ldb=32, stride=256, ldc=8, ct=F16):
+def grouped_i8(l, a=64, b=64, sa=64, sb=64, off=64, wide=0, c=4096, rows=4, e=2, n=8, k=32, lda=32, ldb=32, stride=256, ldc=8, ct=F16):
     return l.tc_grouped_gemm_i8(a, b, sa, sb, off, wide, c, rows, e, n, k, lda, ldb, stride, ldc, ct, None)
 
 
-def dgrad(l, dc=64, b=64, off=64, wide=0, da=64, rows=4, e=2, n=8, k=32, lddc=8, ldb=32, sb=256, ldda=32, it=F16, ot=F16):
+def dgrad(l, dc=64, b=64, off=64, wide=0, da=4096, rows=4, e=2, n=8, k=32, lddc=8, ldb=32, sb=256, ldda=32, it=F16, ot=F16):
     return l.tc_grouped_gemm_dgrad(dc, b, off, wide, da, rows, e, n, k, lddc, ldb, sb, ldda, it, ot, None)
 
 
-def wgrad(l, dc=64, a=64, off=64, wide=0, db=64, rows=4, e=2, n=8, k=32, lddc=8, lda=32, lddb=32, sdb=256, it=F16, ot=F16):
+def wgrad(l, dc=64, a=64, off=64, wide=0, db=4096, rows=4, e=2, n=8, k=32, lddc=8, lda=32, lddb=32, sdb=256, it=F16, ot=F16):
     return l.tc_grouped_gemm_wgrad(dc, a, off, wide, db, rows, e, n, k, lddc, lda, lddb, sdb, it, ot, None)
 
 
@@ -47,6 +47,10 @@ CASES = [
     (grouped, dict(lda=36), BAD, "row stride"), (grouped, dict(ldb=36), BAD, "row stride"), (grouped, dict(sb=260), BAD, "expert stride"),
     (grouped, dict(sb=16), BAD, "expert stride"), (grouped, dict(sb=0), BAD, "expert stride"), (grouped, dict(it=F32, ct=F32), BAD, "in_type"), (grouped, dict(ct=BF16), BAD, "input's type"),
     (grouped, dict(b=72), BAD, "aligned"), (grouped, dict(ldc=0), BAD, "leading dimension"), (grouped, dict(sb=1 << 40), BAD, "too large"),
+    (grouped, dict(c=64), BAD, "overlap"), (grouped, dict(rows=(1 << 31) - 1), BAD, "31 bits"),
+    (grouped, dict(k=1 << 28, lda=1 << 28, ldb=1 << 28, sb=1 << 31), UNSUPPORTED, "terms"), (i8, dict(c=64), BAD, "overlap"),
+    (dgrad, dict(da=64), BAD, "overlap"), (dgrad, dict(n=1 << 28, lddc=1 << 28), UNSUPPORTED, "terms"),
+    (wgrad, dict(db=64), BAD, "overlap"), (wgrad, dict(rows=1 << 28), UNSUPPORTED, "terms"),
     (grouped_i8, dict(off=None), BAD, "offsets"), (grouped_i8, dict(stride=264), BAD, "expert stride"), (grouped_i8, dict(lda=40), BAD, "row stride"),
     (grouped_i8, dict(k=1 << 18, lda=1 << 18, ldb=1 << 18, stride=1 << 21), UNSUPPORTED, "overflow"), (grouped_i8, dict(sa=None), BAD, "null"),
     (dgrad, dict(lddc=12), BAD, "row stride"), (dgrad, dict(ldda=31), BAD, "leading dimension"), (dgrad, dict(dc=None), BAD, "null"),

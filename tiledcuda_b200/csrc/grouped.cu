@@ -14,8 +14,22 @@ static int check_sizes(const char* op, int64_t rows, int64_t experts, int64_t N,
     TCB_REQUIRE(rows >= 0, "%s: the number of rows must not be negative (got %lld)", op, (long long)rows);
     TCB_REQUIRE(experts > 0 && N > 0 && K > 0, "%s: experts, N and K must be positive (got %lld, %lld, %lld)", op, (long long)experts,
                 (long long)N, (long long)K);
-    TCB_REQUIRE(rows < (1ll << 31) && N < (1ll << 31) && K < (1ll << 31), "%s: a dimension does not fit in 31 bits", op);
+    // coordinates are 32-bit and run up to a tile past the end
+    constexpr int64_t kMost = (1ll << 31) - 1024;
+    TCB_REQUIRE(rows < kMost && N < kMost && K < kMost, "%s: a dimension does not fit in 31 bits", op);
     if (experts > kMaxExperts) return fail(TC_ERR_UNSUPPORTED, "%s: %lld experts, at most %d are supported", op, (long long)experts, kMaxExperts);
+    return TC_OK;
+}
+
+// One CTA runs a whole sum; a bounded wait of another warp for it ends after two seconds, which is well above a second of
+// loads at most for this many terms.
+static int check_terms(const char* op, const char* name, int64_t terms) {
+    if (terms > (1ll << 27)) return fail(TC_ERR_UNSUPPORTED, "%s: sums over %s = %lld terms, at most %lld are supported", op, name, (long long)terms, 1ll << 27);
+    return TC_OK;
+}
+
+static int check_distinct(const char* op, const char* out_name, const void* out, const void* in0, const void* in1) {
+    TCB_REQUIRE(out != in0 && out != in1, "%s: %s must not overlap an operand", op, out_name);
     return TC_OK;
 }
 
@@ -134,9 +148,9 @@ static GroupedPlan grouped_plan(const GroupedProblem& g, int sm_count) {
         while (p.splits < 8 && 2 * p.splits * n <= (p.splits == 4 ? 64 : room) && stages >= 16 * p.splits) p.splits *= 2;
     }
     // a bound on the output tiles for any offsets that do not overlap
-    const int64_t row_tiles = g.ragged_x ? groups * ceil_div(g.other, p.tile_rows)
+    p.row_tiles = g.ragged_x ? groups * ceil_div(g.other, p.tile_rows)
                               : g.offsets == nullptr ? ceil_div(g.token_rows, p.tile_rows) : g.token_rows / p.tile_rows + groups;
-    p.tiles = row_tiles * ceil_div(g.cols, p.pair ? 256 : 128);
+    p.tiles = p.row_tiles * ceil_div(g.cols, p.pair ? 256 : 128);
     // The split kernel's CTAs get an SM each, and the ring of one, when they need no more: a few beyond the SMs, of which
     // some will find no tile, do not change that (9 experts x [1001,776], 1333 rows: 152 CTAs 10.8 alone, 14.3 two to an SM).
     p.alone = tiles(p.tile_rows, 128) * p.splits <= sm_count && 10 * p.tiles * p.splits <= 11 * sm_count;
@@ -147,8 +161,7 @@ static int launch_grouped(const GroupedProblem& g, tc_stream_t stream) {
     const DeviceInfo* dev = nullptr;
     if (int rc = current_device(&dev)) return rc;
     const GroupedPlan plan = grouped_plan(g, dev->sm_count);
-    // tile numbers are 32-bit, also for offsets that give every expert all rows
-    if (g.experts * ceil_div(g.ragged_x ? g.other : g.token_rows, plan.tile_rows) * ceil_div(g.cols, 128) * plan.splits >= (1ll << 31))
+    if (plan.tiles * plan.splits >= (1ll << 31))
         return fail(TC_ERR_UNSUPPORTED, "grouped product: too many output tiles (%lld experts, %lld rows, %lld columns)", (long long)g.experts,
                     (long long)g.token_rows, (long long)g.cols);
     auto s = static_cast<cudaStream_t>(stream);
@@ -172,6 +185,7 @@ extern "C" int tc_gemm_i8(const void* A, const void* B, const float* scale_a, co
     TCB_TRY(check_input(op, "A", A, lda, K, 1));
     TCB_TRY(check_input(op, "B", B, ldb, K, 1));
     TCB_TRY(check_output(op, "C", C, ldc, N, c_type));
+    TCB_TRY(check_distinct(op, "C", C, A, B));
     return launch_grouped({B, A, scale_b, scale_a, nullptr, 0, C, M, 1, N, K, ldb, 0, lda, ldc, 0, kTypeI8, c_type, false, false}, stream);
 }
 
@@ -188,6 +202,7 @@ extern "C" int tc_grouped_gemm_i8(const void* A, const void* B, const float* sca
     TCB_TRY(check_input(op, "B", B, ldb, K, 1));
     TCB_TRY(check_stack(op, "B", stride_b, K, experts, 1));
     TCB_TRY(check_output(op, "C", C, ldc, N, c_type));
+    TCB_TRY(check_distinct(op, "C", C, A, B));
     return launch_grouped({B, A, scale_b, scale_a, offsets, offsets_are_int64, C, rows, experts, N, K, ldb, stride_b, lda, ldc, 0, kTypeI8, c_type,
                            false, false}, stream);
 }
@@ -205,6 +220,8 @@ extern "C" int tc_grouped_gemm(const void* A, const void* B, const void* offsets
     TCB_TRY(check_input(op, "B", B, ldb, K, 2));
     TCB_TRY(check_stack(op, "B", stride_b, K, experts, 2));
     TCB_TRY(check_output(op, "C", C, ldc, N, c_type));
+    TCB_TRY(check_distinct(op, "C", C, A, B));
+    TCB_TRY(check_terms(op, "K", K));
     return launch_grouped({B, A, nullptr, nullptr, offsets, offsets_are_int64, C, rows, experts, N, K, ldb, stride_b, lda, ldc, 0, in_type, c_type,
                            false, false}, stream);
 }
@@ -222,6 +239,8 @@ extern "C" int tc_grouped_gemm_dgrad(const void* dC, const void* B, const void* 
     TCB_TRY(check_input(op, "B", B, ldb, K, 2));
     TCB_TRY(check_stack(op, "B", stride_b, K, experts, 2));
     TCB_TRY(check_output(op, "dA", dA, ldda, K, da_type));
+    TCB_TRY(check_distinct(op, "dA", dA, dC, B));
+    TCB_TRY(check_terms(op, "N", N));
     return launch_grouped({B, dC, nullptr, nullptr, offsets, offsets_are_int64, dA, rows, experts, K, N, ldb, stride_b, lddc, ldda, 0, in_type, da_type,
                            true, false}, stream);
 }
@@ -239,6 +258,8 @@ extern "C" int tc_grouped_gemm_wgrad(const void* dC, const void* A, const void* 
         TCB_TRY(check_input(op, "A", A, lda, K, 2));
     }
     TCB_TRY(check_output(op, "dB", dB, lddb, K, db_type));
+    TCB_TRY(check_distinct(op, "dB", dB, dC, A));
+    TCB_TRY(check_terms(op, "rows", rows));
     TCB_REQUIRE(experts == 1 || stride_db >= K, "%s: expert stride of dB smaller than a row", op);
     if (rows == 0) {   // nothing to sum over, and no tensors to describe to TMA
         const size_t es = static_cast<size_t>(type_bytes(db_type));

@@ -40,14 +40,15 @@ __device__ __forceinline__ void group_range(const GroupedArgs& a, int e, int& fi
 // Row tiles of a group: its rows cut evenly, or (wgrad) the same for every group.
 template <bool kRaggedX>
 __device__ __forceinline__ int group_row_tiles(const GroupedArgs& a, int len) {
-    return ((kRaggedX ? a.other : len) + a.tile_rows - 1) / a.tile_rows;
+    const uint32_t rows = static_cast<uint32_t>(kRaggedX ? a.other : len), step = static_cast<uint32_t>(a.tile_rows);
+    return static_cast<int>((rows + step - 1) / step);
 }
 
-__device__ __forceinline__ int warp_inclusive_sum(int v) {
+__device__ __forceinline__ int64_t warp_inclusive_sum(int64_t v) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, v, d);
+        const int64_t up = __shfl_up_sync(0xffffffffu, v, d);
         if (lane >= d) v += up;
     }
     return v;
@@ -56,7 +57,7 @@ __device__ __forceinline__ int warp_inclusive_sum(int v) {
 // Executed by one whole warp (forward and dgrad); `report` lets one CTA of the grid record bad offsets.
 __device__ __forceinline__ void build_group_table(GroupTable* t, const GroupedArgs& a, bool report) {
     const int lane = threadIdx.x & 31;
-    int base = 0;
+    int64_t base = 0;
     bool bad = false;
     for (int e0 = 0; e0 < a.experts; e0 += 32) {
         const int e = e0 + lane;
@@ -68,11 +69,12 @@ __device__ __forceinline__ void build_group_table(GroupTable* t, const GroupedAr
             t->len[e] = len;
             tiles = group_row_tiles<false>(a, len);
         }
-        const int sum = warp_inclusive_sum(tiles);
-        if (e < a.experts) t->tiles_before[e] = base + sum - tiles;
+        const int64_t sum = warp_inclusive_sum(tiles);
+        const int64_t most = a.most_row_tiles;
+        if (e < a.experts) t->tiles_before[e] = static_cast<int>(min(base + sum - tiles, most));
         base += __shfl_sync(0xffffffffu, sum, 31);
     }
-    if (lane == 0) t->tiles_before[a.experts] = base;
+    if (lane == 0) t->tiles_before[a.experts] = static_cast<int>(min(base, static_cast<int64_t>(a.most_row_tiles)));
     if (report && __any_sync(0xffffffffu, bad) && lane == 0) atomicMax(a.status, static_cast<uint32_t>(kDevIndexOutOfRange));
     __syncwarp();
 }
@@ -95,7 +97,7 @@ __device__ __forceinline__ GroupTile make_group_tile(const GroupedArgs& a, int e
         g.x_len = len;
     } else {
         // the rows of a group spread evenly over its tiles, in steps of 32
-        const int step = min(a.tile_rows, ((len + row_tiles - 1) / row_tiles + 31) & ~31);
+        const int step = min(a.tile_rows, ((len - 1) / row_tiles + 32) & ~31);
         g.row0 = first + rt * step;
         g.rows = min(step, len - rt * step);
         g.x0 = 0;

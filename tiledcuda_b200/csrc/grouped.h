@@ -48,13 +48,14 @@ struct GroupedArgs {
     int cols;
     int other;
     int tile_rows;        // most rows of an output tile
+    int most_row_tiles;   // row tiles of all groups together; more come out of overlapping offsets only and are left out
     int out_type;
     int vector_out;       // rows of out start on 16-byte boundaries
     uint32_t idesc;       // instruction descriptor without the N field
     uint32_t* status;
 };
 
-inline GroupedArgs grouped_args(const GroupedProblem& g, int tile_rows, const DeviceInfo* dev) {
+inline GroupedArgs grouped_args(const GroupedProblem& g, int tile_rows, int64_t row_tiles, const DeviceInfo* dev) {
     GroupedArgs a;
     a.offsets = g.offsets;
     a.scale_p = g.scale_p;
@@ -68,6 +69,7 @@ inline GroupedArgs grouped_args(const GroupedProblem& g, int tile_rows, const De
     a.cols = static_cast<int>(g.cols);
     a.other = static_cast<int>(g.other);
     a.tile_rows = tile_rows;
+    a.most_row_tiles = static_cast<int>(row_tiles);
     a.out_type = g.out_type;
     const int es = g.out_type == TC_F32 ? 4 : 2;
     a.vector_out = aligned16(g.out) && (g.ldo * es) % 16 == 0 && (g.stride_o * es) % 16 == 0;
@@ -89,7 +91,8 @@ struct GroupedPlan {
     bool pair;        // grouped_pair.cu, else grouped_split.cu
     int tile_rows;    // most rows of an output tile
     int splits;       // pieces of x per tile (split kernel)
-    int64_t tiles;    // bound on the number of output tiles
+    int64_t row_tiles;   // bound on the row tiles of all groups together
+    int64_t tiles;    // and on the output tiles
     bool alone;       // one CTA per SM (split kernel)
 };
 

@@ -390,7 +390,7 @@ static int launch_variant(const CUtensorMap& tp, const CUtensorMap& tq, const CU
 
 int launch_grouped_pair(const GroupedProblem& g, const GroupedPlan& plan, const DeviceInfo* dev, cudaStream_t stream) {
     const bool i8 = g.in_type == kTypeI8;
-    GroupedArgs a = grouped_args(g, plan.tile_rows, dev);
+    GroupedArgs a = grouped_args(g, plan.tile_rows, plan.row_tiles, dev);
     a.idesc = grouped_idesc(g, 2 * kGpCols);
     // 128-row boxes; of Q also 32-row ones for tiles of fewer rows, or (wgrad) 16 rows of x of both for a group's last step
     CUtensorMap tp, tq, tp_small, tq_small;

@@ -105,13 +105,13 @@ __device__ __forceinline__ GroupTile find_tile(const GroupedArgs& a, int tile, i
     const int e0 = lane * run, e1 = min(a.experts, e0 + run);
     const int row_tile_all = tile / col_tiles;
     bool bad = false;
-    int mine = 0;
+    int64_t mine = 0;
     for (int e = e0; e < e1; ++e) {
         int first, len;
         group_range(a, e, first, len, bad);
         mine += group_row_tiles<kRaggedX>(a, len);
     }
-    int before = warp_inclusive_sum(mine) - mine;
+    int64_t before = warp_inclusive_sum(mine) - mine;
     if (report && __any_sync(0xffffffffu, bad) && lane == 0) atomicMax(a.status, static_cast<uint32_t>(kDevIndexOutOfRange));
     GroupTile g = {};
     const bool here = row_tile_all >= before && row_tile_all < before + mine;
@@ -121,7 +121,7 @@ __device__ __forceinline__ GroupTile find_tile(const GroupedArgs& a, int tile, i
             group_range(a, e, first, len, bad);
             const int tiles = group_row_tiles<kRaggedX>(a, len);
             if (row_tile_all < before + tiles) {
-                g = make_group_tile<kRaggedX>(a, e, first, len, row_tile_all - before, tiles, (tile % col_tiles) * kGsCols);
+                g = make_group_tile<kRaggedX>(a, e, first, len, static_cast<int>(row_tile_all - before), tiles, (tile % col_tiles) * kGsCols);
                 break;
             }
             before += tiles;
@@ -378,7 +378,7 @@ static int launch_variant(const CUtensorMap& tp, const CUtensorMap& tq, const Gr
 
 int launch_grouped_split(const GroupedProblem& g, const GroupedPlan& plan, const DeviceInfo* dev, cudaStream_t stream) {
     const bool i8 = g.in_type == kTypeI8;
-    GroupedArgs a = grouped_args(g, plan.tile_rows, dev);
+    GroupedArgs a = grouped_args(g, plan.tile_rows, plan.row_tiles, dev);
     a.idesc = grouped_idesc(g, kGsCols);
     CUtensorMap tp, tq;
     // P: 128 columns by 128 bytes of x, or (columns contiguous) 64 columns by 64 x; Q: the tile's rows alike

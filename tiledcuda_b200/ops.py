@@ -159,7 +159,9 @@ def _registered(name: str):
         if _OP_LIB.exists():
             torch.ops.load_library(os.fspath(_OP_LIB))
             for op in ("quantize_rows", "gemm_i8", "grouped_gemm", "grouped_gemm_i8", "grouped_gemm_dgrad", "grouped_gemm_wgrad"):
-                _registered_ops[op] = getattr(torch.ops.tiledcuda, op).default
+                packet = getattr(torch.ops.tiledcuda, op, None)   # not in a library built before the op was there
+                if packet is not None:
+                    _registered_ops[op] = packet.default
     return _registered_ops.get(name)
 
 
