@@ -218,12 +218,13 @@ __device__ __forceinline__ void drain_tile(uint32_t taddr, const GroupTile& t, c
         tmem_ld_16x256b_x4(taddr + static_cast<uint32_t>(first), r[0]);
         tmem_ld_16x256b_x4(taddr + static_cast<uint32_t>(first) + (16u << 16), r[1]);
         for (int j0 = first; j0 < t.rows; j0 += step) {
+            __syncwarp();   // the block before this one has left the staging area
             if (kI8) {
                 row_scales[lane] = scales.q;
                 scales.q = j0 + step + lane < t.rows ? scale_q[j0 + step + lane] : 0.f;
             }
             tmem_ld_wait();
-            __syncwarp();   // row_scales are there; the staging area has been read
+            __syncwarp();
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 uint32_t h[4];
@@ -268,22 +269,23 @@ __device__ __forceinline__ void drain_tile(uint32_t taddr, const GroupTile& t, c
     } else {
         for (int j0 = first; j0 < t.rows; j0 += step) {
             uint32_t r[32];
+            __syncwarp();
             if (kI8) {
-                __syncwarp();
                 row_scales[lane] = scales.q;
                 scales.q = j0 + step + lane < t.rows ? scale_q[j0 + step + lane] : 0.f;
                 __syncwarp();
             }
             tmem_ld_x32(taddr + static_cast<uint32_t>(j0), r);
             tmem_ld_wait();
-            if (lane >= cols) continue;
-            const int64_t at = out0 + static_cast<int64_t>(j0) * a.ldo + lane;
+            if (lane < cols) {
+                const int64_t at = out0 + static_cast<int64_t>(j0) * a.ldo + lane;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-                if (j0 + j < t.rows) {
-                    const float v = kI8 ? __int2float_rn(static_cast<int>(r[j])) * row_scales[j] * scales.p[0] : kRaggedX && zero ? 0.f : __uint_as_float(r[j]);
-                    if (a.out_type == TC_F32) static_cast<float*>(a.out)[at + j * a.ldo] = v;
-                    else static_cast<uint16_t*>(a.out)[at + j * a.ldo] = to_half_bits(v, a.out_type);
+                for (int j = 0; j < 32; ++j) {
+                    if (j0 + j < t.rows) {
+                        const float v = kI8 ? __int2float_rn(static_cast<int>(r[j])) * row_scales[j] * scales.p[0] : kRaggedX && zero ? 0.f : __uint_as_float(r[j]);
+                        if (a.out_type == TC_F32) static_cast<float*>(a.out)[at + j * a.ldo] = v;
+                        else static_cast<uint16_t*>(a.out)[at + j * a.ldo] = to_half_bits(v, a.out_type);
+                    }
                 }
             }
         }

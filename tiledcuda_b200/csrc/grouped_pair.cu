@@ -140,6 +140,10 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
         *abort_word = 0;
         fence_barrier_init();
     }
+    if (warp == 2 && lane == 0) {
+        tma_prefetch_desc(&tmap_p);
+        tma_prefetch_desc(&tmap_q);
+    }
     if (warp == 1) {
         tmem_alloc_pair(tmem_slot, 512);
         tmem_relinquish_pair();
@@ -157,10 +161,6 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
     if (warp == 0) {
         // ---------------- TMA producer (both CTAs) ----------------
         const bool leader = elect_one_sync();
-        if (leader) {
-            tma_prefetch_desc(&tmap_p);
-            tma_prefetch_desc(&tmap_q);
-        }
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
