@@ -40,8 +40,7 @@ __device__ __forceinline__ void group_range(const GroupedArgs& a, int e, int& fi
 // Row tiles of a group: its rows cut evenly, or (wgrad) the same for every group.
 template <bool kRaggedX>
 __device__ __forceinline__ int group_row_tiles(const GroupedArgs& a, int len) {
-    const uint32_t rows = static_cast<uint32_t>(kRaggedX ? a.other : len), step = static_cast<uint32_t>(a.tile_rows);
-    return static_cast<int>((rows + step - 1) / step);
+    return static_cast<int>((static_cast<uint32_t>(kRaggedX ? a.other : len) + static_cast<uint32_t>(a.tile_rows) - 1) >> a.tile_shift);
 }
 
 __device__ __forceinline__ int64_t warp_inclusive_sum(int64_t v) {

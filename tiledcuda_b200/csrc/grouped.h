@@ -47,7 +47,8 @@ struct GroupedArgs {
     int experts;
     int cols;
     int other;
-    int tile_rows;        // most rows of an output tile
+    int tile_rows;        // most rows of an output tile, a power of two
+    int tile_shift;       // its logarithm
     int most_row_tiles;   // row tiles of all groups together; more come out of overlapping offsets only and are left out
     int out_type;
     int vector_out;       // rows of out start on 16-byte boundaries
@@ -69,6 +70,8 @@ inline GroupedArgs grouped_args(const GroupedProblem& g, int tile_rows, int64_t 
     a.cols = static_cast<int>(g.cols);
     a.other = static_cast<int>(g.other);
     a.tile_rows = tile_rows;
+    a.tile_shift = 0;
+    while ((1 << a.tile_shift) < tile_rows) ++a.tile_shift;
     a.most_row_tiles = static_cast<int>(row_tiles);
     a.out_type = g.out_type;
     const int es = g.out_type == TC_F32 ? 4 : 2;

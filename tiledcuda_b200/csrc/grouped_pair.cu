@@ -149,11 +149,20 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
         tmem_relinquish_pair();
     }
     grid_launch_dependents();
-    grid_dependency_wait();   // the offsets may come from the kernel before this one
-    if (!kRaggedX && warp == 0) build_group_table(table, a, blockIdx.x == 0);
+    // Without offsets the tiles follow from the sizes: the table, and the scheduler below, need not wait for the kernel before
+    // this one. Everybody who touches global memory waits.
+    const bool dense = a.offsets == nullptr;
+    if (!kRaggedX && dense && warp == 0) build_group_table(table, a, false);
     tc_fence_before_sync();
     cluster_sync_all();   // barriers of both CTAs are initialised before anyone signals across the pair
     tc_fence_after_sync();
+    if (!dense) {
+        grid_dependency_wait();   // the offsets may come from the kernel before this one
+        if (!kRaggedX) {
+            if (warp == 0) build_group_table(table, a, blockIdx.x == 0);
+            __syncthreads();
+        }
+    }
     const uint32_t tmem_base = *tmem_slot;
     TileCursor cursor{tile_ring, bar_tiles_full, bar_tiles_empty, abort_word, 0};
     GroupTile t;
@@ -161,6 +170,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
     if (warp == 0) {
         // ---------------- TMA producer (both CTAs) ----------------
         const bool leader = elect_one_sync();
+        if (dense) grid_dependency_wait();
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
@@ -297,6 +307,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
         __syncwarp();
     } else if (warp < 2 + kGpEpilogueWarps) {
         // ---------------- epilogue (both CTAs) ----------------
+        if (dense) grid_dependency_wait();
         const int quarter = warp & 3;
         uint8_t* stage = staging + (warp - 2) * 2048;
         float* row_scales = scales + (warp - 2) * 32;
