@@ -205,30 +205,41 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
                 const int q_boxes = (half + 31) >> 5;
                 const bool whole_q = t.width == kGpRows;
                 const bool two_rows = half > 64;                         // wgrad: 64-row pieces of Q
-                const uint32_t p_bytes = kPCols ? kGpOperand : chunks * kGpChunk;
-                const uint32_t q_bytes = kRaggedX ? (two_rows ? kGpOperand : kGpChunk) : chunks * (whole_q ? kGpChunk : q_boxes * 4096);
+                // wgrad: of a group's last block only the 16-row steps that it has are fetched
+                const int steps = kRaggedX ? min(kBlockX, x_len - x) >> 4 : 8;
+                const uint32_t p_bytes = kRaggedX ? steps * 2 * kGpTailPiece : kPCols ? kGpOperand : chunks * kGpChunk;
+                const uint32_t q_bytes = kRaggedX ? steps * (two_rows ? 2 : 1) * kGpTailPiece : chunks * (whole_q ? kGpChunk : q_boxes * 4096);
                 const uint32_t bar_addr = map_to_cta(smem_u32(&bar_full[stage]), 0);   // counts the bytes of both CTAs
                 uint8_t* dst_p = smem_p + stage * kGpOperand;
                 uint8_t* dst_q = smem_q + stage * kGpOperand;
                 if (leader) {
                     if (rank == 0) mbar_arrive_expect_tx(&bar_full[stage], 2 * (p_bytes + q_bytes));
-                    if (kPCols) {
-                        const int y = kRaggedX ? t.x0 + x : x;
-                        const int z = kRaggedX ? 0 : t.e;
-                        tma_load_3d_pair(dst_p, &tmap_p, bar_addr, col, y, z);
-                        tma_load_3d_pair(dst_p + kGpChunk, &tmap_p, bar_addr, col + 64, y, z);
-                    } else {
-                        for (int c = 0; c < chunks; ++c) tma_load_3d_pair(dst_p + c * kGpChunk, &tmap_p, bar_addr, x + c * (kBlockX / 2), col, t.e);
-                    }
                     if (kRaggedX) {
-                        tma_load_2d_pair(dst_q, &tmap_q, bar_addr, row, t.x0 + x);
-                        if (two_rows) tma_load_2d_pair(dst_q + kGpChunk, &tmap_q, bar_addr, row + 64, t.x0 + x);
-                    } else if (whole_q) {
-                        for (int c = 0; c < chunks; ++c) tma_load_2d_pair(dst_q + c * kGpChunk, &tmap_q, bar_addr, x + c * (kBlockX / 2), row);
+                        const int y = t.x0 + x;
+                        for (int i = 0; i < (steps < 8 ? steps : 1); ++i) {
+                            const CUtensorMap* mp = steps < 8 ? &tmap_p_small : &tmap_p;
+                            const CUtensorMap* mq = steps < 8 ? &tmap_q_small : &tmap_q;
+                            const int at = i * kGpTailPiece;
+                            tma_load_3d_pair(dst_p + at, mp, bar_addr, col, y + i * 16, 0);
+                            tma_load_3d_pair(dst_p + kGpChunk + at, mp, bar_addr, col + 64, y + i * 16, 0);
+                            tma_load_2d_pair(dst_q + at, mq, bar_addr, row, y + i * 16);
+                            if (two_rows) tma_load_2d_pair(dst_q + kGpChunk + at, mq, bar_addr, row + 64, y + i * 16);
+                        }
                     } else {
-                        for (int c = 0; c < chunks; ++c)
-                            for (int b = 0; b < q_boxes; ++b)
-                                tma_load_2d_pair(dst_q + c * kGpChunk + b * 4096, &tmap_q_small, bar_addr, x + c * (kBlockX / 2), row + b * 32);
+                        if (kPCols) {
+                            tma_load_3d_pair(dst_p, &tmap_p, bar_addr, col, x, t.e);
+                            tma_load_3d_pair(dst_p + kGpChunk, &tmap_p, bar_addr, col + 64, x, t.e);
+                        } else {
+                            for (int c = 0; c < chunks; ++c) tma_load_3d_pair(dst_p + c * kGpChunk, &tmap_p, bar_addr, x + c * (kBlockX / 2), col, t.e);
+                        }
+                        for (int c = 0; c < chunks; ++c) {
+                            if (whole_q) {
+                                tma_load_2d_pair(dst_q + c * kGpChunk, &tmap_q, bar_addr, x + c * (kBlockX / 2), row);
+                            } else {
+                                for (int b = 0; b < q_boxes; ++b)
+                                    tma_load_2d_pair(dst_q + c * kGpChunk + b * 4096, &tmap_q_small, bar_addr, x + c * (kBlockX / 2), row + b * 32);
+                            }
+                        }
                     }
                 }
                 if (++stage == kGpStages) {
