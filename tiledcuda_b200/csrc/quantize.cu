@@ -154,8 +154,9 @@ __device__ __forceinline__ void load_chunks(uint32_t (&w)[kChunks][Chunk<T>::kWo
 // Rows on 16-byte boundaries (x and q), a row in the registers of `threads` threads (a power of two up to 1024), kChunks
 // chunks a thread; a block takes blockDim / threads rows at a time and loads the next ones before it rounds these. What is left
 // over behind the whole chunks of a row goes element by element.
-template <typename T, int kChunks>
-__global__ void __launch_bounds__(1024)
+// kBlock: most threads of a block; 256 where the rows allow, which leaves a thread 80 registers and the loop free of spills.
+template <typename T, int kChunks, int kBlock>
+__global__ void __launch_bounds__(kBlock, kBlock == 256 ? 3 : 1)
 quantize_rows_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scale_out, int rows, int cols, int64_t ldx,
                      int64_t ldq, int threads) {
     __shared__ uint32_t warp_max[2][32];
@@ -212,8 +213,8 @@ quantize_rows_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __r
 }
 
 // Any alignment and length: one block per row, element by element, the row read twice.
-template <typename T>
-__global__ void __launch_bounds__(1024)
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads)
 quantize_rows_any_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scale_out, int64_t cols, int64_t ldx,
                          int64_t ldq) {
     grid_launch_dependents();
@@ -223,16 +224,16 @@ quantize_rows_any_kernel(const T* __restrict__ x, int8_t* __restrict__ q, float*
     __shared__ uint32_t warp_max[32];
     uint32_t m = 0;
 #pragma unroll 8
-    for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) m = max(m, __float_as_uint(to_float(row[c])) & 0x7fffffffu);
+    for (int64_t c = threadIdx.x; c < cols; c += kThreads) m = max(m, __float_as_uint(to_float(row[c])) & 0x7fffffffu);
     m = __reduce_max_sync(0xffffffffu, m);
     if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = m;
     __syncthreads();
-    m = __reduce_max_sync(0xffffffffu, (threadIdx.x & 31) < blockDim.x / 32 ? warp_max[threadIdx.x & 31] : 0u);
+    m = __reduce_max_sync(0xffffffffu, (threadIdx.x & 31) < kThreads / 32 ? warp_max[threadIdx.x & 31] : 0u);
     float scale, inv;
     bool rounds;
     row_scale(m, scale, inv, rounds);
 #pragma unroll 4
-    for (int64_t c = threadIdx.x; c < cols; c += blockDim.x)
+    for (int64_t c = threadIdx.x; c < cols; c += kThreads)
         out[c] = rounds ? quantize_one(to_float(row[c]), inv, scale) : static_cast<int8_t>(0);
     if (threadIdx.x == 0) scale_out[blockIdx.x] = scale;
 }
@@ -242,8 +243,15 @@ static int launch_chunks(const T* x, int8_t* q, float* scale, int64_t rows, int6
                          cudaStream_t stream) {
     const int block = threads > kQuantThreads ? threads : kQuantThreads;
     const int64_t blocks = (rows * threads + block - 1) / block;
-    const int64_t resident = static_cast<int64_t>(sm_count) * (1024 / block);
-    TCB_CUDA(launch_overlapped(quantize_rows_kernel<T, kChunks>, dim3(static_cast<unsigned>(blocks < resident ? blocks : resident)), dim3(block), 0, stream, x, q, scale, static_cast<int>(rows), static_cast<int>(cols), ldx, ldq, threads));
+    const int64_t resident = static_cast<int64_t>(sm_count) * (block > kQuantThreads ? 1024 / block : 3);
+    const dim3 grid(static_cast<unsigned>(blocks < resident ? blocks : resident));
+    if (block > kQuantThreads) {
+        TCB_CUDA(launch_overlapped(quantize_rows_kernel<T, kChunks, 1024>, grid, dim3(block), 0, stream, x, q, scale, static_cast<int>(rows),
+                                   static_cast<int>(cols), ldx, ldq, threads));
+    } else {
+        TCB_CUDA(launch_overlapped(quantize_rows_kernel<T, kChunks, 256>, grid, dim3(block), 0, stream, x, q, scale, static_cast<int>(rows),
+                                   static_cast<int>(cols), ldx, ldq, threads));
+    }
     return TC_OK;
 }
 
@@ -257,13 +265,18 @@ static int launch_quantize(const void* xv, void* qv, float* scale, int64_t rows,
     const bool granular = aligned16(x) && aligned16(q) && (ldx * es) % 16 == 0 && ldq % 16 == 0;
     constexpr int kMost = sizeof(T) == 4 ? 1 : 2;   // chunks a thread can hold twice over in 64 registers
     if (!granular || chunks > kMost * 1024) {
-        // more threads a row where the rows alone do not fill the SMs: 512 x 65536 fp16 62 us, 124 with 256 threads; 2000 x 4099 28 and 11
-        const int threads = cols > 4096 && rows < 8 * sm_count ? 1024 : kQuantThreads;
-        TCB_CUDA(launch_overlapped(quantize_rows_any_kernel<T>, dim3(static_cast<unsigned>(rows)), dim3(threads), 0, stream, x, q, scale, cols, ldx, ldq));
+        // more threads a row where the rows alone do not fill the SMs: 512 x 65536 fp16 49 us, 124 with 256 threads; 2000 x 4099 28 and 11
+        const dim3 grid(static_cast<unsigned>(rows));
+        if (cols > 4096 && rows < 8 * sm_count) {
+            TCB_CUDA(launch_overlapped(quantize_rows_any_kernel<T, 1024>, grid, dim3(1024), 0, stream, x, q, scale, cols, ldx, ldq));
+        } else {
+            TCB_CUDA(launch_overlapped(quantize_rows_any_kernel<T, kQuantThreads>, grid, dim3(kQuantThreads), 0, stream, x, q, scale, cols, ldx, ldq));
+        }
         return TC_OK;
     }
     // Few rows: as many threads as chunks. Many rows: two chunks a thread, so that a thread has four loads in flight
-    // (8192 x 8192 fp16: 36.4 us, 5.5 TB/s; 46.8 before the next row's loads were issued ahead of the rounding).
+    // (8192 x 8192: fp16 34.4 us, 5.9 TB/s; bf16 38.5, fp32 50.6, 6.6 TB/s. fp16 took 46.8 before the next row's loads were
+    // issued ahead of the rounding).
     const int per_thread = rows >= 1024 || chunks > 1024 ? kMost : 1;
     int threads = 1;
     while (threads < 1024 && static_cast<int64_t>(threads) * per_thread < chunks) threads *= 2;
