@@ -272,10 +272,16 @@ GROUPS = [
     ([128, 127, 129], 0, 3, 300, 72), ([255, 256, 257], 0, 0, 264, 200), ([300, 13, 0, 480], 5, 5, 520, 328), ([1, 700, 2], 0, 0, 384, 88),
     ([77] * 20, 0, 0, 200, 160), ([3] * 64, 0, 1, 320, 640), ([1100, 900], 0, 0, 1280, 1032), ([0] * 9 + [2] + [0] * 9, 0, 0, 128, 2056),
 ]
+# Enough tiles for the kernel that works in pairs of SMs: (N, K) of the forward products, the other way round in the gradient
+# to a; the weight gradient takes it for many experts, and cuts long sums over rows in pieces for few.
+RAGGED = [300, 129, 0, 255, 257, 16, 511, 1, 200, 330]
+WIDE = [(RAGGED, 3, 9, 2000, 136), (RAGGED, 0, 0, 1999, 328), ([700, 650], 0, 5, 8200, 72), ([1, 5000, 2], 0, 0, 1290, 1000)]
+WIDE_SUMS = [(RAGGED, 3, 9, 520, 1000), ([16, 32, 48, 15, 17, 0, 127, 128, 129, 143, 144, 145], 0, 1, 777, 1032), ([4101], 2, 1, 200, 136),
+             ([2500, 0, 1700], 0, 0, 130, 100), ([9000], 0, 0, 40, 64)]
 
 
 @pytest.mark.parametrize("dtype,out", [(F16, F16), (BF16, BF16), (F16, F32)])
-@pytest.mark.parametrize("sizes,start,behind,n,k", GROUPS)
+@pytest.mark.parametrize("sizes,start,behind,n,k", GROUPS + WIDE)
 def test_grouped_gemm(cuda_ops, clean_status, sizes, start, behind, n, k, dtype, out):
     g = gen(10)
     total = start + sum(sizes) + behind
@@ -290,7 +296,7 @@ def test_grouped_gemm(cuda_ops, clean_status, sizes, start, behind, n, k, dtype,
 
 
 @pytest.mark.parametrize("out", [F16, BF16, F32])
-@pytest.mark.parametrize("sizes,start,behind,n,k", GROUPS)
+@pytest.mark.parametrize("sizes,start,behind,n,k", GROUPS + WIDE)
 def test_grouped_gemm_i8(cuda_ops, clean_status, sizes, start, behind, n, k, out):
     g = gen(11)
     total = start + sum(sizes) + behind
@@ -309,7 +315,7 @@ def test_grouped_gemm_i8(cuda_ops, clean_status, sizes, start, behind, n, k, out
 
 
 @pytest.mark.parametrize("dtype,out", [(F16, F16), (BF16, BF16), (BF16, F32)])
-@pytest.mark.parametrize("sizes,start,behind,n,k", GROUPS)
+@pytest.mark.parametrize("sizes,start,behind,n,k", GROUPS + [(s, a, b, k, n) for s, a, b, n, k in WIDE])
 def test_grouped_gemm_dgrad(cuda_ops, clean_status, sizes, start, behind, n, k, dtype, out):
     g = gen(12)
     total = start + sum(sizes) + behind
@@ -324,7 +330,7 @@ def test_grouped_gemm_dgrad(cuda_ops, clean_status, sizes, start, behind, n, k, 
 
 
 @pytest.mark.parametrize("dtype,out", [(F16, F16), (BF16, BF16), (F16, F32)])
-@pytest.mark.parametrize("sizes,start,behind,n,k", GROUPS)
+@pytest.mark.parametrize("sizes,start,behind,n,k", GROUPS + WIDE_SUMS)
 def test_grouped_gemm_wgrad(cuda_ops, clean_status, sizes, start, behind, n, k, dtype, out):
     g = gen(13)
     total = start + sum(sizes) + behind
@@ -341,22 +347,23 @@ def test_grouped_gemm_wgrad(cuda_ops, clean_status, sizes, start, behind, n, k, 
             assert (db[e] == 0).all()
 
 
-def test_an_undefined_row_stays_with_its_own_group(cuda_ops, clean_status):
+@pytest.mark.parametrize("n,k,scale", [(136, 72, 1), (1300, 1300, 1), (1300, 1300, 5)])
+def test_an_undefined_row_stays_with_its_own_group(cuda_ops, clean_status, n, k, scale):
     """NaN and infinities in the last rows of one group and the first of the next must not reach the groups between,
     in any of the three products, and in the forward product not even the other rows of their own group."""
-    sizes, n, k = [40, 30, 21, 50], 136, 72
+    sizes = [40 * scale, 30 * scale, 21 * scale, 50 * scale]
     g = gen(14)
-    total = sum(sizes)
+    total, last, next_ = sum(sizes), sizes[0] - 1, sum(sizes[:3])
     a, b, dc = halves(g, (total, k), F16), halves(g, (4, n, k), F16), halves(g, (total, n), F16)
-    a[39], a[91], dc[38], dc[92] = math.nan, math.inf, math.inf, math.nan
+    a[last], a[next_], dc[last - 1], dc[next_ + 1] = math.nan, math.inf, math.inf, math.nan
     off = offsets_of(sizes)
     c, da = torch.empty(total, n, dtype=F16, device=DEV), torch.empty(total, k, dtype=F16, device=DEV)
     db = torch.empty(4, n, k, dtype=F16, device=DEV)
     cuda_ops.grouped_gemm(a, b, off, c)
     cuda_ops.grouped_gemm_dgrad(dc, b, off, da)
     cuda_ops.grouped_gemm_wgrad(dc, a, off, db)
-    assert sorted(torch.nonzero(~torch.isfinite(c).all(1)).flatten().tolist()) == [39, 91]
-    assert sorted(torch.nonzero(~torch.isfinite(da).all(1)).flatten().tolist()) == [38, 92]
+    assert sorted(torch.nonzero(~torch.isfinite(c).all(1)).flatten().tolist()) == [last, next_]
+    assert sorted(torch.nonzero(~torch.isfinite(da).all(1)).flatten().tolist()) == [last - 1, next_ + 1]
     assert [bool(torch.isfinite(db[e]).all()) for e in range(4)] == [False, True, True, False]
 
 
@@ -462,12 +469,13 @@ def test_bad_offsets_are_clamped_and_reported(cuda_ops):
         assert_within(c[clean], exact, product_error(s, k))
 
 
-def test_captured_calls_follow_the_offsets(cuda_ops, clean_status):
+@pytest.mark.parametrize("scale,n,k", [(1, 136, 88), (9, 2600, 2056)])
+def test_captured_calls_follow_the_offsets(cuda_ops, clean_status, scale, n, k):
     """One captured graph, replayed with other offsets and data: the sizes are read on the device at every replay."""
     g = gen(19)
-    total, e, n, k = 333, 5, 136, 88
+    total, e = 333 * scale, 5
     a, b, dc = halves(g, (total, k), F16), halves(g, (e, n, k), F16), halves(g, (total, n), F16)
-    off = offsets_of([100, 0, 33, 150, 50])
+    off = offsets_of([100 * scale, 0, 33 * scale, 150 * scale, 50 * scale])
     c, da = torch.zeros(total, n, dtype=F16, device=DEV), torch.zeros(total, k, dtype=F16, device=DEV)
     db = torch.zeros(e, n, k, dtype=F16, device=DEV)
 
@@ -484,7 +492,7 @@ def test_captured_calls_follow_the_offsets(cuda_ops, clean_status):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         step()
-    for sizes in ([333, 0, 0, 0, 0], [0, 1, 2, 3, 327], [60, 70, 80, 90, 33], [0, 0, 0, 0, 0]):
+    for sizes in ([333 * scale, 0, 0, 0, 0], [0, 1, 2, 3, 327], [60 * scale, 70, 80, 90, 33 * scale], [0, 0, 0, 0, 0]):
         off.copy_(offsets_of(sizes))
         a.copy_(halves(g, (total, k), F16))
         c.fill_(-7.0)
@@ -521,7 +529,7 @@ def test_calls_on_two_streams_at_once(cuda_ops, clean_status):
 
 def test_results_do_not_change_from_run_to_run(cuda_ops, clean_status):
     g = gen(21)
-    for rows, n, k in ((20, 1024, 2048), (1500, 520, 264)):
+    for rows, n, k in ((20, 1024, 2048), (1500, 520, 264), (3000, 2600, 2600)):
         sizes = [rows // 4, rows // 2, rows - rows // 4 - rows // 2]
         a, b, dc = halves(g, (rows, k), F16), halves(g, (3, n, k), F16), halves(g, (rows, n), F16)
         off = offsets_of(sizes)

@@ -1,7 +1,7 @@
 // Rounding of rows to 8-bit integers with one scale per row: scale = max(amax * c, 2^-126) with c = 1 / 127 in fp32,
-// q = x / scale to nearest, ties to even. Bound by memory: each element is read once (2 or 4 bytes) and written once (1 byte). A row stays in the
-// registers of the threads that own it between the maximum and the rounding; rows too long for that, or not on
-// 16-byte boundaries, are read a second time (out of L2).
+// q = x / scale to nearest, ties to even. Bound by memory: each element is read once (2 or 4 bytes) and written once
+// (1 byte). A row stays in the registers of the threads that own it between the maximum and the rounding; rows too long
+// for that, or not on 16-byte boundaries, are read a second time (out of L2).
 #include "host.h"
 #include "sm100.cuh"
 
@@ -87,7 +87,7 @@ __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// Scale of a row from the bit pattern of its largest magnitude. `rounds`: the row is finite and not all of it rounds to 0.
+// Scale of a row from the bit pattern of its largest magnitude. `rounds`: the row is finite; else all of q is 0.
 __device__ __forceinline__ void row_scale(uint32_t largest, float& scale, float& inv, bool& rounds) {
     scale = __uint_as_float(largest) * (1.f / 127.f);
     if (scale < 1.17549435e-38f) scale = 1.17549435e-38f;
