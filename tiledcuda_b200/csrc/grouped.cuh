@@ -138,8 +138,9 @@ __device__ __forceinline__ uint16_t to_half_bits(float v, int type) {
     return type == TC_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
 }
 
-__device__ __forceinline__ uint32_t pack_pair(float lo, float hi, int type) {
-    if (type == TC_BF16) {
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+    if (kBf16) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
         return *reinterpret_cast<const uint32_t*>(&h);
     }
@@ -190,6 +191,72 @@ __device__ __forceinline__ TileScales load_scales(const GroupTile& t, const Grou
     return s;
 }
 
+template <bool kI8, bool kRaggedX, bool kBf16>
+__device__ __forceinline__ void drain_rows(uint32_t taddr, const GroupTile& t, const GroupedArgs& a, int cols, int64_t out0, uint8_t* staging,
+                                           float* row_scales, TileScales scales, bool zero, int lane, int first, int step) {
+    const float* scale_q = kI8 ? a.scale_q + t.row0 : nullptr;
+    const uint32_t stage = smem_u32(staging);
+    // rows of 64 bytes, their 16-byte pieces exchanged so that neither side meets a bank twice
+    const int sr = lane & 7, sm = lane >> 3;
+    const uint32_t st_addr = stage + static_cast<uint32_t>(sr * 64 + ((sm ^ (sr >> 1)) & 3) * 16);
+    const int lr = lane >> 2, lp = lane & 3;
+    const uint8_t* ld_addr = staging + lr * 64 + ((lp ^ (lr >> 1)) & 3) * 16;
+    uint16_t* out = static_cast<uint16_t*>(a.out) + out0 + lr * a.ldo + lp * 8;
+    const int piece_cols = cols - lp * 8;
+    uint32_t r[2][16];
+    tmem_ld_16x256b_x4(taddr + static_cast<uint32_t>(first), r[0]);
+    tmem_ld_16x256b_x4(taddr + static_cast<uint32_t>(first) + (16u << 16), r[1]);
+    for (int j0 = first; j0 < t.rows; j0 += step) {
+        __syncwarp();   // the block before this one has left the staging area
+        if (kI8) {
+            row_scales[lane] = scales.q;
+            scales.q = j0 + step + lane < t.rows ? scale_q[j0 + step + lane] : 0.f;
+        }
+        tmem_ld_wait();
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            uint32_t h[4];
+            uint64_t sq2 = 0;
+            if (kI8) sq2 = *reinterpret_cast<const uint64_t*>(row_scales + 8 * q + 2 * (lane & 3));
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const uint32_t u0 = r[m >> 1][4 * q + 2 * (m & 1)], u1 = r[m >> 1][4 * q + 2 * (m & 1) + 1];
+                float lo, hi;
+                if (kI8) {
+                    const uint64_t v = mul2(pack2(__int2float_rn(static_cast<int>(u0)), __int2float_rn(static_cast<int>(u1))), sq2);
+                    unpack2(mul2(v, pack2(scales.p[m], scales.p[m])), lo, hi);
+                } else {
+                    lo = kRaggedX && zero ? 0.f : __uint_as_float(u0);
+                    hi = kRaggedX && zero ? 0.f : __uint_as_float(u1);
+                }
+                h[m] = pack_pair<kBf16>(lo, hi);
+            }
+            stmatrix_x4_trans(st_addr + static_cast<uint32_t>(q) * 512, h[0], h[1], h[2], h[3]);
+        }
+        if (j0 + step < t.rows) {
+            tmem_ld_16x256b_x4(taddr + static_cast<uint32_t>(j0 + step), r[0]);
+            tmem_ld_16x256b_x4(taddr + static_cast<uint32_t>(j0 + step) + (16u << 16), r[1]);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint4 x = *reinterpret_cast<const uint4*>(ld_addr + i * 512);
+            uint16_t* dst = out + static_cast<int64_t>(j0 + i * 8) * a.ldo;
+            if (j0 + i * 8 + lr < t.rows) {
+                if (piece_cols >= 8) {
+                    *reinterpret_cast<uint4*>(dst) = x;
+                } else {
+                    const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (j < piece_cols) dst[j] = static_cast<uint16_t>(e[j >> 1] >> ((j & 1) * 16));
+                }
+            }
+        }
+    }
+}
+
 // Drains the part of an output tile that one warp owns: 32 output columns (TMEM lanes, from column `col` of the output on)
 // by the tile's rows (TMEM columns), scaled, converted and stored; of the rows the 32 from `first` on, then `step` on. `staging` is 2 KiB and `row_scales` 32 floats of
 // shared memory of this warp. `zero`: the accumulator holds nothing, the sum is empty.
@@ -205,66 +272,8 @@ __device__ __forceinline__ void drain_tile(uint32_t taddr, const GroupTile& t, c
     const int64_t out0 = (kRaggedX ? t.e * a.stride_o : 0) + static_cast<int64_t>(t.row0) * a.ldo + col;
     const float* scale_q = kI8 ? a.scale_q + t.row0 : nullptr;
     if (leaves_by_rows(a)) {
-        const uint32_t stage = smem_u32(staging);
-        // rows of 64 bytes, their 16-byte pieces exchanged so that neither side meets a bank twice
-        const int sr = lane & 7, sm = lane >> 3;
-        const uint32_t st_addr = stage + static_cast<uint32_t>(sr * 64 + ((sm ^ (sr >> 1)) & 3) * 16);
-        const int lr = lane >> 2, lp = lane & 3;
-        const uint8_t* ld_addr = staging + lr * 64 + ((lp ^ (lr >> 1)) & 3) * 16;
-        uint16_t* out = static_cast<uint16_t*>(a.out) + out0 + lr * a.ldo + lp * 8;
-        const int piece_cols = cols - lp * 8;
-        uint32_t r[2][16];
-        tmem_ld_16x256b_x4(taddr + static_cast<uint32_t>(first), r[0]);
-        tmem_ld_16x256b_x4(taddr + static_cast<uint32_t>(first) + (16u << 16), r[1]);
-        for (int j0 = first; j0 < t.rows; j0 += step) {
-            __syncwarp();   // the block before this one has left the staging area
-            if (kI8) {
-                row_scales[lane] = scales.q;
-                scales.q = j0 + step + lane < t.rows ? scale_q[j0 + step + lane] : 0.f;
-            }
-            tmem_ld_wait();
-            __syncwarp();
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                uint32_t h[4];
-                uint64_t sq2 = 0;
-                if (kI8) sq2 = *reinterpret_cast<const uint64_t*>(row_scales + 8 * q + 2 * (lane & 3));
-#pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                    const uint32_t u0 = r[m >> 1][4 * q + 2 * (m & 1)], u1 = r[m >> 1][4 * q + 2 * (m & 1) + 1];
-                    float lo, hi;
-                    if (kI8) {
-                        const uint64_t v = mul2(pack2(__int2float_rn(static_cast<int>(u0)), __int2float_rn(static_cast<int>(u1))), sq2);
-                        unpack2(mul2(v, pack2(scales.p[m], scales.p[m])), lo, hi);
-                    } else {
-                        lo = kRaggedX && zero ? 0.f : __uint_as_float(u0);
-                        hi = kRaggedX && zero ? 0.f : __uint_as_float(u1);
-                    }
-                    h[m] = pack_pair(lo, hi, a.out_type);
-                }
-                stmatrix_x4_trans(st_addr + static_cast<uint32_t>(q) * 512, h[0], h[1], h[2], h[3]);
-            }
-            if (j0 + step < t.rows) {
-                tmem_ld_16x256b_x4(taddr + static_cast<uint32_t>(j0 + step), r[0]);
-                tmem_ld_16x256b_x4(taddr + static_cast<uint32_t>(j0 + step) + (16u << 16), r[1]);
-            }
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint4 x = *reinterpret_cast<const uint4*>(ld_addr + i * 512);
-                uint16_t* dst = out + static_cast<int64_t>(j0 + i * 8) * a.ldo;
-                if (j0 + i * 8 + lr < t.rows) {
-                    if (piece_cols >= 8) {
-                        *reinterpret_cast<uint4*>(dst) = x;
-                    } else {
-                        const uint32_t e[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            if (j < piece_cols) dst[j] = static_cast<uint16_t>(e[j >> 1] >> ((j & 1) * 16));
-                    }
-                }
-            }
-        }
+        if (a.out_type == TC_BF16) drain_rows<kI8, kRaggedX, true>(taddr, t, a, cols, out0, staging, row_scales, scales, zero, lane, first, step);
+        else drain_rows<kI8, kRaggedX, false>(taddr, t, a, cols, out0, staging, row_scales, scales, zero, lane, first, step);
     } else {
         for (int j0 = first; j0 < t.rows; j0 += step) {
             uint32_t r[32];
