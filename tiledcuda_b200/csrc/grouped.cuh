@@ -159,6 +159,24 @@ __device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)
         : "memory");
 }
 
+__device__ __forceinline__ void tmem_ld_16x256b_x2(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld_block(uint32_t taddr, uint32_t (&r)[2][16]) {
+    tmem_ld_16x256b_x4(taddr, r[0]);
+    tmem_ld_16x256b_x4(taddr + (16u << 16), r[1]);
+}
+__device__ __forceinline__ void tmem_ld_block(uint32_t taddr, uint32_t (&r)[2][8]) {
+    tmem_ld_16x256b_x2(taddr, r[0]);
+    tmem_ld_16x256b_x2(taddr + (16u << 16), r[1]);
+}
+__device__ __forceinline__ void tmem_ld_columns(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld_x32(taddr, r); }
+__device__ __forceinline__ void tmem_ld_columns(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld_x16(taddr, r); }
+
 // Four 8 x 8 blocks of 16-bit values, each stored transposed: lane l gives the address of row l % 8 of block l / 8.
 __device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -191,7 +209,10 @@ __device__ __forceinline__ TileScales load_scales(const GroupTile& t, const Grou
     return s;
 }
 
-template <bool kI8, bool kRaggedX, bool kBf16>
+// 16-bit results on 16-byte rows: tcgen05.ld in fragment layout, packed along rows, transposed by stmatrix into
+// [row][column] and stored as 64-byte row pieces. A block of 32 rows costs a warp 4 stmatrix instead of 32 stores of 2 bytes
+// a lane; the block after it is loaded from TMEM meanwhile.
+template <bool kI8, bool kRaggedX, int kRows, bool kBf16>
 __device__ __forceinline__ void drain_rows(uint32_t taddr, const GroupTile& t, const GroupedArgs& a, int cols, int64_t out0, uint8_t* staging,
                                            float* row_scales, TileScales scales, bool zero, int lane, int first, int step) {
     const float* scale_q = kI8 ? a.scale_q + t.row0 : nullptr;
@@ -203,19 +224,18 @@ __device__ __forceinline__ void drain_rows(uint32_t taddr, const GroupTile& t, c
     const uint8_t* ld_addr = staging + lr * 64 + ((lp ^ (lr >> 1)) & 3) * 16;
     uint16_t* out = static_cast<uint16_t*>(a.out) + out0 + lr * a.ldo + lp * 8;
     const int piece_cols = cols - lp * 8;
-    uint32_t r[2][16];
-    tmem_ld_16x256b_x4(taddr + static_cast<uint32_t>(first), r[0]);
-    tmem_ld_16x256b_x4(taddr + static_cast<uint32_t>(first) + (16u << 16), r[1]);
+    uint32_t r[2][kRows / 2];
+    tmem_ld_block(taddr + static_cast<uint32_t>(first), r);
     for (int j0 = first; j0 < t.rows; j0 += step) {
         __syncwarp();   // the block before this one has left the staging area
         if (kI8) {
-            row_scales[lane] = scales.q;
-            scales.q = j0 + step + lane < t.rows ? scale_q[j0 + step + lane] : 0.f;
+            if (lane < kRows) row_scales[lane] = scales.q;
+            scales.q = lane < kRows && j0 + step + lane < t.rows ? scale_q[j0 + step + lane] : 0.f;
         }
         tmem_ld_wait();
         __syncwarp();
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < kRows / 8; ++q) {
             uint32_t h[4];
             uint64_t sq2 = 0;
             if (kI8) sq2 = *reinterpret_cast<const uint64_t*>(row_scales + 8 * q + 2 * (lane & 3));
@@ -234,13 +254,10 @@ __device__ __forceinline__ void drain_rows(uint32_t taddr, const GroupTile& t, c
             }
             stmatrix_x4_trans(st_addr + static_cast<uint32_t>(q) * 512, h[0], h[1], h[2], h[3]);
         }
-        if (j0 + step < t.rows) {
-            tmem_ld_16x256b_x4(taddr + static_cast<uint32_t>(j0 + step), r[0]);
-            tmem_ld_16x256b_x4(taddr + static_cast<uint32_t>(j0 + step) + (16u << 16), r[1]);
-        }
+        if (j0 + step < t.rows) tmem_ld_block(taddr + static_cast<uint32_t>(j0 + step), r);
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kRows / 8; ++i) {
             const uint4 x = *reinterpret_cast<const uint4*>(ld_addr + i * 512);
             uint16_t* dst = out + static_cast<int64_t>(j0 + i * 8) * a.ldo;
             if (j0 + i * 8 + lr < t.rows) {
@@ -258,13 +275,11 @@ __device__ __forceinline__ void drain_rows(uint32_t taddr, const GroupTile& t, c
 }
 
 // Drains the part of an output tile that one warp owns: 32 output columns (TMEM lanes, from column `col` of the output on)
-// by the tile's rows (TMEM columns), scaled, converted and stored; of the rows the 32 from `first` on, then `step` on. `staging` is 2 KiB and `row_scales` 32 floats of
-// shared memory of this warp. `zero`: the accumulator holds nothing, the sum is empty.
-//   16-bit results on 16-byte rows: tcgen05.ld in fragment layout, packed along rows, transposed by stmatrix into
-//     [row][column] and stored as 64-byte row pieces. One warp's 32 x 32 block costs 4 stmatrix instead of 32 stores of
-//     2 bytes a lane; the block after it is loaded meanwhile.
-//   everything else: one column per lane, each row of the block one coalesced store of 32 elements.
-template <bool kI8, bool kRaggedX>
+// by the tile's rows (TMEM columns), scaled, converted and stored; of the rows the kRows from `first` on, then `step` on.
+// `staging` is kRows * 64 bytes and `row_scales` kRows floats of shared memory of this warp. `zero`: the accumulator holds
+// nothing, the sum is empty. 16-bit results on 16-byte rows go through drain_rows; everything else keeps one column per
+// lane, and each row of a block is one coalesced store of 32 elements.
+template <bool kI8, bool kRaggedX, int kRows>
 __device__ __forceinline__ void drain_tile(uint32_t taddr, const GroupTile& t, const GroupedArgs& a, int col, uint8_t* staging,
                                            float* row_scales, TileScales scales, bool zero, int lane, int first, int step) {
     const int cols = a.cols - col;
@@ -272,23 +287,23 @@ __device__ __forceinline__ void drain_tile(uint32_t taddr, const GroupTile& t, c
     const int64_t out0 = (kRaggedX ? t.e * a.stride_o : 0) + static_cast<int64_t>(t.row0) * a.ldo + col;
     const float* scale_q = kI8 ? a.scale_q + t.row0 : nullptr;
     if (leaves_by_rows(a)) {
-        if (a.out_type == TC_BF16) drain_rows<kI8, kRaggedX, true>(taddr, t, a, cols, out0, staging, row_scales, scales, zero, lane, first, step);
-        else drain_rows<kI8, kRaggedX, false>(taddr, t, a, cols, out0, staging, row_scales, scales, zero, lane, first, step);
+        if (a.out_type == TC_BF16) drain_rows<kI8, kRaggedX, kRows, true>(taddr, t, a, cols, out0, staging, row_scales, scales, zero, lane, first, step);
+        else drain_rows<kI8, kRaggedX, kRows, false>(taddr, t, a, cols, out0, staging, row_scales, scales, zero, lane, first, step);
     } else {
         for (int j0 = first; j0 < t.rows; j0 += step) {
-            uint32_t r[32];
+            uint32_t r[kRows];
             __syncwarp();
             if (kI8) {
-                row_scales[lane] = scales.q;
-                scales.q = j0 + step + lane < t.rows ? scale_q[j0 + step + lane] : 0.f;
+                if (lane < kRows) row_scales[lane] = scales.q;
+                scales.q = lane < kRows && j0 + step + lane < t.rows ? scale_q[j0 + step + lane] : 0.f;
                 __syncwarp();
             }
-            tmem_ld_x32(taddr + static_cast<uint32_t>(j0), r);
+            tmem_ld_columns(taddr + static_cast<uint32_t>(j0), r);
             tmem_ld_wait();
             if (lane < cols) {
                 const int64_t at = out0 + static_cast<int64_t>(j0) * a.ldo + lane;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
+                for (int j = 0; j < kRows; ++j) {
                     if (j0 + j < t.rows) {
                         const float v = kI8 ? __int2float_rn(static_cast<int>(r[j])) * row_scales[j] * scales.p[0] : kRaggedX && zero ? 0.f : __uint_as_float(r[j]);
                         if (a.out_type == TC_F32) static_cast<float*>(a.out)[at + j * a.ldo] = v;

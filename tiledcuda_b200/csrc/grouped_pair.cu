@@ -3,11 +3,14 @@
 //   warp 0      TMA producer (both CTAs): per stage 256 bytes of x for 128 columns of P and half of the tile's rows of Q,
 //               landing in the issuing CTA's shared memory and completing on the leader's full barrier;
 //   warp 1      TMEM owner; in the leader also the MMA issuer;
-//   warps 2..9  epilogue (both CTAs), two per TMEM lane quarter: accumulator -> scaled -> converted -> shared memory -> rows
-//               of the output. Four warps took 6500 cycles for a 128 x 256 accumulator, more than the MMAs of a short sum;
-//   warp 10     works out the CTA's tiles, 16 at a time (one per lane), into a ring in shared memory: a search and three
+//   warps 2..17 epilogue (both CTAs), four per TMEM lane quarter: accumulator -> scaled -> converted -> shared memory -> rows
+//               of the output, 16 rows at a time. A warp spends most of a block waiting (TMEM, stmatrix, stores), so their
+//               number counts: four took 6500 cycles for a 128 x 256 accumulator, more than the MMAs of a short sum, eight
+//               4500; sixteen take another 7 to 12 % off a weight gradient of many experts (64 x [2048, 1024]: 97 us from
+//               105) and a fifth off 8-bit results on unaligned rows;
+//   warp 18     works out the CTA's tiles, 16 at a time (one per lane), into a ring in shared memory: a search and three
 //               divisions, about 1000 cycles, which the MMA issuer would otherwise spend between any two tiles;
-//   warp 11     wgrad only: the last K step (16 rows of x) of a group may hold rows of the next group, which have to count as
+//   warp 19     wgrad only: the last K step (16 rows of x) of a group may hold rows of the next group, which have to count as
 //               zero whatever they hold (NaN included), in both operands. Such a step has a buffer of its own, loaded when
 //               the producer starts the tile; this warp overwrites the foreign rows with zeros long before the MMA issuer
 //               comes to it. (Cleared in the ring instead, it held up every tile by about 1000 cycles.)
@@ -23,7 +26,9 @@ constexpr int kGpStages = 3;
 constexpr int kGpOperand = 128 * 256;     // bytes of one operand per stage and CTA: 128 columns / rows x 256 bytes of x
 constexpr int kGpChunk = kGpOperand / 2;  // 128 bytes of x (x contiguous), or 64 columns / rows (those contiguous)
 constexpr int kGpStageBytes = 2 * kGpOperand;
-constexpr int kGpEpilogueWarps = 8;
+constexpr int kGpEpilogueWarps = 16;
+constexpr int kGpDrainRows = 16;          // rows of a block
+constexpr int kGpThreads = 32 * (3 + kGpEpilogueWarps);   // and a warp more for wgrad
 constexpr int kGpBatch = 16;              // tiles worked out at a time; the ring holds two batches
 constexpr int kGpTailPiece = 16 * 128;    // 16 rows of x for 64 columns / rows
 constexpr int kGpTailSlot = 4 * kGpTailPiece;
@@ -33,8 +38,8 @@ template <bool kI8, bool kRaggedX>
 struct PairSmem {
     static constexpr int kTail = kGpStages * kGpStageBytes;                          // wgrad: two slots
     static constexpr int kStaging = kTail + (kRaggedX ? 2 * kGpTailSlot : 0);
-    static constexpr int kScales = kStaging + kGpEpilogueWarps * 2048;
-    static constexpr int kTiles = kScales + (kI8 ? kGpEpilogueWarps * 128 : 0);
+    static constexpr int kScales = kStaging + kGpEpilogueWarps * kGpDrainRows * 64;
+    static constexpr int kTiles = kScales + (kI8 ? kGpEpilogueWarps * kGpDrainRows * 4 : 0);
     static constexpr int kBars = kTiles + 2 * kGpBatch * static_cast<int>(sizeof(GroupTile));
     static constexpr int kTable = kBars + 256;                                        // forward, dgrad
     static constexpr int kTotal = kTable + (kRaggedX ? 0 : static_cast<int>(sizeof(GroupTable))) + 1024;
@@ -88,7 +93,7 @@ __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorM
 }
 
 template <bool kI8, bool kPCols, bool kRaggedX>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kRaggedX ? 384 : 352, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kRaggedX ? kGpThreads + 32 : kGpThreads, 1)
 grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q,
                     const __grid_constant__ CUtensorMap tmap_p_small,
                     const __grid_constant__ CUtensorMap tmap_q_small, const GroupedArgs a) {
@@ -320,18 +325,19 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
         // ---------------- epilogue (both CTAs) ----------------
         if (dense) grid_dependency_wait();
         const int quarter = warp & 3;
-        uint8_t* stage = staging + (warp - 2) * 2048;
-        float* row_scales = scales + (warp - 2) * 32;
-        const int row_part = (warp - 2) >> 2;   // which of every two 32-row blocks
+        uint8_t* stage = staging + (warp - 2) * kGpDrainRows * 64;
+        float* row_scales = scales + (warp - 2) * kGpDrainRows;
+        const int first_row = ((warp - 2) >> 2) * kGpDrainRows;   // its first block of rows; the warps of a quarter take turns
         int acc = 0;
         uint32_t acc_phase = 0;
         while (cursor.next<true>(t)) {
             const int col = t.col0 + static_cast<int>(rank) * kGpCols + quarter * 32;
-            const TileScales tile_scales = load_scales<kI8>(t, a, col, lane, row_part * 32);
+            const TileScales tile_scales = load_scales<kI8>(t, a, col, lane, first_row);
             if (!mbar_wait_warp(&bar_acc_full[acc], acc_phase, abort_word, kDevTimeoutEpilogue)) break;
             tc_fence_after_sync();
             const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * kGpRows);
-            drain_tile<kI8, kRaggedX>(taddr, t, a, col, stage, row_scales, tile_scales, t.x_len == 0, lane, row_part * 32, 64);
+            drain_tile<kI8, kRaggedX, kGpDrainRows>(taddr, t, a, col, stage, row_scales, tile_scales, t.x_len == 0, lane, first_row,
+                                                     kGpEpilogueWarps / 4 * kGpDrainRows);
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&bar_acc_empty[acc]), 0));
@@ -406,7 +412,7 @@ static int launch_variant(const CUtensorMap& tp, const CUtensorMap& tq, const CU
     constexpr int smem = PairSmem<kI8, kRaggedX>::kTotal;
     static OncePerDevice once;
     if (int rc = raise_smem_limit_once(once, dev->device, kernel, smem)) return rc;
-    TCB_CUDA(launch_overlapped(kernel, dim3(2 * pairs), dim3(kRaggedX ? 384 : 352), smem, stream, tp, tq, tp_small, tq_small, a));
+    TCB_CUDA(launch_overlapped(kernel, dim3(2 * pairs), dim3(kRaggedX ? kGpThreads + 32 : kGpThreads), smem, stream, tp, tq, tp_small, tq_small, a));
     return TC_OK;
 }
 

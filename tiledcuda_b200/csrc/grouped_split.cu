@@ -284,7 +284,7 @@ grouped_split_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
     const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     const int64_t out0 = (kRaggedX ? t.e * a.stride_o : 0) + static_cast<int64_t>(t.row0) * a.ldo;
     if (splits == 1) {
-        if (ok) drain_tile<kI8, kRaggedX>(taddr, t, a, t.col0 + quarter * 32, ring + 4096 + (warp - 2) * 2048, scales + (warp - 2) * 32,
+        if (ok) drain_tile<kI8, kRaggedX, 32>(taddr, t, a, t.col0 + quarter * 32, ring + 4096 + (warp - 2) * 2048, scales + (warp - 2) * 32,
                                           tile_scales, !summed, lane, part_of_rows * 32, 64);
     } else {
         // raw partial sums [row][column] into shared memory (every MMA of this CTA has read the ring), then rank s adds up and
