@@ -154,19 +154,17 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
         tmem_relinquish_pair();
     }
     grid_launch_dependents();
-    // Without offsets the tiles follow from the sizes: the table, and the scheduler below, need not wait for the kernel before
-    // this one. Everybody who touches global memory waits.
-    const bool dense = a.offsets == nullptr;
-    if (!kRaggedX && dense && warp == 0) build_group_table(table, a, false);
+    // Without offsets the tiles follow from the sizes, and in the weight gradient all but what is summed over: the table, and
+    // the scheduler below, need not wait for the kernel before this one. Everybody who touches global memory waits.
+    const bool wait_later = kRaggedX || a.offsets == nullptr;
+    if (!kRaggedX && wait_later && warp == 0) build_group_table(table, a, false);
     tc_fence_before_sync();
     cluster_sync_all();   // barriers of both CTAs are initialised before anyone signals across the pair
     tc_fence_after_sync();
-    if (!dense) {
+    if (!wait_later) {
         grid_dependency_wait();   // the offsets may come from the kernel before this one
-        if (!kRaggedX) {
-            if (warp == 0) build_group_table(table, a, blockIdx.x == 0);
-            __syncthreads();
-        }
+        if (warp == 0) build_group_table(table, a, blockIdx.x == 0);
+        __syncthreads();
     }
     const uint32_t tmem_base = *tmem_slot;
     TileCursor cursor{tile_ring, bar_tiles_full, bar_tiles_empty, abort_word, 0};
@@ -175,7 +173,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
     if (warp == 0) {
         // ---------------- TMA producer (both CTAs) ----------------
         const bool leader = elect_one_sync();
-        if (dense) grid_dependency_wait();
+        if (wait_later) grid_dependency_wait();
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
@@ -323,7 +321,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
         __syncwarp();
     } else if (warp < 2 + kGpEpilogueWarps) {
         // ---------------- epilogue (both CTAs) ----------------
-        if (dense) grid_dependency_wait();
+        if (wait_later) grid_dependency_wait();
         const int quarter = warp & 3;
         uint8_t* stage = staging + (warp - 2) * kGpDrainRows * 64;
         float* row_scales = scales + (warp - 2) * kGpDrainRows;
@@ -355,19 +353,21 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
             const int half = batch & 1;
             if (batch >= 2 && !mbar_wait_warp(&bar_tiles_empty[half], (static_cast<uint32_t>(batch >> 1) & 1u) ^ 1u, abort_word, kDevTimeoutMma)) break;
             const int64_t tile = pair + static_cast<int64_t>(batch * kGpBatch + lane) * num_pairs;
+            GroupTile g = {};   // no rows: the end
             if (lane < kGpBatch) {
-                GroupTile g = {};   // no rows: the end
                 if (tile < num_tiles) {
                     if (kRaggedX) {
                         const int per_group = row_tiles * col_tiles;
                         const int e = static_cast<int>(tile) / per_group;
-                        int first, len;
-                        group_range(a, e, first, len, bad);
-                        g = banded_tile<true>(a, e, first, len, static_cast<int>(tile) - e * per_group, row_tiles, col_tiles, 2 * kGpCols);
+                        g = banded_tile<true>(a, e, 0, 0, static_cast<int>(tile) - e * per_group, row_tiles, col_tiles, 2 * kGpCols);
                     } else {
                         g = group_tile(table, a, static_cast<int>(tile), col_tiles, 2 * kGpCols);
                     }
                 }
+            }
+            if (kRaggedX && batch == 0) grid_dependency_wait();   // only what is summed over depends on the offsets
+            if (lane < kGpBatch) {
+                if (kRaggedX && g.rows > 0) group_range(a, g.e, g.x0, g.x_len, bad);
                 tile_ring[half * kGpBatch + lane] = g;
             }
             __syncwarp();
