@@ -154,18 +154,10 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
         tmem_relinquish_pair();
     }
     grid_launch_dependents();
-    // Without offsets the tiles follow from the sizes, and in the weight gradient all but what is summed over: the table, and
-    // the scheduler below, need not wait for the kernel before this one. Everybody who touches global memory waits.
-    const bool wait_later = kRaggedX || a.offsets == nullptr;
-    if (!kRaggedX && wait_later && warp == 0) build_group_table(table, a, false);
     tc_fence_before_sync();
     cluster_sync_all();   // barriers of both CTAs are initialised before anyone signals across the pair
     tc_fence_after_sync();
-    if (!wait_later) {
-        grid_dependency_wait();   // the offsets may come from the kernel before this one
-        if (warp == 0) build_group_table(table, a, blockIdx.x == 0);
-        __syncthreads();
-    }
+    // From here on everybody who touches global memory first waits for the kernel before this one (griddepcontrol.wait).
     const uint32_t tmem_base = *tmem_slot;
     TileCursor cursor{tile_ring, bar_tiles_full, bar_tiles_empty, abort_word, 0};
     GroupTile t;
@@ -173,7 +165,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
     if (warp == 0) {
         // ---------------- TMA producer (both CTAs) ----------------
         const bool leader = elect_one_sync();
-        if (wait_later) grid_dependency_wait();
+        grid_dependency_wait();
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
@@ -321,7 +313,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
         __syncwarp();
     } else if (warp < 2 + kGpEpilogueWarps) {
         // ---------------- epilogue (both CTAs) ----------------
-        if (wait_later) grid_dependency_wait();
+        grid_dependency_wait();
         const int quarter = warp & 3;
         uint8_t* stage = staging + (warp - 2) * kGpDrainRows * 64;
         float* row_scales = scales + (warp - 2) * kGpDrainRows;
@@ -346,6 +338,12 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
         }
     } else if (warp == 2 + kGpEpilogueWarps) {
         // ---------------- which tiles (both CTAs) ----------------
+        // Without offsets the tiles follow from the sizes, and in the weight gradient all but what is summed over; neither
+        // waits for the kernel before this one.
+        if (!kRaggedX) {
+            if (a.offsets != nullptr) grid_dependency_wait();
+            build_group_table(table, a, blockIdx.x == 0);
+        }
         const int row_tiles = group_row_tiles<kRaggedX>(a, 0);   // wgrad: of every group
         const int num_tiles = (kRaggedX ? a.experts * row_tiles : table->tiles_before[a.experts]) * col_tiles;
         bool bad = false;
