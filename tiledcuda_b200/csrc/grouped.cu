@@ -112,18 +112,19 @@ static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // The kernel and tile for a problem, from its sizes alone; of the offsets the host knows nothing, so the rule takes the
 // rows to be spread evenly. Times below in us: B200, CUDA graph replays, three sets of operands in turn.
 //  * Pair tiles (256 columns x up to 256 rows) once there are enough of them for the 74 pairs and the groups have 128
-//    rows or more to fill them: 32 experts x [4096,1024] with 4096 rows 59 against 69 in the split kernel, weight gradient
-//    of 16 x [2048,1024] 31 against 48. With 64 tiles the split kernel is ahead for one dense product (int8 2048^3 10.8
-//    against 12.2), the pair kernel where each group brings its own weights (8 x [2048,1024], 2048 rows: 18.4 against 19.3).
+//    rows or more to fill them: 32 experts x [4096,1024] with 4096 rows 58 against 67 in the split kernel, weight gradient
+//    of 16 x [2048,1024] 30 against 46. With 64 tiles the split kernel is ahead for one dense product (int8 2048^3 9.4
+//    against 11.5), the pair kernel where each group brings its own weights (8 x [2048,1024], 2048 rows: 17.8 against 18.5).
 //  * Else the split kernel. Where the weights' bytes count (few rows per group), a tile takes all rows of a group up to
-//    four times the even share, so that a popular expert's weights are read once: 16 x [2048,2048] with 512 rows 25
-//    with 128-row tiles against 30 with 32.
-//  * Tiles are halved while they still all run at once, one per SM: int8 1024^3 4.4 with 64 rows, 5.4 with 128; for long
-//    sums not below 64 rows, where cutting the sum does more: int8 300 x 1024 x 8192 9.4 with two pieces of 64-row
-//    tiles, 10.8 with 32-row tiles.
-//  * The sum is cut while SMs are idle and a piece keeps eight stages: int8 1 x 4096 x 4096 5.9 in four pieces, 6.7 in one.
-//    Clusters of eight only for a handful of tiles: a GPC holds two of them at most, and a weight gradient of 512 x 512
-//    from 4096 rows took 17.2 in eight pieces and 9.2 in four.
+//    four times the even share, so that a popular expert's weights are read once: 16 x [2048,2048] with 512 rows 24.6
+//    with 128-row tiles against 29.7 with 32.
+//  * Tiles are halved while they still all run at once, one per SM: int8 1024^3 3.7 with 64 rows, 4.1 with 128; for long
+//    sums not below 64 rows, where cutting the sum does more (int8 300 x 1024 x 8192 8.7 with two pieces of 64-row
+//    tiles, 9.9 with 32-row tiles), unless even eight pieces would leave most SMs idle (64 x 512 x 4096: 6.0 against 7.2).
+//  * The sum is cut in four where that many pieces still run at once (int8 1 x 4096 x 4096 5.1, in one piece 5.9; 64 x 2048
+//    x 4096 5.1 and 6.1). Two pieces save less than joining them costs unless the sum is long (128 x 4096 x 4096 7.5, in one
+//    piece 6.7; 300 x 1024 x 8192 8.7 and 10.1). Clusters of eight only for a handful of tiles: a GPC holds two of them at
+//    most, and a weight gradient of 512 x 512 from 4096 rows takes 13.3 in eight pieces and 8.3 in four.
 static GroupedPlan grouped_plan(const GroupedProblem& g, int sm_count) {
     const int64_t groups = g.offsets == nullptr ? 1 : g.ragged_x ? g.experts : (g.experts < g.token_rows ? g.experts : g.token_rows);
     const int64_t share = ceil_div(g.token_rows, groups);               // rows of a group, spread evenly
@@ -143,9 +144,12 @@ static GroupedPlan grouped_plan(const GroupedProblem& g, int sm_count) {
         const int64_t least = g.ragged_x || stages > 16 ? 64 : 32;
         while (p.tile_rows > least && tiles(p.tile_rows / 2, 128) <= sm_count && (!own_weights || share > 128 || p.tile_rows / 2 >= share))
             p.tile_rows /= 2;
+        while (p.tile_rows > (g.ragged_x ? 64 : 16) && 8 * tiles(p.tile_rows, 128) < 48) p.tile_rows /= 2;
         const int64_t n = tiles(p.tile_rows, 128);
         const int64_t room = own_weights ? sm_count / 2 : sm_count;   // uneven groups make more tiles than counted here
-        while (p.splits < 8 && 2 * p.splits * n <= (p.splits == 4 ? 64 : room) && stages >= 16 * p.splits) p.splits *= 2;
+        if (8 * n <= 64 && stages >= 64) p.splits = 8;
+        else if (4 * n <= room && stages >= 32) p.splits = 4;
+        else if (2 * n <= room && stages >= 48) p.splits = 2;
     }
     // a bound on the output tiles for any offsets that do not overlap
     p.row_tiles = g.ragged_x ? groups * ceil_div(g.other, p.tile_rows)
