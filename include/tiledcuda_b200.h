@@ -90,11 +90,11 @@ enum tc_type { TC_F32 = 0, TC_F16 = 1, TC_BF16 = 4 };
 
 /* Rounds each row (token, or output channel of a weight) of x to 8-bit integers with one fp32 scale:
  *   scale[r] = max(max_c |x[r,c]| * (1/127), 2^-126),   q[r,c] = x[r,c] / scale[r] rounded to nearest, ties to even,
- * with 1/127 and the product rounded to fp32, so that q[r,c] * scale[r] stands for x[r,c] and |q| <= 127. The quotient is rounded as the exact one would be (the
- * division leaves no rounding of its own). A row of zeros gives zeros; a row with an infinity or NaN gives
- * scale = inf or NaN and q = 0, so that what is computed from it is NaN. x is [rows, cols] of x_type (tc_type) with row
- * stride ldx, q int8 with row stride ldq, scale fp32 [rows]; no alignment is asked for beyond that of the types.
- * The reference has no 8-bit path; no counterpart there. */
+ * with 1/127 and the product rounded to fp32, so that q[r,c] * scale[r] stands for x[r,c] and |q| <= 127. The quotient is
+ * rounded as the exact one would be (the division leaves no rounding of its own). A row of zeros gives zeros; a row with an
+ * infinity or NaN gives scale = inf or NaN and q = 0, so that what is computed from it is NaN. x is [rows, cols] of x_type
+ * (tc_type) with row stride ldx, q int8 with row stride ldq, scale fp32 [rows]; no alignment is asked for beyond that of the
+ * types. q and scale must not overlap x or each other. The reference has no 8-bit path; no counterpart there. */
 int tc_quantize_rows(const void* x, void* q, float* scale, int64_t rows, int64_t cols, int64_t ldx, int64_t ldq,
                      int x_type, tc_stream_t stream);
 
@@ -139,8 +139,8 @@ int tc_grouped_gemm_dgrad(const void* dC, const void* B, const void* offsets, in
                           int64_t stride_b, int64_t ldda, int in_type, int da_type, tc_stream_t stream);
 
 /* Gradient of tc_grouped_gemm to B: dB[e] = sum over the rows t of expert e of dC[t,:]^T A[t,:], the whole of dB
- * [experts,N,K] (row stride lddb, expert stride stride_db): an expert without rows gets zeros. rows <= 2^27. Rows outside all groups
- * take no part, whatever they hold. The sum runs over the rows in order, so the result does not change from run to run.
+ * [experts,N,K] (row stride lddb, expert stride stride_db): an expert without rows gets zeros. rows <= 2^27. Rows outside
+ * all groups take no part, whatever they hold. The sum runs over the rows in order, so the result does not change from run to run.
  * Needs lddc and lda multiples of 16 bytes. The reference has no backward pass; no counterpart there. */
 int tc_grouped_gemm_wgrad(const void* dC, const void* A, const void* offsets, int offsets_are_int64, void* dB,
                           int64_t rows, int64_t experts, int64_t N, int64_t K, int64_t lddc, int64_t lda, int64_t lddb,

@@ -37,6 +37,7 @@ CASES = [
     (quantize, dict(x=None), BAD, "null"), (quantize, dict(s=None), BAD, "null"), (quantize, dict(cols=0), BAD, "positive"),
     (quantize, dict(rows=-1), BAD, "negative"), (quantize, dict(rows=1 << 31), BAD, "31 bits"), (quantize, dict(ldx=7), BAD, "leading dimension"),
     (quantize, dict(ldq=7), BAD, "leading dimension"), (quantize, dict(ty=I32), BAD, "x_type"), (quantize, dict(x=65), BAD, "aligned"),
+    (quantize, dict(q=128), BAD, "overlap"), (quantize, dict(s=128), BAD, "overlap"), (quantize, dict(x=128), BAD, "overlap"),
     (i8, dict(a=None), BAD, "null"), (i8, dict(sa=None), BAD, "null"), (i8, dict(c=None), BAD, "null"), (i8, dict(m=-1), BAD, "negative"),
     (i8, dict(n=0), BAD, "positive"), (i8, dict(k=0), BAD, "positive"), (i8, dict(lda=40), BAD, "row stride"), (i8, dict(ldb=24), BAD, "leading dimension"),
     (i8, dict(ldc=7), BAD, "leading dimension"), (i8, dict(a=72), BAD, "aligned"), (i8, dict(c=65), BAD, "aligned"), (i8, dict(sb=66), BAD, "aligned"),
@@ -96,3 +97,13 @@ def test_python_route_refuses_cpu_tensors_and_wrong_types():
         ops.grouped_gemm(None, b, off, c)
     with pytest.raises(TypeError):
         ops.quantize_rows([1.0], None, None)
+
+
+@pytest.mark.parametrize("file", [None, b"not a library"])
+def test_an_op_library_that_does_not_load_leaves_the_other_route(tmp_path, monkeypatch, file):
+    path = tmp_path / "libtiledcuda.so"
+    if file is not None:
+        path.write_bytes(file)
+    monkeypatch.setattr(ops, "_OP_LIB", path)
+    monkeypatch.setattr(ops, "_registered_ops", None)
+    assert all(ops._registered(name) is None for name in ("gemm_i8", "grouped_gemm_wgrad"))

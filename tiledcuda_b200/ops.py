@@ -156,8 +156,11 @@ def _registered(name: str):
     global _registered_ops
     if _registered_ops is None:
         _registered_ops = {}
-        if _OP_LIB.exists():
+        try:
             torch.ops.load_library(os.fspath(_OP_LIB))
+        except OSError:
+            pass   # not built, or for another torch
+        else:
             for op in ("quantize_rows", "gemm_i8", "grouped_gemm", "grouped_gemm_i8", "grouped_gemm_dgrad", "grouped_gemm_wgrad"):
                 packet = getattr(torch.ops.tiledcuda, op, None)   # not in a library built before the op was there
                 if packet is not None:
