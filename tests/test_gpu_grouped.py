@@ -747,3 +747,43 @@ def test_refusals_on_device_tensors(cuda_ops):
         cuda_ops.grouped_gemm_i8(a.to(torch.int8), b.to(torch.int8), torch.ones(10, device=DEV), torch.ones(2, 48, device=DEV)[:, :24], off, c)
     with pytest.raises(TypeError, match="scale_a"):
         cuda_ops.gemm_i8(a.to(torch.int8), b[0].to(torch.int8), torch.ones(10, device=DEV, dtype=torch.float64), torch.ones(24, device=DEV), c)
+
+
+def test_calls_past_the_dispatcher(cuda_ops, clean_status):
+    """Plain tensors and parameters skip the dispatcher, with the same result; a subclass or a dispatch mode sees its call."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Seen(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            names.append(func.name())
+            return func(*args, **(kwargs or {}))
+
+    class Sub(torch.Tensor):
+        pass
+
+    g = gen(31)
+    sizes, n, k = [7, 0, 30], 72, 48
+    off = offsets_of(sizes)
+    a, b = halves(g, (sum(sizes), k), BF16), halves(g, (len(sizes), n, k), BF16)
+    c = [torch.full((sum(sizes), n), float("nan"), device=DEV) for _ in range(4)]
+    assert cuda_ops._registered("grouped_gemm") is not None
+    direct = cuda_ops._direct_calls["grouped_gemm"]
+    assert direct(a, torch.nn.Parameter(b), off, c[0]) is True
+    names = []
+    with Seen():
+        assert direct(a, b, off, c[1]) is False
+        cuda_ops.grouped_gemm(a, b, off, c[1])
+    assert names == ["tiledcuda::grouped_gemm"]
+    assert direct(a.as_subclass(Sub), b, off, c[2]) is False
+    cuda_ops.grouped_gemm(a.as_subclass(Sub), b, off, c[2])
+    assert direct(a, b, off[:-1], c[3]) is False and direct(a, b, off.cpu(), c[3]) is False and direct(a, b, off) is False
+    assert bool(c[3].isnan().all())
+    cuda_ops.grouped_gemm(a, b, off, c[3])
+    assert all(torch.equal(c[0], x) for x in c[1:])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):   # the current stream is the one the call goes to
+        c[1].fill_(float("nan"))
+        assert direct(a, b, off, c[1]) is True
+    side.synchronize()
+    assert torch.equal(c[0], c[1])

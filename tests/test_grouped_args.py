@@ -107,3 +107,12 @@ def test_an_op_library_that_does_not_load_leaves_the_other_route(tmp_path, monke
     monkeypatch.setattr(ops, "_OP_LIB", path)
     monkeypatch.setattr(ops, "_registered_ops", None)
     assert all(ops._registered(name) is None for name in ("gemm_i8", "grouped_gemm_wgrad"))
+
+
+def test_direct_calls_leave_what_is_not_for_them():
+    calls = pytest.importorskip("tiledcuda_b200._calls")
+    t = [torch.zeros(4, 16, dtype=torch.int8), torch.zeros(8, 16, dtype=torch.int8), torch.zeros(4), torch.zeros(8), torch.zeros(4, 8)]
+    assert calls.gemm_i8(*t) is False
+    assert calls.gemm_i8(*t[:4]) is False
+    assert calls.gemm_i8(None, *t[1:]) is False
+    assert calls.gemm_i8() is False

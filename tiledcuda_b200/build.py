@@ -1,7 +1,7 @@
 """Builds the in-tree native libraries with nvcc for sm_100a.
 
     python -m tiledcuda_b200.build            # libtiledcuda_b200.so (C ABI, no torch dependency)
-    python -m tiledcuda_b200.build --torch    # also libtiledcuda.so (torch.ops.tiledcuda.* registrations)
+    python -m tiledcuda_b200.build --torch    # also libtiledcuda.so (torch.ops.tiledcuda.* registrations) and _calls.so
 
 Objects land in tiledcuda_b200/build/, the shared libraries beside this file. A source is recompiled
 only when it, or a header it can include, is newer than its object.
@@ -13,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -21,6 +22,7 @@ CSRC = PKG / "csrc"
 OBJ = PKG / "build"
 LIB = PKG / "libtiledcuda_b200.so"
 TORCH_LIB = PKG / "libtiledcuda.so"
+CALLS_LIB = PKG / "_calls.so"
 
 KERNEL_SOURCES = ["host.cu", "scatter_nd.cu", "gemm.cu", "gemm_pair.cu", "gemm_host.cu", "quantize.cu", "grouped.cu", "grouped_pair.cu", "grouped_split.cu", "chain.cu", "attn.cu", "lstm.cu"]
 
@@ -73,16 +75,23 @@ def build_core(force: bool = False) -> Path:
 
 
 def build_torch(force: bool = False) -> Path:
-    """libtiledcuda.so: TORCH_LIBRARY(tiledcuda, ...) over the C ABI; links libtiledcuda_b200.so."""
+    """libtiledcuda.so: TORCH_LIBRARY(tiledcuda, ...) over the C ABI; links libtiledcuda_b200.so. And _calls.so, the Python
+    module that calls some of its functions without the dispatcher."""
+    build_core(force)
+    _build_torch_cc(CSRC / "torch_bind.cc", TORCH_LIB, LIB, ["-ltiledcuda_b200"], force)
+    _build_torch_cc(CSRC / "py_calls.cc", CALLS_LIB, TORCH_LIB, ["-l:libtiledcuda.so", "-ltiledcuda_b200", "-ltorch_python"], force,
+                    ["-I", sysconfig.get_paths()["include"]])
+    return TORCH_LIB
+
+
+def _build_torch_cc(src: Path, lib: Path, needs: Path, links: list[str], force: bool, extra: list[str] = []) -> None:
     import torch
     from torch.utils import cpp_extension
 
-    build_core(force)
-    src = CSRC / "torch_bind.cc"
-    newest = max(src.stat().st_mtime, _headers_mtime(), LIB.stat().st_mtime)
-    if not force and TORCH_LIB.exists() and TORCH_LIB.stat().st_mtime >= newest:
-        return TORCH_LIB
-    inc = []
+    newest = max(src.stat().st_mtime, _headers_mtime(), needs.stat().st_mtime)
+    if not force and lib.exists() and lib.stat().st_mtime >= newest:
+        return
+    inc = list(extra)
     for p in cpp_extension.include_paths():
         inc += ["-I", p]
     torch_lib_dir = os.path.join(os.path.dirname(torch.__file__), "lib")
@@ -90,15 +99,14 @@ def build_torch(force: bool = False) -> Path:
         "g++", "-O2", "-std=c++17", "-fPIC", "-shared", *inc,
         "-I", "/usr/local/cuda/include",
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-        str(src), "-o", str(TORCH_LIB),
-        f"-L{PKG}", "-ltiledcuda_b200", "-Wl,-rpath,$ORIGIN",
+        str(src), "-o", str(lib),
+        f"-L{PKG}", *links, "-Wl,-rpath,$ORIGIN",
         f"-L{torch_lib_dir}", "-lc10", "-ltorch_cpu", "-ltorch", "-lc10_cuda",
         f"-Wl,-rpath,{torch_lib_dir}",
     ]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"torch binding build failed:\n{res.stderr[-6000:]}")
-    return TORCH_LIB
 
 
 TILE_INCLUDE = PKG / "include"

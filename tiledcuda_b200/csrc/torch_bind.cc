@@ -14,6 +14,7 @@
 #include <vector>
 
 #include "../../include/tiledcuda_b200.h"
+#include "torch_ops.h"
 
 namespace {
 
@@ -234,7 +235,11 @@ int wide_offsets(const char* op, const at::Tensor& offsets, int64_t experts) {
     return offsets.scalar_type() == at::kLong ? 1 : 0;
 }
 
-void quantize_rows_op(const at::Tensor& x, at::Tensor& q, at::Tensor& scale) {
+}  // namespace
+
+namespace tiledcuda {
+
+void quantize_rows(const at::Tensor& x, at::Tensor& q, at::Tensor& scale) {
     const char* op = "quantize_rows";
     TORCH_CHECK(x.dim() == 2, op, ": x must be 2-D");
     need_rows(op, "x", x, x.sizes(), x.scalar_type() == at::kFloat || is_half(x));
@@ -246,7 +251,7 @@ void quantize_rows_op(const at::Tensor& x, at::Tensor& q, at::Tensor& scale) {
                                stream_of(x)));
 }
 
-void gemm_i8_op(const at::Tensor& A, const at::Tensor& B, const at::Tensor& scale_a, const at::Tensor& scale_b, at::Tensor& C) {
+void gemm_i8(const at::Tensor& A, const at::Tensor& B, const at::Tensor& scale_a, const at::Tensor& scale_b, at::Tensor& C) {
     const char* op = "gemm_i8";
     TORCH_CHECK(A.dim() == 2 && B.dim() == 2, op, ": A and B must be 2-D");
     const int64_t m = A.size(0), k = A.size(1), n = B.size(0);
@@ -261,7 +266,7 @@ void gemm_i8_op(const at::Tensor& A, const at::Tensor& B, const at::Tensor& scal
                          ld(B, 0, 16), ld(C, 0), type_code(C), stream_of(A)));
 }
 
-void grouped_gemm_op(const at::Tensor& A, const at::Tensor& B, const at::Tensor& offsets, at::Tensor& C) {
+void grouped_gemm(const at::Tensor& A, const at::Tensor& B, const at::Tensor& offsets, at::Tensor& C) {
     const char* op = "grouped_gemm";
     TORCH_CHECK(A.dim() == 2 && B.dim() == 3, op, ": A must be 2-D and B 3-D");
     const int64_t t = A.size(0), k = A.size(1), e = B.size(0), n = B.size(1);
@@ -275,7 +280,7 @@ void grouped_gemm_op(const at::Tensor& A, const at::Tensor& B, const at::Tensor&
                               ld(B, 0, 8), ld(C, 0), type_code(A), type_code(C), stream_of(A)));
 }
 
-void grouped_gemm_i8_op(const at::Tensor& A, const at::Tensor& B, const at::Tensor& scale_a, const at::Tensor& scale_b,
+void grouped_gemm_i8(const at::Tensor& A, const at::Tensor& B, const at::Tensor& scale_a, const at::Tensor& scale_b,
                         const at::Tensor& offsets, at::Tensor& C) {
     const char* op = "grouped_gemm_i8";
     TORCH_CHECK(A.dim() == 2 && B.dim() == 3, op, ": A must be 2-D and B 3-D");
@@ -293,7 +298,7 @@ void grouped_gemm_i8_op(const at::Tensor& A, const at::Tensor& B, const at::Tens
                                  C.data_ptr(), t, e, n, k, ld(A, 0, 16), ld(B, 1, 16), ld(B, 0, 16), ld(C, 0), type_code(C), stream_of(A)));
 }
 
-void grouped_gemm_dgrad_op(const at::Tensor& dC, const at::Tensor& B, const at::Tensor& offsets, at::Tensor& dA) {
+void grouped_gemm_dgrad(const at::Tensor& dC, const at::Tensor& B, const at::Tensor& offsets, at::Tensor& dA) {
     const char* op = "grouped_gemm_dgrad";
     TORCH_CHECK(dC.dim() == 2 && B.dim() == 3, op, ": dC must be 2-D and B 3-D");
     const int64_t t = dC.size(0), n = dC.size(1), e = B.size(0), k = B.size(2);
@@ -307,7 +312,7 @@ void grouped_gemm_dgrad_op(const at::Tensor& dC, const at::Tensor& B, const at::
                                     ld(B, 0, 8), ld(dA, 0), type_code(dC), type_code(dA), stream_of(dC)));
 }
 
-void grouped_gemm_wgrad_op(const at::Tensor& dC, const at::Tensor& A, const at::Tensor& offsets, at::Tensor& dB) {
+void grouped_gemm_wgrad(const at::Tensor& dC, const at::Tensor& A, const at::Tensor& offsets, at::Tensor& dB) {
     const char* op = "grouped_gemm_wgrad";
     TORCH_CHECK(dC.dim() == 2 && A.dim() == 2 && dB.dim() == 3, op, ": dC and A must be 2-D and dB 3-D");
     const int64_t t = dC.size(0), n = dC.size(1), e = dB.size(0), k = A.size(1);
@@ -321,7 +326,7 @@ void grouped_gemm_wgrad_op(const at::Tensor& dC, const at::Tensor& A, const at::
                                     ld(dB, 1), ld(dB, 0), type_code(dC), type_code(dB), stream_of(dC)));
 }
 
-}  // namespace
+}  // namespace tiledcuda
 
 TORCH_LIBRARY(tiledcuda, m) {
     m.def("scatter_nd(Tensor(a!) data, Tensor updates, Tensor indices) -> ()");
@@ -350,12 +355,12 @@ TORCH_LIBRARY_IMPL(tiledcuda, CUDA, m) {
     m.impl("gemm", &gemm_op);
     m.impl("back2back_gemm", &back2back_gemm_op);
     m.impl("lstm_cell", &lstm_cell_op);
-    m.impl("quantize_rows", &quantize_rows_op);
-    m.impl("gemm_i8", &gemm_i8_op);
-    m.impl("grouped_gemm", &grouped_gemm_op);
-    m.impl("grouped_gemm_i8", &grouped_gemm_i8_op);
-    m.impl("grouped_gemm_dgrad", &grouped_gemm_dgrad_op);
-    m.impl("grouped_gemm_wgrad", &grouped_gemm_wgrad_op);
+    m.impl("quantize_rows", &tiledcuda::quantize_rows);
+    m.impl("gemm_i8", &tiledcuda::gemm_i8);
+    m.impl("grouped_gemm", &tiledcuda::grouped_gemm);
+    m.impl("grouped_gemm_i8", &tiledcuda::grouped_gemm_i8);
+    m.impl("grouped_gemm_dgrad", &tiledcuda::grouped_gemm_dgrad);
+    m.impl("grouped_gemm_wgrad", &tiledcuda::grouped_gemm_wgrad);
 }
 
 // The grouped and 8-bit products take no part in autograd (their gradients are operators of their own): parameters that

@@ -1,0 +1,17 @@
+// The grouped and 8-bit products as functions of tensors (torch_bind.cc): their checks, then the call of the C ABI on the
+// tensors' device and its current stream. A refusal is a c10::Error.
+#pragma once
+
+#include <ATen/core/Tensor.h>
+
+namespace tiledcuda {
+
+void quantize_rows(const at::Tensor& x, at::Tensor& q, at::Tensor& scale);
+void gemm_i8(const at::Tensor& A, const at::Tensor& B, const at::Tensor& scale_a, const at::Tensor& scale_b, at::Tensor& C);
+void grouped_gemm(const at::Tensor& A, const at::Tensor& B, const at::Tensor& offsets, at::Tensor& C);
+void grouped_gemm_i8(const at::Tensor& A, const at::Tensor& B, const at::Tensor& scale_a, const at::Tensor& scale_b,
+                     const at::Tensor& offsets, at::Tensor& C);
+void grouped_gemm_dgrad(const at::Tensor& dC, const at::Tensor& B, const at::Tensor& offsets, at::Tensor& dA);
+void grouped_gemm_wgrad(const at::Tensor& dC, const at::Tensor& A, const at::Tensor& offsets, at::Tensor& dB);
+
+}  // namespace tiledcuda
