@@ -76,11 +76,13 @@ def build_core(force: bool = False) -> Path:
 
 def build_torch(force: bool = False) -> Path:
     """libtiledcuda.so: TORCH_LIBRARY(tiledcuda, ...) over the C ABI; links libtiledcuda_b200.so. And _calls.so, the Python
-    module that calls some of its functions without the dispatcher."""
+    module that calls some of its functions without the dispatcher (left out where Python's headers are not installed)."""
     build_core(force)
     _build_torch_cc(CSRC / "torch_bind.cc", TORCH_LIB, LIB, ["-ltiledcuda_b200"], force)
-    _build_torch_cc(CSRC / "py_calls.cc", CALLS_LIB, TORCH_LIB, ["-l:libtiledcuda.so", "-ltiledcuda_b200", "-ltorch_python"], force,
-                    ["-I", sysconfig.get_paths()["include"]])
+    python_include = sysconfig.get_paths()["include"]
+    if os.path.exists(os.path.join(python_include, "Python.h")):
+        _build_torch_cc(CSRC / "py_calls.cc", CALLS_LIB, TORCH_LIB, ["-l:libtiledcuda.so", "-ltiledcuda_b200", "-ltorch_python"], force,
+                        ["-I", python_include])
     return TORCH_LIB
 
 
