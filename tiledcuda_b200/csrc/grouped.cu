@@ -111,10 +111,13 @@ static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // The kernel and tile for a problem, from its sizes alone; of the offsets the host knows nothing, so the rule takes the
 // rows to be spread evenly. Times below in us: B200, CUDA graph replays, three sets of operands in turn.
-//  * Pair tiles (256 columns x up to 256 rows) once there are enough of them for the 74 pairs and the groups have 128
-//    rows or more to fill them: 32 experts x [4096,1024] with 4096 rows 58 against 67 in the split kernel, weight gradient
-//    of 16 x [2048,1024] 30 against 46. With 64 tiles the split kernel is ahead for one dense product (int8 2048^3 9.4
-//    against 11.5), the pair kernel where each group brings its own weights (8 x [2048,1024], 2048 rows: 17.8 against 18.5).
+//  * Pair tiles (256 columns x up to 256 rows) once there are more of them than the 74 pairs, and the groups have 128 rows or
+//    more to fill them: 32 experts x [4096,1024] with 4096 rows 58 against 67 in the split kernel, int8 2048 x 2560 x 2048 (80
+//    tiles) 14.9 against 15.7, weight gradient of one [2048,2560] from 2048 rows 26.7 against 30.2; a short sum gains nothing
+//    (int8 2048 x 2432 x 512 9.3 against 8.8). With 64 tiles the split kernel, of whose tiles two run on an SM, is ahead for
+//    one dense product (int8 2048^3 9.4 against 11.1) and for a few large groups (input gradient of 4 x [1280,1024], 4096 rows:
+//    13.3 against 17.8), the pair kernel where groups of up to 256 rows bring weights of their own and come out uneven
+//    (16 x [1024,2048], 4096 rows: 28.4 against 31.1).
 //  * Else the split kernel. Where the weights' bytes count (few rows per group), a tile takes all rows of a group up to
 //    four times the even share, so that a popular expert's weights are read once: 16 x [2048,2048] with 512 rows 24.6
 //    with 128-row tiles against 29.7 with 32.
@@ -134,7 +137,7 @@ static GroupedPlan grouped_plan(const GroupedProblem& g, int sm_count) {
     GroupedPlan p;
     p.splits = 1;
     const bool own_weights = groups > 1 && !g.ragged_x;
-    p.pair = rows >= 128 && tiles(256, 256) >= (own_weights ? 64 : 100);
+    p.pair = rows >= 128 && (tiles(256, 256) > sm_count / 2 || (own_weights && share <= 256 && tiles(256, 256) >= 64));
     if (p.pair) {
         p.tile_rows = 256;
     } else {
