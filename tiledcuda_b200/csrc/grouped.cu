@@ -3,6 +3,8 @@
 #include "grouped.h"
 #include "sm100.cuh"
 
+#include <algorithm>
+
 namespace tcb {
 
 static bool half_type(int t) { return t == TC_F16 || t == TC_BF16; }
@@ -111,13 +113,16 @@ static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // The kernel and tile for a problem, from its sizes alone; of the offsets the host knows nothing, so the rule takes the
 // rows to be spread evenly. Times below in us: B200, CUDA graph replays, three sets of operands in turn.
-//  * Pair tiles (256 columns x up to 256 rows) once there are more of them than the 74 pairs, and the groups have 128 rows or
-//    more to fill them: 32 experts x [4096,1024] with 4096 rows 58 against 67 in the split kernel, int8 2048 x 2560 x 2048 (80
-//    tiles) 14.9 against 15.7, weight gradient of one [2048,2560] from 2048 rows 26.7 against 30.2; a short sum gains nothing
-//    (int8 2048 x 2432 x 512 9.3 against 8.8). With 64 tiles the split kernel, of whose tiles two run on an SM, is ahead for
-//    one dense product (int8 2048^3 9.4 against 11.1) and for a few large groups (input gradient of 4 x [1280,1024], 4096 rows:
-//    13.3 against 17.8), the pair kernel where groups of up to 256 rows bring weights of their own and come out uneven
-//    (16 x [1024,2048], 4096 rows: 28.4 against 31.1).
+//  * One group, and the weight gradient: pair tiles (256 columns x up to 256 rows) once there are more of them than the 74 pairs
+//    and 128 rows or more to fill them: int8 2048 x 2560 x 2048 (80 tiles) 14.9 against 15.7 in the split kernel, weight
+//    gradient of one [2048,2560] from 2048 rows 26.7 against 30.2; a short sum gains nothing (int8 2048 x 2432 x 512 9.3 against
+//    8.8), and with 64 tiles the split kernel, of whose tiles two run on an SM, is ahead (int8 2048^3 9.4 against 11.1).
+//  * Groups with weights of their own come out uneven: half a tile of each counts as wasted. The split kernel as long as its
+//    tiles of 128 rows all run at once, two per SM (1600 rows, 12 x [2048,2048]: 23.7 against 29.2 in two unequal waves of pair
+//    tiles; input gradient of 7 x [512,1536], 2048 rows: 7.7 against 9.0), or nearly so where groups of fewer than 128 rows leave half of a
+//    pair tile empty (2500 rows, 20 x [1408,2048]: 26.0 against 29.4); beyond that pair tiles (4096 rows, 16 x [1024,2048]: 28.4
+//    against 31.1; 2000 rows, 16 x [2048,2048]: 31.4 against 37.7; 6400 rows, 64 x [2048,1024]: 55 against 65), but not for
+//    fewer than 96 rows a group (1024 rows, 16 x [4096,2048]: 52.9 against 48.9).
 //  * Else the split kernel. Where the weights' bytes count (few rows per group), a tile takes all rows of a group up to
 //    four times the even share, so that a popular expert's weights are read once: 16 x [2048,2048] with 512 rows 24.6
 //    with 128-row tiles against 29.7 with 32.
@@ -137,7 +142,9 @@ static GroupedPlan grouped_plan(const GroupedProblem& g, int sm_count) {
     GroupedPlan p;
     p.splits = 1;
     const bool own_weights = groups > 1 && !g.ragged_x;
-    p.pair = rows >= 128 && (tiles(256, 256) > sm_count / 2 || (own_weights && share <= 256 && tiles(256, 256) >= 64));
+    const int64_t lone2 = std::max(2 * groups, g.token_rows / 64 + groups) * ceil_div(g.cols, 128);   // twice the split kernel's tiles
+    p.pair = own_weights ? share >= 96 && 100 * lone2 > (share >= 128 ? 100 : 118) * 4 * sm_count
+                         : rows >= 128 && tiles(256, 256) > sm_count / 2;
     if (p.pair) {
         p.tile_rows = 256;
     } else {
