@@ -787,3 +787,63 @@ def test_calls_past_the_dispatcher(cuda_ops, clean_status):
         assert direct(a, b, off, c[1]) is True
     side.synchronize()
     assert torch.equal(c[0], c[1])
+
+
+# Few output tiles and long sums: the sum is cut into two, four or eight pieces, the last of them shorter or empty.
+@pytest.mark.parametrize("m,n,k", [(300, 1024, 8192), (290, 1000, 6160), (1, 4096, 4096), (33, 128, 8208), (64, 500, 9000)])
+def test_gemm_i8_sums_in_pieces(cuda_ops, clean_status, m, n, k):
+    g = gen(32)
+    a, b = ints(g, (m, k)), ints(g, (n, k))
+    sa, sb = torch.rand(m, generator=g, device=DEV) + 0.5, torch.rand(n, generator=g, device=DEV) + 0.5
+    c = torch.full((m, n), float("nan"), device=DEV)
+    cuda_ops.gemm_i8(a, b, sa, sb, c)
+    exact = i8_exact(a, b, sa, sb)
+    assert_within(c, exact, exact.abs() * 3.01 * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("sizes,start,behind,n,x", [([300], 0, 0, 1024, 3136), ([290], 4, 3, 1000, 3400), ([30, 20, 0, 14], 1, 2, 300, 3200),
+                                                    ([2, 1], 0, 0, 200, 5000), ([64], 0, 0, 512, 4200)])
+def test_grouped_sums_in_pieces(cuda_ops, clean_status, sizes, start, behind, n, x):
+    g = gen(33)
+    total, off = start + sum(sizes) + behind, offsets_of(sizes, start)
+    a, b = halves(g, (total, x), BF16), halves(g, (len(sizes), n, x), BF16)
+    mask = inside(total, sizes, start)
+    a[~mask] = math.nan
+    exact, s = plain_forward(a, b, sizes, start)
+    c = torch.full((total, n), -7.0, device=DEV)
+    cuda_ops.grouped_gemm(a, b, off, c)
+    assert_within(c[mask], exact[mask], product_error(s[mask], x))
+    da = torch.full((total, n), -7.0, device=DEV)
+    bt = torch.empty(len(sizes), x, -(-n // 8) * 8, dtype=BF16, device=DEV)[..., :n]
+    bt.copy_(b.transpose(1, 2))
+    cuda_ops.grouped_gemm_dgrad(a, bt, off, da)
+    assert_within(da[mask], exact[mask], product_error(s[mask], x))
+    assert (c[~mask] == -7.0).all() and (da[~mask] == -7.0).all()
+
+
+@pytest.mark.parametrize("sizes,start,n,k", [([3200], 0, 512, 640), ([4096], 3, 512, 512), ([4001, 3000], 0, 320, 300), ([3333], 0, 500, 600)])
+def test_wgrad_sums_in_pieces(cuda_ops, clean_status, sizes, start, n, k):
+    g = gen(34)
+    total = start + sum(sizes)
+    dc, a = halves(g, (total, n), F16), halves(g, (total, k), F16)
+    db = torch.full((len(sizes), n, k), math.nan, device=DEV)
+    cuda_ops.grouped_gemm_wgrad(dc, a, offsets_of(sizes, start), db)
+    exact, s = plain_wgrad(dc, a, sizes, start)
+    assert_within(db, exact, product_error(s, max(sizes)))
+
+
+# Around the size where groups with weights of their own change from lone tiles to pairs.
+@pytest.mark.parametrize("sizes", [[125] * 16, [100] * 16, [250, 3, 0, 128, 129, 300, 1, 127, 64, 400, 0, 33, 90, 75], [95] * 20, [97] * 20])
+@pytest.mark.parametrize("n", [1400, 2056])
+def test_uneven_groups_of_about_a_tile(cuda_ops, clean_status, sizes, n):
+    g = gen(35)
+    k, total, off = 136, sum(sizes) + 2, offsets_of(sizes, 1)
+    a, b = halves(g, (total, k), F16), halves(g, (len(sizes), n, k), F16)
+    mask = inside(total, sizes, 1)
+    exact, s = plain_forward(a, b, sizes, 1)
+    c, da = torch.full((total, n), -7.0, dtype=F16, device=DEV), torch.full((total, n), -7.0, dtype=F16, device=DEV)
+    cuda_ops.grouped_gemm(a, b, off, c)
+    cuda_ops.grouped_gemm_dgrad(a, b.transpose(1, 2).contiguous(), off, da)
+    for got in (c, da):
+        assert_within(got[mask], exact[mask], product_error(s[mask], k))
+        assert (got[~mask] == -7.0).all()

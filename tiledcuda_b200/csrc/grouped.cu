@@ -112,17 +112,17 @@ int grouped_map_q(CUtensorMap* map, const GroupedProblem& g, int box_rows) {
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // The kernel and tile for a problem, from its sizes alone; of the offsets the host knows nothing, so the rule takes the
-// rows to be spread evenly. Times below in us: B200, CUDA graph replays, three sets of operands in turn.
+// rows to be spread evenly, or nearly so. Times below in us: B200, CUDA graph replays, three sets of operands in turn.
 //  * One group, and the weight gradient: pair tiles (256 columns x up to 256 rows) once there are more of them than the 74 pairs
 //    and 128 rows or more to fill them: int8 2048 x 2560 x 2048 (80 tiles) 14.9 against 15.7 in the split kernel, weight
 //    gradient of one [2048,2560] from 2048 rows 26.7 against 30.2; a short sum gains nothing (int8 2048 x 2432 x 512 9.3 against
 //    8.8), and with 64 tiles the split kernel, of whose tiles two run on an SM, is ahead (int8 2048^3 9.4 against 11.1).
 //  * Groups with weights of their own come out uneven: half a tile of each counts as wasted. The split kernel as long as its
 //    tiles of 128 rows all run at once, two per SM (1600 rows, 12 x [2048,2048]: 23.7 against 29.2 in two unequal waves of pair
-//    tiles; input gradient of 7 x [512,1536], 2048 rows: 7.7 against 9.0), or nearly so where groups of fewer than 128 rows leave half of a
-//    pair tile empty (2500 rows, 20 x [1408,2048]: 26.0 against 29.4); beyond that pair tiles (4096 rows, 16 x [1024,2048]: 28.4
-//    against 31.1; 2000 rows, 16 x [2048,2048]: 31.4 against 37.7; 6400 rows, 64 x [2048,1024]: 55 against 65), but not for
-//    fewer than 96 rows a group (1024 rows, 16 x [4096,2048]: 52.9 against 48.9).
+//    tiles; input gradient of 7 x [512,1536], 2048 rows: 7.7 against 9.0), or nearly so where groups of fewer than 128 rows
+//    leave half of a pair tile empty (2500 rows, 20 x [1408,2048]: 26.0 against 29.4). Beyond that pair tiles (4096 rows, 16 x
+//    [1024,2048]: 28.4 against 31.1; 2000 rows, 16 x [2048,2048]: 31.4 against 37.7; 6400 rows, 64 x [2048,1024]: 55 against
+//    65), but not for fewer than 96 rows a group (1024 rows, 16 x [4096,2048]: 52.9 against 48.9).
 //  * Else the split kernel. Where the weights' bytes count (few rows per group), a tile takes all rows of a group up to
 //    four times the even share, so that a popular expert's weights are read once: 16 x [2048,2048] with 512 rows 24.6
 //    with 128-row tiles against 29.7 with 32.
