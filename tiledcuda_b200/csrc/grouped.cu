@@ -167,7 +167,11 @@ static GroupedPlan grouped_plan(const GroupedProblem& g, int sm_count) {
     p.tiles = p.row_tiles * ceil_div(g.cols, p.pair ? 256 : 128);
     // The split kernel's CTAs get an SM each, and the ring of one, when they need no more: a few beyond the SMs, of which
     // some will find no tile, do not change that (9 experts x [1001,776], 1333 rows: 152 CTAs 10.8 alone, 14.3 two to an SM).
-    p.alone = tiles(p.tile_rows, 128) * p.splits <= sm_count && 10 * p.tiles * p.splits <= 11 * sm_count;
+    // So it is where the bound is well above the SMs but the tiles of uneven groups probably are not (2600 rows, 13 x [640,2048]
+    // 12.7 and 17.0; 1500 rows, 14 x [896,1024] 8.5 and 10.8); nearer to the SMs a second wave would cost what the ring gains
+    // (1900 rows, 11 x [896,2048], for three spreads of the rows 19.8, 20.3, 12.9 alone, 17.4, 16.9, 17.4 two to an SM).
+    p.alone = (tiles(p.tile_rows, 128) * p.splits <= sm_count && 10 * p.tiles * p.splits <= 11 * sm_count) ||
+              (own_weights && p.tile_rows == 128 && p.splits == 1 && 10 * lone2 <= 18 * sm_count && 4 * p.tiles <= 5 * sm_count);
     return p;
 }
 
