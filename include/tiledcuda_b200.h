@@ -110,7 +110,10 @@ int tc_gemm_i8(const void* A, const void* B, const float* scale_a, const float* 
 /* Matrix products grouped by expert. The rows of A are sorted by expert: expert e owns rows offsets[e] up to (not
  * including) offsets[e+1], and  C[t,:] = A[t,:] B[e]^T  for its rows t. A [rows,K] (lda) and C [rows,N] (ldc) row-major,
  * B [experts,N,K] with row stride ldb and expert stride stride_b (elements); A and B are of in_type (TC_F16 or TC_BF16),
- * fp32 accumulation, C is rounded once to c_type (in_type or TC_F32). offsets is DEVICE memory, experts + 1 integers
+ * fp32 accumulation, C is rounded once to c_type (in_type or TC_F32). The tensor cores' accumulators cut instead of rounding, which
+ * costs a sum of L terms of one sign about L * 6.5e-9 of it; sums of more than 8192 terms are therefore formed in pieces of
+ * at most that length, each joined to the others with one rounding to nearest (2^-24), so that before the rounding to c_type a sum
+ * of any length is off by about 6e-5 of sum |a||b| at most. offsets is DEVICE memory, experts + 1 integers
  * (int64 when offsets_are_int64 else int32), nondecreasing and within [0, rows]: the host never reads them, so sizes
  * decided by a router on the device need no synchronisation. Empty experts are fine; rows before offsets[0] and from
  * offsets[experts] on are not read into any result and their rows of C stay as they were. Offsets outside
@@ -140,7 +143,8 @@ int tc_grouped_gemm_dgrad(const void* dC, const void* B, const void* offsets, in
 
 /* Gradient of tc_grouped_gemm to B: dB[e] = sum over the rows t of expert e of dC[t,:]^T A[t,:], the whole of dB
  * [experts,N,K] (row stride lddb, expert stride stride_db): an expert without rows gets zeros. rows <= 2^27. Rows outside
- * all groups take no part, whatever they hold. The sum runs over the rows in order, so the result does not change from run to run.
+ * all groups take no part, whatever they hold. A sum is formed of consecutive pieces of the group's rows, joined in order; how it is
+ * cut follows from the sizes, the offsets and the device's number of SMs, so the result does not change from run to run on a device.
  * Needs lddc and lda multiples of 16 bytes. The reference has no backward pass; no counterpart there. */
 int tc_grouped_gemm_wgrad(const void* dC, const void* A, const void* offsets, int offsets_are_int64, void* dB,
                           int64_t rows, int64_t experts, int64_t N, int64_t K, int64_t lddc, int64_t lda, int64_t lddb,

@@ -847,3 +847,84 @@ def test_uneven_groups_of_about_a_tile(cuda_ops, clean_status, sizes, n):
     for got in (c, da):
         assert_within(got[mask], exact[mask], product_error(s[mask], k))
         assert (got[~mask] == -7.0).all()
+
+
+# Sums of more than 8192 terms run in pieces of that length, joined in fp32 to nearest: a piece is off as product_error says, and
+# each joining by half a step of the total. One accumulator for the whole sum would be off by 2e-3 of it at 2^20 terms of one sign.
+def long_product_error(s, terms):
+    return product_error(s, min(terms, 8192)) + -(-terms // 8192) * 2.0 ** -24 * s
+
+
+def uniform(g, shape, dtype):
+    """Values of one sign with full mantissas, in rows that start on 16-byte boundaries."""
+    ld = -(-shape[-1] // 8) * 8
+    return (torch.rand(*shape[:-1], ld, generator=g, device=DEV) * 0.5 + 0.5).to(dtype)[..., :shape[-1]]
+
+
+def exact_t(x, y):
+    """x^T y in 64 bits, a few rows at a time."""
+    out = torch.zeros(x.shape[1], y.shape[1], dtype=torch.float64, device=DEV)
+    for i in range(0, x.shape[0], 1 << 14):
+        out += x[i:i + (1 << 14)].double().t() @ y[i:i + (1 << 14)].double()
+    return out
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("terms,n,k", [(1 << 20, 40, 64), (300007, 136, 24), (65536 + 17, 16, 8), (8192 * 9 + 1, 328, 72)])
+def test_long_sums_keep_fp32_accuracy(cuda_ops, clean_status, terms, n, k, dtype):
+    g = gen(40)
+    dc, a = uniform(g, (terms, n), dtype), uniform(g, (terms, k), dtype)
+    exact = exact_t(dc, a)
+    db = torch.empty(1, n, k, device=DEV)
+    cuda_ops.grouped_gemm_wgrad(dc, a, offsets_of([terms]), db)
+    assert_within(db[0], exact, long_product_error(exact, terms))
+    x = torch.zeros(n + 2, -(-terms // 8) * 8, dtype=dtype, device=DEV)[1:-1, :terms]
+    x.copy_(dc.t())
+    w = torch.zeros(1, k, -(-terms // 8) * 8, dtype=dtype, device=DEV)[..., :terms]
+    w.copy_(a.t())
+    c = torch.empty(n, k, device=DEV)
+    cuda_ops.grouped_gemm(x, w, offsets_of([n]), c)
+    assert_within(c, exact, long_product_error(exact, terms))
+    c.fill_(math.nan)
+    cuda_ops.grouped_gemm_dgrad(x, a[None], offsets_of([n]), c)
+    assert_within(c, exact, long_product_error(exact, terms))
+
+
+# Groups on both sides of one, two and three pieces in one call, in the split kernel (whose CTAs may take a part of a sum each)
+# and, with enough output tiles, in the kernel of CTA pairs, where short sums follow long ones through the same accumulators.
+@pytest.mark.parametrize("dtype,out", [(F16, F32), (BF16, BF16)])
+@pytest.mark.parametrize("n,k", [(100, 72), (1300, 776)])
+def test_wgrad_of_long_and_short_groups(cuda_ops, clean_status, n, k, dtype, out):
+    sizes = [20000, 40, 8192, 8193, 0, 16384, 8207, 16389, 24576 + 5, 100, 8192 + 128, 3]
+    g = gen(41)
+    total, start = sum(sizes) + 9, 5
+    dc, a = uniform(g, (total, n), dtype), uniform(g, (total, k), dtype)
+    mask = inside(total, sizes, start)
+    dc[~mask] = math.nan
+    db = torch.full((len(sizes), n, k), math.nan, dtype=out, device=DEV)
+    cuda_ops.grouped_gemm_wgrad(dc, a, offsets_of(sizes, start), db)
+    at = start
+    for e, size in enumerate(sizes):
+        exact = exact_t(dc[at:at + size], a[at:at + size])
+        assert_within(db[e], exact, long_product_error(exact, size))
+        at += size
+
+
+@pytest.mark.parametrize("sizes,n", [([3, 0, 20], 72), ([700, 250, 0, 1100], 2600)])
+@pytest.mark.parametrize("x", [8192, 16392, 24600])
+def test_forward_and_dgrad_of_long_sums(cuda_ops, clean_status, sizes, n, x):
+    g = gen(42)
+    total, off = sum(sizes) + 4, offsets_of(sizes, 2)
+    a, b = uniform(g, (total, x), F16), uniform(g, (len(sizes), n, x), F16)
+    mask = inside(total, sizes, 2)
+    a[~mask] = math.nan
+    exact = torch.zeros(total, n, dtype=torch.float64, device=DEV)
+    at = 2
+    for e, size in enumerate(sizes):
+        exact[at:at + size] = a[at:at + size].double() @ b[e].double().t()
+        at += size
+    for call, w in ((cuda_ops.grouped_gemm, b), (cuda_ops.grouped_gemm_dgrad, b.transpose(1, 2).contiguous())):
+        c = torch.full((total, n), -7.0, device=DEV)
+        call(a, w, off, c)
+        assert_within(c[mask], exact[mask], long_product_error(exact[mask], x))
+        assert (c[~mask] == -7.0).all()

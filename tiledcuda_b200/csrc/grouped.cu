@@ -23,8 +23,8 @@ static int check_sizes(const char* op, int64_t rows, int64_t experts, int64_t N,
     return TC_OK;
 }
 
-// One CTA runs a whole sum; a bounded wait of another warp for it ends after two seconds, which is well above a second of
-// loads at most for this many terms.
+// What the joining of pieces (kSumPiece) leaves uncertain grows by 2^-24 a piece, 2^-10 of the sum of magnitudes for this many
+// terms.
 static int check_terms(const char* op, const char* name, int64_t terms) {
     if (terms > (1ll << 27)) return fail(TC_ERR_UNSUPPORTED, "%s: sums over %s = %lld terms, at most %lld are supported", op, name, (long long)terms, 1ll << 27);
     return TC_OK;

@@ -136,6 +136,36 @@ __device__ __forceinline__ GroupTile group_tile(const GroupTable* t, const Group
     return banded_tile<false>(a, lo, t->first[lo], t->len[lo], tile - before * col_tiles, t->tiles_before[lo + 1] - before, col_tiles, tile_cols);
 }
 
+// 16-bit operands: the tensor cores cut what they add to an accumulator, at about 2^-24 of it on average in each step of 16
+// terms, always towards zero. Over a long sum of one sign that adds up (2^20 terms in one accumulator: 2e-3 of the sum), so an
+// accumulator takes 8192 terms at most, 5e-5; the pieces of a longer sum are added in fp32 to nearest, in order, and kept
+// in TMEM columns beside the accumulator. An epilogue warp does so for the lanes and columns that it drains.
+constexpr int kSumPiece = 8192;
+
+// One piece of a long sum: total = acc for the first, total += acc for those between, acc += total for the last. Of the
+// tile's rows (TMEM columns) those that this warp drains: `block` of them (16 or 32) from `first` on, then `step` on.
+static __device__ __noinline__ void add_sum_piece(uint32_t acc, uint32_t total, bool is_first, bool is_last, int rows, int first, int step,
+                                                  int block) {
+    for (int j0 = first; j0 < rows; j0 += step) {
+        for (int j = j0; j < min(rows, j0 + block); j += 16) {
+            uint32_t v[16];
+            __syncwarp();
+            tmem_ld_x16(acc + static_cast<uint32_t>(j), v);
+            if (!is_first) {
+                uint32_t t[16];
+                tmem_ld_x16(total + static_cast<uint32_t>(j), t);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(t[i]) + __uint_as_float(v[i]));
+            } else {
+                tmem_ld_wait();
+            }
+            tmem_st_x16((is_last ? acc : total) + static_cast<uint32_t>(j), v);
+        }
+    }
+    tmem_st_wait();
+}
+
 __device__ __forceinline__ uint16_t to_half_bits(float v, int type) {
     return type == TC_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
 }

@@ -14,8 +14,9 @@
 //               zero whatever they hold (NaN included), in both operands. Such a step has a buffer of its own, loaded when
 //               the producer starts the tile; this warp overwrites the foreign rows with zeros long before the MMA issuer
 //               comes to it. (Cleared in the ring instead, it held up every tile by about 1000 cycles.)
-// Persistent over tiles; accumulators are double-buffered in TMEM. Which tiles there are follows from the offsets, which
-// every CTA reads from device memory into a table at the start.
+// Persistent over tiles; accumulators are double-buffered in TMEM, except for a tile whose sum is longer than kSumPiece: its
+// pieces all go through one accumulator, and the columns of the other one hold their total. Which tiles there are follows from
+// the offsets, which every CTA reads from device memory into a table at the start.
 #include "grouped.cuh"
 
 namespace tcb {
@@ -92,13 +93,33 @@ __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorM
         : "memory");
 }
 
-template <bool kI8, bool kPCols, bool kRaggedX>
+// The epilogue's part in a tile whose sum comes in `before_last` + 1 pieces: waits for each, adds it to the total, and leaves the
+// whole sum in the accumulator. One warp; false when a wait ran out.
+static __device__ __noinline__ bool join_pieces(uint32_t acc, uint32_t total, uint64_t* bar_full, uint64_t* bar_empty, uint32_t parity,
+                                                int before_last, int rows, int first, volatile uint32_t* abort_word) {
+    for (int piece = 0;; ++piece) {
+        if (!mbar_wait_warp(bar_full, parity, abort_word, kDevTimeoutEpilogue)) return false;
+        tc_fence_after_sync();
+        const bool is_last = piece == before_last;
+        add_sum_piece(acc, total, piece == 0, is_last, rows, first, kGpEpilogueWarps / 4 * kGpDrainRows, kGpDrainRows);
+        if (is_last) return true;
+        tc_fence_before_sync();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive_cluster(map_to_cta(smem_u32(bar_empty), 0));
+        parity ^= 1u;
+    }
+}
+
+// kLong: a sum may be longer than kSumPiece (never for 8-bit operands, whose sums are exact).
+template <bool kI8, bool kPCols, bool kRaggedX, bool kLong>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kRaggedX ? kGpThreads + 32 : kGpThreads, 1)
 grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q,
                     const __grid_constant__ CUtensorMap tmap_p_small,
                     const __grid_constant__ CUtensorMap tmap_q_small, const GroupedArgs a) {
     constexpr int kBlockX = kI8 ? 256 : 128;   // x elements per stage
     constexpr int kStepX = kBlockX / 8;        // per MMA
+    constexpr int kPieceBlocks = kSumPiece / kBlockX;
+    static_assert(!(kI8 && kLong));
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = align_smem_1024(smem_raw);
     uint8_t* smem_p = smem;
@@ -257,18 +278,29 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
             int stage = 0;
             uint32_t phase = 0;
             int acc = 0;
-            uint32_t acc_phase = 0;
+            uint32_t acc_phase = 0;   // bit per accumulator
             int tails = 0;
             bool ok = true;
             while (ok && cursor.next<false>(t)) {
                 const int x_len = kRaggedX ? t.x_len & ~15 : t.x_len;
                 const int blocks = (x_len + kBlockX - 1) / kBlockX;
                 const uint32_t idesc = a.idesc | (static_cast<uint32_t>(t.width >> 3) << 17);
-                if (!mbar_wait(&bar_acc_empty[acc], acc_phase ^ 1u, abort_word, kDevTimeoutMma)) break;
+                if (!mbar_wait(&bar_acc_empty[acc], ((acc_phase >> acc) & 1u) ^ 1u, abort_word, kDevTimeoutMma)) break;
                 tc_fence_after_sync();
                 const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kGpRows);
                 bool landed = false;   // the next stage was seen full while the MMAs of this one were being issued
+                int piece_end = kLong ? kPieceBlocks : blocks;
                 for (int kb = 0; kb < blocks; ++kb) {
+                    if (kLong && kb == piece_end) {
+                        umma_commit_pair_both(smem_u32(&bar_acc_full[acc]));
+                        acc_phase ^= 1u << acc;
+                        piece_end += kPieceBlocks;
+                        if (!mbar_wait(&bar_acc_empty[acc], ((acc_phase >> acc) & 1u) ^ 1u, abort_word, kDevTimeoutMma)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after_sync();
+                    }
                     if (!landed && !mbar_wait(&bar_full[stage], phase, abort_word, kDevTimeoutMma)) {
                         ok = false;
                         break;
@@ -288,7 +320,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
                             const uint32_t off_q = kRaggedX ? k * (2048u >> 4) : static_cast<uint32_t>(((k >> 2) * kGpChunk + (k & 3) * 32) >> 4);
                             const uint64_t dp = smem_desc_join(p_lo + off_p, desc_hi), dq = smem_desc_join(q_lo + off_q, desc_hi);
                             if (kI8) umma_i8_ss_pair(d_tmem, dp, dq, idesc, (kb | k) != 0);
-                            else umma_f16_ss_pair(d_tmem, dp, dq, idesc, (kb | k) != 0);
+                            else umma_f16_ss_pair(d_tmem, dp, dq, idesc, kLong && k == 0 ? kb + kPieceBlocks != piece_end : (kb | k) != 0);
                         }
                     }
                     umma_commit_pair_both(smem_u32(&bar_empty[stage]));
@@ -308,10 +340,9 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
                     ++tails;
                 }
                 umma_commit_pair_both(smem_u32(&bar_acc_full[acc]));
-                if (++acc == 2) {
-                    acc = 0;
-                    acc_phase ^= 1u;
-                }
+                acc_phase ^= 1u << acc;
+                // behind a long sum the same one again: once it is free, so is its total in the other one
+                if (!kLong || blocks <= kPieceBlocks) acc ^= 1;
             }
         }
         __syncwarp();
@@ -323,22 +354,30 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
         float* row_scales = scales + (warp - 2) * kGpDrainRows;
         const int first_row = ((warp - 2) >> 2) * kGpDrainRows;   // its first block of rows; the warps of a quarter take turns
         int acc = 0;
-        uint32_t acc_phase = 0;
+        uint32_t acc_phase = 0;   // bit per accumulator
         while (cursor.next<true>(t)) {
             const int col = t.col0 + static_cast<int>(rank) * kGpCols + quarter * 32;
             const TileScales tile_scales = load_scales<kI8>(t, a, col, lane, first_row);
-            if (!mbar_wait_warp(&bar_acc_full[acc], acc_phase, abort_word, kDevTimeoutEpilogue)) break;
-            tc_fence_after_sync();
-            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * kGpRows);
+            const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+            const uint32_t taddr = lanes + static_cast<uint32_t>(acc * kGpRows);
+            const int x_len = kRaggedX ? t.x_len & ~15 : t.x_len;   // what goes through the ring
+            const bool in_pieces = kLong && x_len > kSumPiece;
+            if (in_pieces) {
+                if (!join_pieces(taddr, lanes + static_cast<uint32_t>((acc ^ 1) * kGpRows), &bar_acc_full[acc], &bar_acc_empty[acc],
+                                 (acc_phase >> acc) & 1u, (x_len - 1) / kSumPiece, t.rows, first_row, abort_word))
+                    break;
+                acc_phase ^= static_cast<uint32_t>((x_len - 1) / kSumPiece & 1) << acc;
+            } else {
+                if (!mbar_wait_warp(&bar_acc_full[acc], (acc_phase >> acc) & 1u, abort_word, kDevTimeoutEpilogue)) break;
+                tc_fence_after_sync();
+            }
+            acc_phase ^= 1u << acc;
             drain_tile<kI8, kRaggedX, kGpDrainRows>(taddr, t, a, col, stage, row_scales, tile_scales, t.x_len == 0, lane, first_row,
                                                      kGpEpilogueWarps / 4 * kGpDrainRows);
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&bar_acc_empty[acc]), 0));
-            if (++acc == 2) {
-                acc = 0;
-                acc_phase ^= 1u;
-            }
+            if (!in_pieces) acc ^= 1;
         }
     } else if (warp == 2 + kGpEpilogueWarps) {
         // ---------------- which tiles (both CTAs) ----------------
@@ -406,10 +445,10 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_con
     if (threadIdx.x == 0 && *abort_word != 0) atomicMax(a.status, *abort_word);
 }
 
-template <bool kI8, bool kPCols, bool kRaggedX>
+template <bool kI8, bool kPCols, bool kRaggedX, bool kLong>
 static int launch_variant(const CUtensorMap& tp, const CUtensorMap& tq, const CUtensorMap& tp_small, const CUtensorMap& tq_small,
                           const GroupedArgs& a, int pairs, const DeviceInfo* dev, cudaStream_t stream) {
-    auto kernel = grouped_pair_kernel<kI8, kPCols, kRaggedX>;
+    auto kernel = grouped_pair_kernel<kI8, kPCols, kRaggedX, kLong>;
     constexpr int smem = PairSmem<kI8, kRaggedX>::kTotal;
     static OncePerDevice once;
     if (int rc = raise_smem_limit_once(once, dev->device, kernel, smem)) return rc;
@@ -433,10 +472,15 @@ int launch_grouped_pair(const GroupedProblem& g, const GroupedPlan& plan, const 
     }
     const int64_t max_pairs = dev->sm_count / 2;
     const int pairs = static_cast<int>(plan.tiles < max_pairs ? plan.tiles : max_pairs);
-    if (i8) return launch_variant<true, false, false>(tp, tq, tp_small, tq_small, a, pairs, dev, stream);
-    if (g.ragged_x) return launch_variant<false, true, true>(tp, tq, tp_small, tq_small, a, pairs, dev, stream);
-    if (g.p_c_contiguous) return launch_variant<false, true, false>(tp, tq, tp_small, tq_small, a, pairs, dev, stream);
-    return launch_variant<false, false, false>(tp, tq, tp_small, tq_small, a, pairs, dev, stream);
+    if (i8) return launch_variant<true, false, false, false>(tp, tq, tp_small, tq_small, a, pairs, dev, stream);
+    if ((g.ragged_x ? g.token_rows : g.other) > kSumPiece) {
+        if (g.ragged_x) return launch_variant<false, true, true, true>(tp, tq, tp_small, tq_small, a, pairs, dev, stream);
+        if (g.p_c_contiguous) return launch_variant<false, true, false, true>(tp, tq, tp_small, tq_small, a, pairs, dev, stream);
+        return launch_variant<false, false, false, true>(tp, tq, tp_small, tq_small, a, pairs, dev, stream);
+    }
+    if (g.ragged_x) return launch_variant<false, true, true, false>(tp, tq, tp_small, tq_small, a, pairs, dev, stream);
+    if (g.p_c_contiguous) return launch_variant<false, true, false, false>(tp, tq, tp_small, tq_small, a, pairs, dev, stream);
+    return launch_variant<false, false, false, false>(tp, tq, tp_small, tq_small, a, pairs, dev, stream);
 }
 
 }  // namespace tcb

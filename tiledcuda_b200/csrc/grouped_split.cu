@@ -130,12 +130,31 @@ __device__ __forceinline__ void find_tile(const GroupedArgs& a, int row_tile, in
     if (!__any_sync(0xffffffffu, here) && lane == 0) out->rows = 0;
 }
 
-template <bool kI8, bool kPCols, bool kRaggedX>
+// The epilogue's part in a sum that comes in `before_last` + 1 pieces: waits for each, adds it to the total, and leaves the whole
+// sum in the accumulator. One warp; false when a wait ran out.
+static __device__ __noinline__ bool join_pieces(uint32_t acc, uint32_t total, uint64_t* bar_full, uint64_t* bar_empty, int before_last,
+                                                int rows, int first, volatile uint32_t* abort_word) {
+    for (int piece = 0;; ++piece) {
+        if (!mbar_wait_warp(bar_full, static_cast<uint32_t>(piece) & 1u, abort_word, kDevTimeoutEpilogue)) return false;
+        tc_fence_after_sync();
+        const bool is_last = piece == before_last;
+        add_sum_piece(acc, total, piece == 0, is_last, rows, first, 64, 32);
+        if (is_last) return true;
+        tc_fence_before_sync();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(bar_empty);
+    }
+}
+
+// kLong: a CTA's part of a sum may be longer than kSumPiece (never for 8-bit operands, whose sums are exact).
+template <bool kI8, bool kPCols, bool kRaggedX, bool kLong>
 __global__ void __launch_bounds__(kGsThreads, 2)
 grouped_split_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q, const GroupedArgs a,
                      int splits, int ring_bytes) {
     constexpr int kBlockX = kI8 ? 128 : 64;   // x elements per stage
     constexpr int kStepX = kBlockX / 4;       // per MMA
+    constexpr int kPieceBlocks = kSumPiece / kBlockX;
+    static_assert(!(kI8 && kLong));
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = align_smem_1024(smem_raw);
     const int q_bytes = a.tile_rows * 128;
@@ -144,7 +163,8 @@ grouped_split_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
     uint64_t* bar_full = reinterpret_cast<uint64_t*>(ring + ring_bytes);
     uint64_t* bar_empty = bar_full + kGsMaxStages;
     uint64_t* bar_acc = bar_empty + kGsMaxStages;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_acc + 1);
+    uint64_t* bar_acc_empty = bar_acc + 1;   // of sums in pieces
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_acc_empty + 1);
     volatile uint32_t* abort_word = tmem_slot + 1;
     GroupTile* shared_tile = reinterpret_cast<GroupTile*>(tmem_slot + 2);
     float* scales = reinterpret_cast<float*>(ring);   // epilogue, after the ring has been read
@@ -153,7 +173,8 @@ grouped_split_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
     const int lane = threadIdx.x & 31;
     const int rank = splits > 1 ? static_cast<int>(__shfl_sync(0xffffffffu, cluster_ctarank(), 0)) : 0;
     const int col_tiles = (a.cols + kGsCols - 1) / kGsCols;
-    const uint32_t tmem_cols = a.tile_rows <= 32 ? 32u : static_cast<uint32_t>(a.tile_rows);
+    // the total of a long sum takes as many columns again as the accumulator
+    const uint32_t tmem_cols = static_cast<uint32_t>(max(32, kLong ? 2 * a.tile_rows : a.tile_rows));
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kGsMaxStages; ++s) {
@@ -161,6 +182,7 @@ grouped_split_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
             mbar_init(&bar_empty[s], 1);
         }
         mbar_init(bar_acc, 1);
+        mbar_init(bar_acc_empty, kGsEpilogueWarps);
         *abort_word = 0;
         fence_barrier_init();
     }
@@ -236,7 +258,18 @@ grouped_split_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
+        uint32_t acc_phase = 0;
+        int first = block0;   // of the piece
         for (int b = block0; b < block1; ++b) {
+            if (kLong && b == first + kPieceBlocks) {
+                first = b;
+                if (leader) umma_commit(bar_acc);
+                if (!mbar_wait_warp(bar_acc_empty, acc_phase, abort_word, kDevTimeoutMma)) {
+                    ok = false;
+                    break;
+                }
+                acc_phase ^= 1u;
+            }
             if (!mbar_wait_warp(&bar_full[stage], phase, abort_word, kDevTimeoutMma)) {
                 ok = false;
                 break;
@@ -259,7 +292,7 @@ grouped_split_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
             for (int k = 0; k < 4; ++k) {
                 if (k < steps && leader)
                     umma_ss<kI8>(tmem_base, smem_desc_join(p_lo + k * (kPCols ? 2048u >> 4 : 2u), desc_hi),
-                                 smem_desc_join(q_lo + k * (kRaggedX ? 2048u >> 4 : 2u), desc_hi), idesc, b != block0 || k != 0);
+                                 smem_desc_join(q_lo + k * (kRaggedX ? 2048u >> 4 : 2u), desc_hi), idesc, b != first || k != 0);
             }
             if (leader) umma_commit(&bar_empty[stage]);
             if (++stage == stages) {
@@ -279,9 +312,15 @@ grouped_split_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
     const bool summed = block1 > block0;   // else this CTA's part is zero
     TileScales tile_scales = {};
     if (kI8 && drains && t.rows > 0 && splits == 1) tile_scales = load_scales<kI8>(t, a, t.col0 + quarter * 32, lane, part_of_rows * 32);
-    const bool ok = drains && t.rows > 0 && mbar_wait_warp(bar_acc, 0, abort_word, kDevTimeoutEpilogue);
-    if (ok) tc_fence_after_sync();
     const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+    bool ok = drains && t.rows > 0;
+    if (kLong && ok && block1 - block0 > kPieceBlocks) {
+        ok = join_pieces(taddr, taddr + static_cast<uint32_t>(a.tile_rows), bar_acc, bar_acc_empty, (block1 - block0 - 1) / kPieceBlocks,
+                         t.rows, part_of_rows * 32, abort_word);
+    } else if (ok) {
+        ok = mbar_wait_warp(bar_acc, 0, abort_word, kDevTimeoutEpilogue);
+        if (ok) tc_fence_after_sync();
+    }
     const int64_t out0 = (kRaggedX ? t.e * a.stride_o : 0) + static_cast<int64_t>(t.row0) * a.ldo;
     if (splits == 1) {
         if (ok) drain_tile<kI8, kRaggedX, 32>(taddr, t, a, t.col0 + quarter * 32, ring + 4096 + (warp - 2) * 2048, scales + (warp - 2) * 32,
@@ -348,10 +387,10 @@ grouped_split_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
     if (threadIdx.x == 0 && *abort_word != 0) atomicMax(a.status, *abort_word);
 }
 
-template <bool kI8, bool kPCols, bool kRaggedX>
+template <bool kI8, bool kPCols, bool kRaggedX, bool kLong>
 static int launch_variant(const CUtensorMap& tp, const CUtensorMap& tq, const GroupedArgs& a, const GroupedPlan& plan, const DeviceInfo* dev,
                           cudaStream_t stream) {
-    auto kernel = grouped_split_kernel<kI8, kPCols, kRaggedX>;
+    auto kernel = grouped_split_kernel<kI8, kPCols, kRaggedX, kLong>;
     static OncePerDevice once;
     if (int rc = raise_smem_limit_once(once, dev->device, kernel, gs_smem(kGsRingAlone))) return rc;
     const int ring = plan.alone ? kGsRingAlone : kGsRing;
@@ -381,10 +420,16 @@ int launch_grouped_split(const GroupedProblem& g, const GroupedPlan& plan, const
     // P: 128 columns by 128 bytes of x, or (columns contiguous) 64 columns by 64 x; Q: the tile's rows alike
     if (int rc = grouped_map_p(&tp, g, g.p_c_contiguous ? 64 : 128)) return rc;
     if (int rc = grouped_map_q(&tq, g, g.ragged_x ? 64 : plan.tile_rows)) return rc;
-    if (i8) return launch_variant<true, false, false>(tp, tq, a, plan, dev, stream);
-    if (g.ragged_x) return launch_variant<false, true, true>(tp, tq, a, plan, dev, stream);
-    if (g.p_c_contiguous) return launch_variant<false, true, false>(tp, tq, a, plan, dev, stream);
-    return launch_variant<false, false, false>(tp, tq, a, plan, dev, stream);
+    if (i8) return launch_variant<true, false, false, false>(tp, tq, a, plan, dev, stream);
+    const int64_t most_blocks = ((g.ragged_x ? g.token_rows : g.other) + 63) / 64;
+    if ((most_blocks + plan.splits - 1) / plan.splits > kSumPiece / 64) {
+        if (g.ragged_x) return launch_variant<false, true, true, true>(tp, tq, a, plan, dev, stream);
+        if (g.p_c_contiguous) return launch_variant<false, true, false, true>(tp, tq, a, plan, dev, stream);
+        return launch_variant<false, false, false, true>(tp, tq, a, plan, dev, stream);
+    }
+    if (g.ragged_x) return launch_variant<false, true, true, false>(tp, tq, a, plan, dev, stream);
+    if (g.p_c_contiguous) return launch_variant<false, true, false, false>(tp, tq, a, plan, dev, stream);
+    return launch_variant<false, false, false, false>(tp, tq, a, plan, dev, stream);
 }
 
 }  // namespace tcb
