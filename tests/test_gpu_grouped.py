@@ -928,3 +928,45 @@ def test_forward_and_dgrad_of_long_sums(cuda_ops, clean_status, sizes, n, x):
         call(a, w, off, c)
         assert_within(c[mask], exact[mask], long_product_error(exact[mask], x))
         assert (c[~mask] == -7.0).all()
+
+
+@pytest.mark.parametrize("op", ["gemm_i8", "wgrad"])
+def test_the_wait_limit_does_not_count_the_kernel_in_front(cuda_ops, clean_status, op):
+    """A GEMM on two SMs that runs for three seconds releases the SMs it does not use at once. The kernel behind it starts there,
+    and its waits, limited to two seconds each, must not end before that GEMM does."""
+    n, k = 16384, 65536
+    b = torch.zeros(n, k, dtype=F16, device=DEV)
+    a, c = torch.zeros(65536, k, dtype=F16, device=DEV), torch.empty(65536, n, device=DEV)
+
+    def front(rows):
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        cuda_ops.gemm(a[:rows], b, c[:rows], max_sms=2)
+        end.record()
+        return start, end
+
+    front(512)
+    start, end = front(4096)
+    end.synchronize()
+    rows = min(65536, math.ceil(3000 / start.elapsed_time(end) * 8) * 512)
+    g = gen(43)
+    if op == "gemm_i8":
+        x, w = ints(g, (2500, 2080)), ints(g, (3000, 2080))
+        sx, sw = torch.rand(2500, generator=g, device=DEV) + 0.5, torch.rand(3000, generator=g, device=DEV) + 0.5
+        out = torch.full((2500, 3000), math.nan, device=DEV)
+        exact = i8_exact(x, w, sx, sw)
+        error = exact.abs() * 3.01 * 2.0 ** -24
+        call = lambda: cuda_ops.gemm_i8(x, w, sx, sw, out)
+    else:
+        sizes = [700, 333, 0, 1200, 90]
+        dc, x = halves(g, (sum(sizes), 1300), F16), halves(g, (sum(sizes), 776), F16)
+        out, off = torch.full((len(sizes), 1300, 776), math.nan, device=DEV), offsets_of(sizes)
+        exact, s = plain_wgrad(dc, x, sizes, 0)
+        error = product_error(s, max(sizes))
+        call = lambda: cuda_ops.grouped_gemm_wgrad(dc, x, off, out)
+    torch.cuda.synchronize()
+    start, end = front(rows)
+    call()
+    torch.cuda.synchronize()
+    assert start.elapsed_time(end) > 2100, "the kernel in front is over before a wait could run out"
+    assert_within(out, exact, error)

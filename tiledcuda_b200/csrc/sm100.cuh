@@ -102,7 +102,9 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 // Bounded waits. The common case, a phase that is already complete or completes within a few polls, must
 // cost no more than the poll itself (about a dozen cycles): the fast path is a single try_wait and a
 // uniform branch, and everything that needs a loop, the clock or the abort word lives in a separate
-// non-inlined function, so that the caller carries none of its control flow.
+// non-inlined function, so that the caller carries none of its control flow. A role may start to wait before the kernel in front
+// of this one is over (programmatic launch), and what it waits for may need that kernel's results: the clock of the limit
+// starts when that kernel has ended, however long it takes.
 //
 // mbar_wait: one thread. Returns false when another role has aborted or when the limit ran out (then it
 // records `code` in the CTA's abort word).
@@ -113,6 +115,7 @@ static __device__ __noinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parit
     while (!mbar_try_wait(bar, parity)) {
         if ((++it & 0xfffu) == 0) {
             if (*abort_word != 0) return false;
+            if (t0 == 0) grid_dependency_wait();
             const uint64_t now = global_timer_ns();
             if (t0 == 0) {
                 t0 = now;
@@ -152,6 +155,7 @@ static __device__ __noinline__ bool mbar_wait_warp_slow(uint64_t* bar, uint32_t 
             if (*abort_word != 0) {
                 give_up = 1;
             } else {
+                if (t0 == 0) grid_dependency_wait();
                 const uint64_t now = global_timer_ns();
                 if (t0 == 0) {
                     t0 = now;
