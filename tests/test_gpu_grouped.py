@@ -970,3 +970,26 @@ def test_the_wait_limit_does_not_count_the_kernel_in_front(cuda_ops, clean_statu
     torch.cuda.synchronize()
     assert start.elapsed_time(end) > 2100, "the kernel in front is over before a wait could run out"
     assert_within(out, exact, error)
+
+
+def test_a_mode_that_refuses_is_heard(cuda_ops, clean_status):
+    """An error that a dispatch mode raises for the call reaches the caller, and nothing is launched behind the mode's back."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class NotHere(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            raise RuntimeError("not here")
+
+    g = gen(44)
+    sizes, n, k = [7, 0, 30], 72, 48
+    off, total = offsets_of(sizes), sum(sizes)
+    a, b, dc = halves(g, (total, k), F16), halves(g, (3, n, k), F16), halves(g, (total, n), F16)
+    q, qb, sa, sb = ints(g, (total, k)), ints(g, (3, n, k)), torch.ones(total, device=DEV), torch.ones(3, n, device=DEV)
+    new_q, scale = torch.full((total, k), 77, dtype=torch.int8, device=DEV), torch.full((total,), -7.0, device=DEV)
+    c, da, db = (torch.full(s, -7.0, dtype=F16, device=DEV) for s in ((total, n), (total, k), (3, n, k)))
+    for call in (lambda: cuda_ops.quantize_rows(a, new_q, scale), lambda: cuda_ops.gemm_i8(q, qb[0], sa, sb[0], c),
+                 lambda: cuda_ops.grouped_gemm(a, b, off, c), lambda: cuda_ops.grouped_gemm_i8(q, qb, sa, sb, off, c),
+                 lambda: cuda_ops.grouped_gemm_dgrad(dc, b, off, da), lambda: cuda_ops.grouped_gemm_wgrad(dc, a, off, db)):
+        with NotHere(), pytest.raises(RuntimeError, match="not here"):
+            call()
+    assert (new_q == 77).all() and all((t == -7.0).all() for t in (scale, c, da, db))

@@ -116,3 +116,61 @@ def test_direct_calls_leave_what_is_not_for_them():
     assert calls.gemm_i8(*t[:4]) is False
     assert calls.gemm_i8(None, *t[1:]) is False
     assert calls.gemm_i8() is False
+
+
+@pytest.fixture()
+def shapes_on_a_gpu(monkeypatch):
+    """CUDA tensors without a GPU, for the way a call takes; whatever is launched in the end is an error."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    def launched(*args):
+        raise AssertionError("launched")
+
+    monkeypatch.setattr(ops, "_launch", launched)
+    monkeypatch.setattr(ops, "_registered_ops", {})
+    monkeypatch.setattr(ops, "_direct_calls", {})
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        yield [torch.empty(4, 16, dtype=torch.int8, device="cuda"), torch.empty(8, 16, dtype=torch.int8, device="cuda"),
+               torch.empty(4, device="cuda"), torch.empty(8, device="cuda"), torch.empty(4, 8, device="cuda")]
+
+
+@pytest.mark.parametrize("error", [RuntimeError("not here"), TypeError("nor there"), NotImplementedError("no such kernel")])
+def test_an_error_of_the_op_is_raised_and_nothing_else_launched(shapes_on_a_gpu, error):
+    calls = []
+
+    def op(*args):
+        calls.append(args)
+        raise error
+
+    ops._registered_ops["gemm_i8"] = op
+    with pytest.raises(type(error), match=str(error)):
+        ops.gemm_i8(*shapes_on_a_gpu)
+    assert len(calls) == 1
+    with pytest.raises(ValueError, match="scale_a must be"):   # what the checks can explain they do
+        ops.gemm_i8(*shapes_on_a_gpu[:2], shapes_on_a_gpu[3], *shapes_on_a_gpu[3:])
+
+
+def test_what_the_c_entry_point_refused_is_raised_as_such(shapes_on_a_gpu):
+    calls = []
+
+    def op(*args):
+        calls.append(args)
+        raise RuntimeError("tiledcuda::gemm_i8 failed with status -3: a call failed\nbacktrace")
+
+    ops._registered_ops["gemm_i8"] = op
+    with pytest.raises(_lib.TiledCudaError, match="tc_gemm_i8 failed with status -3: a call failed$") as raised:
+        ops.gemm_i8(*shapes_on_a_gpu)
+    assert raised.value.status == -3 and len(calls) == 1
+    ops._registered_ops["gemm_i8"] = lambda *args: calls.append(args)
+    ops._direct_calls["gemm_i8"] = op   # past the dispatcher: not made again through it
+    with pytest.raises(_lib.TiledCudaError, match="a call failed"):
+        ops.gemm_i8(*shapes_on_a_gpu)
+    assert len(calls) == 2
+
+
+def test_without_the_op_the_c_entry_point_is_called(shapes_on_a_gpu, monkeypatch):
+    names = []
+    monkeypatch.setattr(ops, "_launch", lambda name, *args: names.append(name))
+    monkeypatch.setattr(torch.Tensor, "data_ptr", lambda t: 64)
+    ops.gemm_i8(*shapes_on_a_gpu)
+    assert names == ["tc_gemm_i8"]

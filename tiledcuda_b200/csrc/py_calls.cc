@@ -2,13 +2,14 @@
 // host longer than the device, and of the 4.7 us that a call through torch.ops costs, 2 are argument parsing and dispatch.
 // Each function returns True if it made the call. It returns False, and has done nothing, for arguments that are not plain
 // tensors or parameters, under a torch dispatch or function mode (which would not see the call), and where the checks refused:
-// the caller then takes the way through the dispatcher.
+// the caller then takes the way through the dispatcher. A CUDA call that failed is a RuntimeError: the call is not made twice.
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 
 #include <array>
+#include <string>
 #include <utility>
 
 #include "torch_ops.h"
@@ -21,14 +22,18 @@ bool modes_active() {
 
 template <typename F, size_t... I>
 bool invoke(F* op, const std::array<at::Tensor*, sizeof...(I)>& t, std::index_sequence<I...>) {
-    bool done = true;
+    bool done = false;
+    std::string failure;
     PyThreadState* state = PyEval_SaveThread();   // a launch can wait for room in the stream's queue
     try {
         op(*t[I]...);
+        done = true;
+    } catch (const tiledcuda::CudaFailure& e) {
+        failure = e.what_without_backtrace();
     } catch (...) {
-        done = false;
     }
     PyEval_RestoreThread(state);
+    if (!failure.empty()) PyErr_SetString(PyExc_RuntimeError, failure.c_str());
     return done;
 }
 
@@ -41,6 +46,7 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (plain) t[i] = const_cast<at::Tensor*>(&THPVariable_Unpack(args[i]));   // the caller's frame holds the arguments
     }
     if (plain && invoke(op, t, std::make_index_sequence<kArgs>{})) Py_RETURN_TRUE;
+    if (PyErr_Occurred()) return nullptr;
     Py_RETURN_FALSE;
 }
 

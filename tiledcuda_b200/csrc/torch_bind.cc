@@ -19,6 +19,9 @@
 namespace {
 
 void check(const char* op, int status) {
+    if (status == TC_ERR_CUDA)
+        throw tiledcuda::CudaFailure({__func__, __FILE__, static_cast<uint32_t>(__LINE__)},
+                                     c10::str("tiledcuda::", op, " failed with status ", status, ": ", tc_last_error()));
     TORCH_CHECK(status == TC_OK, "tiledcuda::", op, " failed with status ", status, ": ", tc_last_error());
 }
 

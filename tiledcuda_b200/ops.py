@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+import re
 from pathlib import Path
 
 import torch
@@ -149,6 +150,7 @@ def _launch(name: str, device: int, *args) -> None:
 _OP_LIB = Path(__file__).resolve().parent / "libtiledcuda.so"
 _registered_ops: dict | None = None
 _direct_calls: dict = {}
+_OP_FAILED = re.compile(r"tiledcuda::(\w+) failed with status (-?\d+): (.*)")   # how torch_bind.cc passes a status on
 
 
 def _registered(name: str):
@@ -176,21 +178,34 @@ def _registered(name: str):
     return _registered_ops.get(name)
 
 
-def _done(name: str, *args) -> bool:
-    """Makes the call through the registered op, or past the dispatcher where that makes no difference (_calls). False where
-    there is no such op, or where it refused: then the checks of the function that called this, or the C entry point, say why
-    in their own words."""
+_DONE = Exception()
+
+
+def _through_op(name: str, *args) -> Exception | None:
+    """Makes the call through the registered op, or past the dispatcher where nothing would see it there (_calls), and returns _DONE.
+    Returns None where there is no such op, and its error where it raised one: the checks of the function that called this then say
+    in their own words what is wrong with the arguments, and _pass_on raises what they do not explain."""
     op = _registered(name)
     if op is None:
-        return False
-    direct = _direct_calls.get(name)
-    if direct is not None and direct(*args):
-        return True
+        return None
     try:
-        op(*args)
-    except (RuntimeError, TypeError):
-        return False
-    return True
+        direct = _direct_calls.get(name)
+        if direct is None or not direct(*args):
+            op(*args)
+    except (RuntimeError, TypeError) as error:
+        return error
+    return _DONE
+
+
+def _pass_on(error: Exception | None) -> None:
+    """Raises the error of a registered op: what the C entry point said as the other way to it has it, anything else (a failure of a
+    dispatch mode, say) as it is. None: there was no op, and the call is still to be made."""
+    if error is None:
+        return
+    status = _OP_FAILED.match(str(error))
+    if status is None:
+        raise error
+    raise _lib.TiledCudaError("tc_" + status[1], int(status[2]), status[3]) from error
 
 
 def quantize_rows(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> None:
@@ -200,7 +215,8 @@ def quantize_rows(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> None
     activations, one per output channel for a weight [N,K]. A row with an infinity or NaN gets that as its scale
     and q = 0. Row strides of x and q may exceed the row length.
     """
-    if _done("quantize_rows", x, q, scale):
+    refused = _through_op("quantize_rows", x, q, scale)
+    if refused is _DONE:
         return
     shape = _shape(x, "x", 2)
     m, k = shape
@@ -208,6 +224,7 @@ def quantize_rows(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> None
     dense_x = _need_rows(x, "x", shape, _TYPES, dev)
     dense_q = _need_rows(q, "q", shape, _INT8, dev)
     _need_rows(scale, "scale", (m,), _FLOAT, dev)
+    _pass_on(refused)
     _launch("tc_quantize_rows", dev, x.data_ptr(), q.data_ptr(), scale.data_ptr(), m, k, _ld(x, shape, dense_x), _ld(q, shape, dense_q),
             _TYPES[x.dtype])
 
@@ -219,7 +236,8 @@ def gemm_i8(a: torch.Tensor, b: torch.Tensor, scale_a: torch.Tensor, scale_b: to
     scaled in fp32 and rounded once. Row strides of a and b must be multiples of 16 bytes, K and N may be any size; M
     may be 0.
     """
-    if _done("gemm_i8", a, b, scale_a, scale_b, c):
+    refused = _through_op("gemm_i8", a, b, scale_a, scale_b, c)
+    if refused is _DONE:
         return
     sa, sb = _shape(a, "a", 2), _shape(b, "b", 2)
     m, k = sa
@@ -230,6 +248,7 @@ def gemm_i8(a: torch.Tensor, b: torch.Tensor, scale_a: torch.Tensor, scale_b: to
     _need_rows(scale_a, "scale_a", (m,), _FLOAT, dev)
     _need_rows(scale_b, "scale_b", (n,), _FLOAT, dev)
     dense_c = _need_rows(c, "c", (m, n), _TYPES, dev)
+    _pass_on(refused)
     _launch("tc_gemm_i8", dev, a.data_ptr(), b.data_ptr(), scale_a.data_ptr(), scale_b.data_ptr(), c.data_ptr(), m, n, k,
             _ld(a, sa, dense_a, 0, 16), _ld(b, sb, dense_b, 0, 16), _ld(c, (m, n), dense_c), _TYPES[c.dtype])
 
@@ -246,7 +265,8 @@ def grouped_gemm(a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor, c: tor
     CUDA int32 / int64 tensor [E + 1], nondecreasing, within [0, T]; it is read on the device only. Experts may be
     empty; rows of c outside all groups stay as they were. Row strides of a and b must be multiples of 16 bytes.
     """
-    if _done("grouped_gemm", a, b, offsets, c):
+    refused = _through_op("grouped_gemm", a, b, offsets, c)
+    if refused is _DONE:
         return
     sa, sb = _shape(a, "a", 2), _shape(b, "b", 3)
     t, k = sa
@@ -256,6 +276,7 @@ def grouped_gemm(a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor, c: tor
     dense_b = _need_rows(b, "b", (e, n, k), (a.dtype,), dev)
     dense_c = _need_rows(c, "c", (t, n), (a.dtype, torch.float32), dev)
     wide = _need_offsets(offsets, e, dev)
+    _pass_on(refused)
     _launch("tc_grouped_gemm", dev, a.data_ptr(), b.data_ptr(), offsets.data_ptr(), wide, c.data_ptr(), t, e, n, k, _ld(a, sa, dense_a, 0, 8),
             _ld(b, sb, dense_b, 1, 8), _ld(b, sb, dense_b, 0, 8), _ld(c, (t, n), dense_c), _TYPES[a.dtype], _TYPES[c.dtype])
 
@@ -267,7 +288,8 @@ def grouped_gemm_i8(a: torch.Tensor, b: torch.Tensor, scale_a: torch.Tensor, sca
     scale_a fp32 [T], scale_b fp32 [E,N] contiguous, c [T,N] fp16, bf16 or fp32; sums as in gemm_i8, offsets and
     rows outside all groups as in grouped_gemm. Strides of a and b must be multiples of 16 bytes.
     """
-    if _done("grouped_gemm_i8", a, b, scale_a, scale_b, offsets, c):
+    refused = _through_op("grouped_gemm_i8", a, b, scale_a, scale_b, offsets, c)
+    if refused is _DONE:
         return
     sa, sb = _shape(a, "a", 2), _shape(b, "b", 3)
     t, k = sa
@@ -281,6 +303,7 @@ def grouped_gemm_i8(a: torch.Tensor, b: torch.Tensor, scale_a: torch.Tensor, sca
         raise ValueError("scale_b must be contiguous")
     dense_c = _need_rows(c, "c", (t, n), _TYPES, dev)
     wide = _need_offsets(offsets, e, dev)
+    _pass_on(refused)
     _launch("tc_grouped_gemm_i8", dev, a.data_ptr(), b.data_ptr(), scale_a.data_ptr(), scale_b.data_ptr(), offsets.data_ptr(), wide,
             c.data_ptr(), t, e, n, k, _ld(a, sa, dense_a, 0, 16), _ld(b, sb, dense_b, 1, 16), _ld(b, sb, dense_b, 0, 16),
             _ld(c, (t, n), dense_c), _TYPES[c.dtype])
@@ -292,7 +315,8 @@ def grouped_gemm_dgrad(dc: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor,
     dc [T,N] and b [E,N,K] of one type (fp16 or bf16), da [T,K] of that type or fp32; offsets and the rows outside all
     groups as in grouped_gemm. Row strides of dc and b must be multiples of 16 bytes.
     """
-    if _done("grouped_gemm_dgrad", dc, b, offsets, da):
+    refused = _through_op("grouped_gemm_dgrad", dc, b, offsets, da)
+    if refused is _DONE:
         return
     sc, sb = _shape(dc, "dc", 2), _shape(b, "b", 3)
     t, n = sc
@@ -302,6 +326,7 @@ def grouped_gemm_dgrad(dc: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor,
     dense_b = _need_rows(b, "b", (e, n, k), (dc.dtype,), dev)
     dense_da = _need_rows(da, "da", (t, k), (dc.dtype, torch.float32), dev)
     wide = _need_offsets(offsets, e, dev)
+    _pass_on(refused)
     _launch("tc_grouped_gemm_dgrad", dev, dc.data_ptr(), b.data_ptr(), offsets.data_ptr(), wide, da.data_ptr(), t, e, n, k,
             _ld(dc, sc, dense_dc, 0, 8), _ld(b, sb, dense_b, 1, 8), _ld(b, sb, dense_b, 0, 8), _ld(da, (t, k), dense_da), _TYPES[dc.dtype], _TYPES[da.dtype])
 
@@ -312,7 +337,8 @@ def grouped_gemm_wgrad(dc: torch.Tensor, a: torch.Tensor, offsets: torch.Tensor,
     dc [T,N] and a [T,K] of one type (fp16 or bf16), db [E,N,K] of that type or fp32, overwritten as a whole. Rows
     outside all groups take no part. Row strides of dc and a must be multiples of 16 bytes.
     """
-    if _done("grouped_gemm_wgrad", dc, a, offsets, db):
+    refused = _through_op("grouped_gemm_wgrad", dc, a, offsets, db)
+    if refused is _DONE:
         return
     sc, sa, sb = _shape(dc, "dc", 2), _shape(a, "a", 2), _shape(db, "db", 3)
     t, n = sc
@@ -323,6 +349,7 @@ def grouped_gemm_wgrad(dc: torch.Tensor, a: torch.Tensor, offsets: torch.Tensor,
     dense_a = _need_rows(a, "a", (t, k), (dc.dtype,), dev)
     dense_db = _need_rows(db, "db", (e, n, k), (dc.dtype, torch.float32), dev)
     wide = _need_offsets(offsets, e, dev)
+    _pass_on(refused)
     _launch("tc_grouped_gemm_wgrad", dev, dc.data_ptr(), a.data_ptr(), offsets.data_ptr(), wide, db.data_ptr(), t, e, n, k,
             _ld(dc, sc, dense_dc, 0, 8), _ld(a, sa, dense_a, 0, 8), _ld(db, sb, dense_db, 1), _ld(db, sb, dense_db, 0), _TYPES[dc.dtype], _TYPES[db.dtype])
 
