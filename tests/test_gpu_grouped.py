@@ -993,3 +993,39 @@ def test_a_mode_that_refuses_is_heard(cuda_ops, clean_status):
         with NotHere(), pytest.raises(RuntimeError, match="not here"):
             call()
     assert (new_q == 77).all() and all((t == -7.0).all() for t in (scale, c, da, db))
+
+
+def test_tracers_and_profilers_see_the_calls(cuda_ops, clean_status):
+    """torch.jit.trace records the operators, torch.profiler lists them; outside of both a plain call goes past the dispatcher."""
+    g = gen(45)
+    sizes, n, k = [7, 0, 30], 72, 48
+    off, total = offsets_of(sizes), sum(sizes)
+
+    def inputs():
+        return [halves(g, (total, k), F16), halves(g, (3, n, k), F16), halves(g, (total, n), F16), ints(g, (3, n, k)),
+                torch.rand(3, n, generator=g, device=DEV)]
+
+    def step(a, b, dc, qb, sb):
+        q, scale = torch.empty(total, k, dtype=torch.int8, device=DEV), torch.zeros(total, device=DEV)
+        c, c1, c8 = torch.zeros(total, n, device=DEV), torch.zeros(total, n, device=DEV), torch.zeros(total, n, device=DEV)
+        da, db = torch.zeros(total, k, device=DEV), torch.zeros(3, n, k, device=DEV)
+        cuda_ops.quantize_rows(a, q, scale)
+        cuda_ops.gemm_i8(q, qb[0], scale, sb[0], c1)
+        cuda_ops.grouped_gemm_i8(q, qb, scale, sb, off, c8)
+        cuda_ops.grouped_gemm(a, b, off, c)
+        cuda_ops.grouped_gemm_dgrad(dc, b, off, da)
+        cuda_ops.grouped_gemm_wgrad(dc, a, off, db)
+        return q, scale, c1, c8, c, da, db
+
+    names = ["quantize_rows", "gemm_i8", "grouped_gemm_i8", "grouped_gemm", "grouped_gemm_dgrad", "grouped_gemm_wgrad"]
+    traced = torch.jit.trace(step, inputs(), check_trace=False)
+    recorded = [node.kind() for node in traced.graph.nodes() if node.kind().startswith("tiledcuda::")]
+    assert recorded == ["tiledcuda::" + name for name in names]
+    other = inputs()
+    assert all(torch.equal(x, y) for x, y in zip(traced(*other), step(*other)))
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+        step(*other)
+    listed = {event.key for event in prof.key_averages()}
+    assert listed.issuperset("tiledcuda::" + name for name in names)
+    a, b = other[:2]
+    assert cuda_ops._direct_calls["grouped_gemm"](a, b, off, torch.empty(total, n, device=DEV)) is True

@@ -1,11 +1,13 @@
 // Python module _calls: the functions of torch_ops.h called without the dispatcher. Small calls of these operators take the
 // host longer than the device, and of the 4.7 us that a call through torch.ops costs, 2 are argument parsing and dispatch.
 // Each function returns True if it made the call. It returns False, and has done nothing, for arguments that are not plain
-// tensors or parameters, under a torch dispatch or function mode (which would not see the call), and where the checks refused:
-// the caller then takes the way through the dispatcher. A CUDA call that failed is a RuntimeError: the call is not made twice.
+// tensors or parameters, where something waits for the call in the dispatcher (a dispatch or function mode, a tracer, a function
+// transform, a profiler), and where the checks refused: the caller then takes the way through the dispatcher. A CUDA call that failed is a RuntimeError: the call is not made twice.
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/PythonTorchFunctionTLS.h>
+#include <ATen/record_function.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 
 #include <array>
@@ -16,8 +18,11 @@
 
 namespace {
 
-bool modes_active() {
-    return c10::impl::TorchDispatchModeTLS::any_modes_set() || at::impl::torch_function_mode_enabled();
+// Modes, tracers and transforms put dispatch keys of their own in front of the usual ones; profilers are called back.
+bool watched() {
+    const c10::DispatchKeySet keys = c10::impl::tls_local_dispatch_key_set().included_;
+    return !c10::default_included_set.has_all(keys) || c10::impl::TorchDispatchModeTLS::any_modes_set() ||
+           at::impl::torch_function_mode_enabled() || at::hasCallbacks();
 }
 
 template <typename F, size_t... I>
@@ -40,7 +45,7 @@ bool invoke(F* op, const std::array<at::Tensor*, sizeof...(I)>& t, std::index_se
 template <size_t kArgs, auto op>
 PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
     std::array<at::Tensor*, kArgs> t;
-    bool plain = n == static_cast<Py_ssize_t>(kArgs) && !modes_active();
+    bool plain = n == static_cast<Py_ssize_t>(kArgs) && !watched();
     for (size_t i = 0; plain && i < kArgs; ++i) {
         plain = THPVariable_CheckExact(args[i]);
         if (plain) t[i] = const_cast<at::Tensor*>(&THPVariable_Unpack(args[i]));   // the caller's frame holds the arguments
