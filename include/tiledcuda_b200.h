@@ -102,7 +102,7 @@ int tc_quantize_rows(const void* x, void* q, float* scale, int64_t rows, int64_t
  * [K,N] of tc_gemm_f16_f32), scales fp32 [M] and [N] (one per token and per output channel), C of c_type (tc_type)
  * with row stride ldc. The sum over K is exact (32-bit integers; K <= 131071, so that it cannot overflow for any
  * 8-bit values), then (float(sum) * scale_a) * scale_b in fp32 is rounded once to c_type. M may be 0. Needs lda % 16 == 0,
- * ldb % 16 == 0 and 16-byte aligned A and B; K and N may be any size. C must not overlap A or B. The reference is fp16-only
+ * ldb % 16 == 0 and 16-byte aligned A and B; K and N may be any size. C must not overlap anything the call reads (refused). The reference is fp16-only
  * (include/cell/compute/gemm.hpp:26-29); no counterpart there. */
 int tc_gemm_i8(const void* A, const void* B, const float* scale_a, const float* scale_b, void* C, int64_t M, int64_t N,
                int64_t K, int64_t lda, int64_t ldb, int64_t ldc, int c_type, tc_stream_t stream);
@@ -119,7 +119,8 @@ int tc_gemm_i8(const void* A, const void* B, const float* scale_a, const float* 
  * offsets[experts] on are not read into any result and their rows of C stay as they were. Offsets outside
  * [0, rows] are clamped to it, a decreasing pair makes an empty expert, and either is reported through tc_device_status()
  * (code 16). 1 <= experts <= 1024; K <= 2^27; rows may be 0. Needs lda, ldb, stride_b multiples of 16 bytes and 16-byte
- * aligned A and B; N, K and ldc may be any size. C must not overlap A or B. No workspace is used and nothing is kept
+ * aligned A and B; N, K and ldc may be any size. C must not overlap anything the call reads (refused; rows that lie
+ * between those of an operand without touching them do not). No workspace is used and nothing is kept
  * between calls, so calls on several streams may overlap and a call may be captured into a graph (after a first one on
  * the device) and replayed with other offsets. One expert's products are the reference's `gemm`
  * (examples/cpp/01_gemm/02_gemm_all_mem/gemm.hpp:92-155); the grouping has no counterpart there. */
@@ -145,6 +146,7 @@ int tc_grouped_gemm_dgrad(const void* dC, const void* B, const void* offsets, in
  * [experts,N,K] (row stride lddb, expert stride stride_db): an expert without rows gets zeros. rows <= 2^27. Rows outside
  * all groups take no part, whatever they hold. A sum is formed of consecutive pieces of the group's rows, joined in order; how it is
  * cut follows from the sizes, the offsets and the device's number of SMs, so the result does not change from run to run on a device.
+ * The experts of dB may interleave ([N,E,K] seen as [E,N,K]) but not overlap.
  * Needs lddc and lda multiples of 16 bytes. The reference has no backward pass; no counterpart there. */
 int tc_grouped_gemm_wgrad(const void* dC, const void* A, const void* offsets, int offsets_are_int64, void* dB,
                           int64_t rows, int64_t experts, int64_t N, int64_t K, int64_t lddc, int64_t lda, int64_t lddb,

@@ -1,5 +1,12 @@
 """CPU tests of the argument checks of the scaled 8-bit and the expert-grouped products: every refusal is a status and a
 message before anything touches CUDA. Addresses are made up and never dereferenced."""
+import os
+import random
+import subprocess
+import sys
+from pathlib import Path
+
+import numpy as np
 import pytest
 import torch
 
@@ -174,3 +181,93 @@ def test_without_the_op_the_c_entry_point_is_called(shapes_on_a_gpu, monkeypatch
     monkeypatch.setattr(torch.Tensor, "data_ptr", lambda t: 64)
     ops.gemm_i8(*shapes_on_a_gpu)
     assert names == ["tc_gemm_i8"]
+
+
+# An operand as (address, bytes of a row, rows, bytes from row to row, slices, bytes from slice to slice), byte by byte.
+def covered(base, width, rows=1, step=0, slices=1, slice_step=0):
+    count = np.zeros(1 << 15, dtype=np.int32)
+    for e in range(slices):
+        for r in range(rows):
+            at = base + e * slice_step + r * step
+            count[at:at + width] += 1
+    return count
+
+
+def random_overlap_calls(rng):
+    """(call, whether the output meets an operand or itself): layouts in a few kilobytes, dense, with gaps and interleaved."""
+    def addr(granule, top=4096):
+        return rng.randrange(0, top, granule)
+
+    def stack(e, n, k, granule, shared=False):
+        """row and expert stride"""
+        k = -(-k // granule) * granule
+        ld = k + rng.choice([0, 0, 0, granule, 3 * granule, 10 * granule])
+        return rng.choice([(ld, n * ld), (ld, n * ld + 2 * granule), (e * ld, ld), (e * ld + 5 * granule, ld)] + [(ld, max(k, ld * n // 2 // granule * granule))] * shared)
+
+    kind = rng.choice(["quantize", "i8", "grouped", "dgrad", "wgrad"])
+    m, n, k, e = rng.randrange(1, 7), rng.randrange(1, 12), rng.randrange(1, 12), rng.randrange(1, 4)
+    if kind == "quantize":
+        x, q, s, ldx, ldq = addr(2), addr(1), addr(4), k + rng.choice([0, 0, 1, 7, 20]), k + rng.choice([0, 0, 2, 13, k + 20])
+        if rng.random() < 0.3:
+            ldq = 2 * ldx
+        parts = [covered(x, 2 * k, m, 2 * ldx), covered(q, k, m, ldq), covered(s, 4 * m)]
+        return (lambda l, b: l.tc_quantize_rows(b + x, b + q, b + s, m, k, ldx, ldq, F16, None)), (sum(p > 0 for p in parts) > 1).any()
+    a, b, off, sa, sb, c = addr(16), addr(16), addr(8), addr(4), addr(4), addr(4)
+    esz, ct = rng.choice([(4, F32), (2, F16)])
+    if kind == "i8":
+        lda, ldb, ldc = (16 * rng.randrange(1, 6) for _ in range(3))
+        ins = [covered(a, k, m, lda), covered(b, k, n, ldb), covered(sa, 4 * m), covered(sb, 4 * n)]
+        out = covered(c, n * esz, m, ldc * esz)
+        return (lambda l, p: l.tc_gemm_i8(p + a, p + b, p + sa, p + sb, p + c, m, n, k, lda, ldb, ldc, ct, None)), (sum(i > 0 for i in ins) * out > 0).any()
+    ld_in = -(-max(n, k) // 8) * 8 + rng.choice([0, 8, 40])
+    if kind == "wgrad":
+        ld, stride = stack(e, n, k, 1, True)
+        ins = [covered(a, 2 * n, m, 2 * ld_in), covered(b, 2 * k, m, 2 * ld_in), covered(off, 4 * (e + 1))]
+        out = covered(c, k * esz, n, ld * esz, e, stride * esz)
+        return (lambda l, p: l.tc_grouped_gemm_wgrad(p + a, p + b, p + off, 0, p + c, m, e, n, k, ld_in, ld_in, ld, stride, F16, ct, None),
+                (out > 1).any() or (sum(i > 0 for i in ins) * out > 0).any())
+    ld, stride = stack(e, n, k, 8, True)
+    wide = rng.randrange(2)
+    ins = [covered(b, 2 * k, n, 2 * ld, e, 2 * stride), covered(off, (8 if wide else 4) * (e + 1))]
+    ldo = rng.choice([12, 24, ld_in, 2 * ld_in, 100])
+    if kind == "grouped":
+        ins.append(covered(a, 2 * k, m, 2 * ld_in))
+        out = covered(c, n * esz, m, ldo * esz)
+        call = lambda l, p: l.tc_grouped_gemm(p + a, p + b, p + off, wide, p + c, m, e, n, k, ld_in, ld, stride, ldo, F16, ct, None)
+    else:
+        ins.append(covered(a, 2 * n, m, 2 * ld_in))
+        out = covered(c, k * esz, m, ldo * esz)
+        call = lambda l, p: l.tc_grouped_gemm_dgrad(p + a, p + b, p + off, wide, p + c, m, e, n, k, ld_in, ld, stride, ldo, F16, ct, None)
+    return call, (sum(i > 0 for i in ins) * out > 0).any()
+
+
+def check_random_overlaps():
+    """In a process that sees no GPU: a call that passes the checks ends with the failure to find one."""
+    lib, rng, seen = _lib.load(), random.Random(0), [0, 0]
+    for _ in range(4000):
+        call, meets = random_overlap_calls(rng)
+        status = call(lib, 1 << 20)
+        text = lib.tc_last_error().decode()
+        assert (status, "overlap" in text) == ((BAD, True) if meets else (-3, False)), (status, text, meets)
+        seen[int(meets)] += 1
+    assert min(seen) > 500, seen
+
+
+def test_outputs_that_overlap_an_operand_are_refused_and_others_are_not():
+    code = "import sys; sys.path[:0] = sys.argv[1:]; import test_grouped_args as t; t.check_random_overlaps()"
+    here = Path(__file__).resolve().parent
+    done = subprocess.run([sys.executable, "-c", code, str(here), str(here.parent)], env={**os.environ, "CUDA_VISIBLE_DEVICES": ""}, capture_output=True, text=True)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("call,change", [
+    (quantize, dict(x=4096, q=4096 + 63, s=64)), (quantize, dict(x=4096, q=8192, s=4096 + 60)), (quantize, dict(x=4096, q=8192, s=8192 + 28)),
+    (i8, dict(c=64 + 96)), (i8, dict(a=4096, c=4048)), (i8, dict(sa=4096 + 60)), (i8, dict(sb=4096 + 4)),
+    (grouped, dict(a=4096 + 16)), (grouped, dict(b=4096 - 1024 + 16)), (grouped, dict(off=4096 + 60)), (grouped, dict(off=4096 - 16, wide=1)),
+    (grouped_i8, dict(sb=4096 - 60)), (grouped_i8, dict(c=64 + 480)), (dgrad, dict(b=4096 + 240)), (dgrad, dict(dc=4096 - 48)),
+    (wgrad, dict(a=4096 + 1008)), (wgrad, dict(dc=4096 - 16)), (wgrad, dict(off=4096, rows=0)), (wgrad, dict(sdb=32)), (wgrad, dict(lddb=64)),
+])
+def test_partial_overlaps_are_refused(call, change):
+    lib = _lib.load()
+    assert call(lib, **change) == BAD
+    assert "overlap" in lib.tc_last_error().decode()

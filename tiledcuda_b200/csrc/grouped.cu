@@ -4,6 +4,7 @@
 #include "sm100.cuh"
 
 #include <algorithm>
+#include <initializer_list>
 
 namespace tcb {
 
@@ -30,10 +31,13 @@ static int check_terms(const char* op, const char* name, int64_t terms) {
     return TC_OK;
 }
 
-static int check_distinct(const char* op, const char* out_name, const void* out, const void* in0, const void* in1) {
-    TCB_REQUIRE(out != in0 && out != in1, "%s: %s must not overlap an operand", op, out_name);
+// The output against everything that a call reads. What is read twice (experts in one place, A within B) may overlap.
+static int check_distinct(const char* op, const char* out_name, const Extent& out, std::initializer_list<Extent> inputs) {
+    for (const Extent& in : inputs) TCB_REQUIRE(!extents_meet(out, in), "%s: %s must not overlap an operand", op, out_name);
     return TC_OK;
 }
+
+static Extent offsets_of(const void* ptr, int64_t experts, int wide) { return extent_of_vector(ptr, experts + 1, wide ? 8 : 4); }
 
 static int check_input(const char* op, const char* name, const void* ptr, int64_t ld, int64_t cols, int es) {
     TCB_REQUIRE(ptr != nullptr, "%s: null pointer argument (%s)", op, name);
@@ -203,7 +207,8 @@ extern "C" int tc_gemm_i8(const void* A, const void* B, const float* scale_a, co
     TCB_TRY(check_input(op, "A", A, lda, K, 1));
     TCB_TRY(check_input(op, "B", B, ldb, K, 1));
     TCB_TRY(check_output(op, "C", C, ldc, N, c_type));
-    TCB_TRY(check_distinct(op, "C", C, A, B));
+    TCB_TRY(check_distinct(op, "C", extent_of_rows(C, M, N, ldc, type_bytes(c_type)),
+                           {extent_of_rows(A, M, K, lda, 1), extent_of_rows(B, N, K, ldb, 1), extent_of_vector(scale_a, M, 4), extent_of_vector(scale_b, N, 4)}));
     return launch_grouped({B, A, scale_b, scale_a, nullptr, 0, C, M, 1, N, K, ldb, 0, lda, ldc, 0, kTypeI8, c_type, false, false}, stream);
 }
 
@@ -220,7 +225,9 @@ extern "C" int tc_grouped_gemm_i8(const void* A, const void* B, const float* sca
     TCB_TRY(check_input(op, "B", B, ldb, K, 1));
     TCB_TRY(check_stack(op, "B", stride_b, K, experts, 1));
     TCB_TRY(check_output(op, "C", C, ldc, N, c_type));
-    TCB_TRY(check_distinct(op, "C", C, A, B));
+    TCB_TRY(check_distinct(op, "C", extent_of_rows(C, rows, N, ldc, type_bytes(c_type)),
+                           {extent_of_rows(A, rows, K, lda, 1), extent_of_stack(B, experts, N, K, ldb, stride_b, 1), extent_of_vector(scale_a, rows, 4),
+                            extent_of_vector(scale_b, experts * N, 4), offsets_of(offsets, experts, offsets_are_int64)}));
     return launch_grouped({B, A, scale_b, scale_a, offsets, offsets_are_int64, C, rows, experts, N, K, ldb, stride_b, lda, ldc, 0, kTypeI8, c_type,
                            false, false}, stream);
 }
@@ -238,8 +245,9 @@ extern "C" int tc_grouped_gemm(const void* A, const void* B, const void* offsets
     TCB_TRY(check_input(op, "B", B, ldb, K, 2));
     TCB_TRY(check_stack(op, "B", stride_b, K, experts, 2));
     TCB_TRY(check_output(op, "C", C, ldc, N, c_type));
-    TCB_TRY(check_distinct(op, "C", C, A, B));
     TCB_TRY(check_terms(op, "K", K));
+    TCB_TRY(check_distinct(op, "C", extent_of_rows(C, rows, N, ldc, type_bytes(c_type)),
+                           {extent_of_rows(A, rows, K, lda, 2), extent_of_stack(B, experts, N, K, ldb, stride_b, 2), offsets_of(offsets, experts, offsets_are_int64)}));
     return launch_grouped({B, A, nullptr, nullptr, offsets, offsets_are_int64, C, rows, experts, N, K, ldb, stride_b, lda, ldc, 0, in_type, c_type,
                            false, false}, stream);
 }
@@ -257,8 +265,9 @@ extern "C" int tc_grouped_gemm_dgrad(const void* dC, const void* B, const void* 
     TCB_TRY(check_input(op, "B", B, ldb, K, 2));
     TCB_TRY(check_stack(op, "B", stride_b, K, experts, 2));
     TCB_TRY(check_output(op, "dA", dA, ldda, K, da_type));
-    TCB_TRY(check_distinct(op, "dA", dA, dC, B));
     TCB_TRY(check_terms(op, "N", N));
+    TCB_TRY(check_distinct(op, "dA", extent_of_rows(dA, rows, K, ldda, type_bytes(da_type)),
+                           {extent_of_rows(dC, rows, N, lddc, 2), extent_of_stack(B, experts, N, K, ldb, stride_b, 2), offsets_of(offsets, experts, offsets_are_int64)}));
     return launch_grouped({B, dC, nullptr, nullptr, offsets, offsets_are_int64, dA, rows, experts, K, N, ldb, stride_b, lddc, ldda, 0, in_type, da_type,
                            true, false}, stream);
 }
@@ -276,9 +285,12 @@ extern "C" int tc_grouped_gemm_wgrad(const void* dC, const void* A, const void* 
         TCB_TRY(check_input(op, "A", A, lda, K, 2));
     }
     TCB_TRY(check_output(op, "dB", dB, lddb, K, db_type));
-    TCB_TRY(check_distinct(op, "dB", dB, dC, A));
     TCB_TRY(check_terms(op, "rows", rows));
     TCB_REQUIRE(experts == 1 || stride_db >= K, "%s: expert stride of dB smaller than a row", op);
+    const Extent out = extent_of_stack(dB, experts, N, K, lddb, stride_db, type_bytes(db_type));
+    TCB_REQUIRE(!slices_meet(out), "%s: the experts of dB must not overlap each other", op);
+    TCB_TRY(check_distinct(op, "dB", out, {offsets_of(offsets, experts, offsets_are_int64)}));
+    if (rows > 0) TCB_TRY(check_distinct(op, "dB", out, {extent_of_rows(dC, rows, N, lddc, 2), extent_of_rows(A, rows, K, lda, 2)}));
     if (rows == 0) {   // nothing to sum over, and no tensors to describe to TMA
         const size_t es = static_cast<size_t>(type_bytes(db_type));
         for (int64_t e = 0; e < experts; ++e)

@@ -47,6 +47,90 @@ int current_device(const DeviceInfo** out) {
     return TC_OK;
 }
 
+// ---- overlap of operands ------------------------------------------------------------------------------------
+struct Rows {
+    Bytes base, width, step, count;
+    Bytes end() const { return base + (count - 1) * step + width; }
+};
+
+static Bytes floor_div(Bytes a, Bytes b) { return a / b - (a % b != 0 && a < 0); }   // b > 0
+
+static bool meets_block(const Rows& r, Bytes lo, Bytes hi) {
+    // the first row that ends behind lo
+    Bytes j = r.count > 1 ? floor_div(lo - r.base - r.width, r.step) + 1 : 0;
+    if (j < 0) j = 0;
+    return j < r.count && r.base + j * r.step + r.width > lo && r.base + j * r.step < hi;
+}
+
+static bool rows_meet(const Rows& a, const Rows& b) {
+    if (a.end() <= b.base || b.end() <= a.base) return false;
+    if (a.count == 1) return meets_block(b, a.base, a.base + a.width);
+    if (b.count == 1) return meets_block(a, b.base, b.base + b.width);
+    if (a.step == b.step) {
+        // row i of a meets row j of b where d - a.width < (i - j) * step < d + b.width
+        const Bytes d = b.base - a.base;
+        Bytes lo = floor_div(d - a.width, a.step) + 1, hi = -floor_div(-(d + b.width), a.step) - 1;
+        if (lo < 1 - b.count) lo = 1 - b.count;
+        if (hi > a.count - 1) hi = a.count - 1;
+        return lo <= hi;
+    }
+    const Rows& few = a.count < b.count ? a : b;
+    const Rows& many = a.count < b.count ? b : a;
+    for (Bytes j = 0; j < few.count; ++j)
+        if (meets_block(many, few.base + j * few.step, few.base + j * few.step + few.width)) return true;
+    return false;
+}
+
+// One slice of an operand, or (whole) all of them as rows where they can be taken as such.
+static Rows slice_of(const Extent& e, int64_t slice, bool* whole) {
+    Rows r = {static_cast<Bytes>(reinterpret_cast<uintptr_t>(e.base)) + static_cast<Bytes>(slice) * e.slice_step, e.width, e.step, e.rows};
+    if (r.count > 1 && r.step <= r.width) r = {r.base, (r.count - 1) * r.step + r.width, 0, 1};   // no gaps
+    *whole = e.slices == 1;
+    if (e.slices > 1 && r.count == 1 && e.slice_step > 0) {
+        *whole = true;
+        r.step = e.slice_step;
+        r.count = e.slices;
+        if (r.step <= r.width) r = {r.base, (r.count - 1) * r.step + r.width, 0, 1};
+    }
+    return r;
+}
+
+bool extents_meet(const Extent& a, const Extent& b) {
+    auto end = [](const Extent& e) {
+        return static_cast<Bytes>(reinterpret_cast<uintptr_t>(e.base)) + static_cast<Bytes>(e.slices - 1) * e.slice_step +
+               static_cast<Bytes>(e.rows - 1) * e.step + e.width;
+    };
+    if (end(a) <= static_cast<Bytes>(reinterpret_cast<uintptr_t>(b.base)) || end(b) <= static_cast<Bytes>(reinterpret_cast<uintptr_t>(a.base))) return false;
+    for (int64_t i = 0; i < a.slices; ++i) {
+        bool whole_a;
+        const Rows ra = slice_of(a, i, &whole_a);
+        for (int64_t j = 0; j < b.slices; ++j) {
+            bool whole_b;
+            const Rows rb = slice_of(b, j, &whole_b);
+            if (rows_meet(ra, rb)) return true;
+            if (whole_b) break;
+        }
+        if (whole_a) break;
+    }
+    return false;
+}
+
+bool slices_meet(const Extent& a) {
+    const Bytes slice = static_cast<Bytes>(a.rows - 1) * a.step + a.width;
+    if (a.slices == 1 || a.slice_step >= slice) return false;                                            // one behind the other
+    if (a.rows == 1 || a.step >= static_cast<Bytes>(a.slices - 1) * a.slice_step + a.width) return false;   // row by row
+    Extent one = a;
+    one.slices = 1;
+    for (int64_t k = 1; k < a.slices; ++k) {
+        bool whole;
+        const Rows r0 = slice_of(one, 0, &whole);
+        Rows rk = r0;
+        rk.base += static_cast<Bytes>(k) * a.slice_step;
+        if (rows_meet(r0, rk)) return true;
+    }
+    return false;
+}
+
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);

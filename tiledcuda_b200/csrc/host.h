@@ -77,6 +77,32 @@ inline int raise_smem_limit_once(OncePerDevice& once, int device, Kernel kernel,
     return TC_OK;
 }
 
+// Memory that an operand covers: `slices` times `rows` rows of `width` bytes; `step` and `slice_step` bytes from one to the next.
+// Rows do not overlap within a slice (step >= width where there are several).
+typedef __int128 Bytes;   // a dimension of 2^31 times a stride of 2^40 is beyond 64 bits
+struct Extent {
+    const void* base;
+    Bytes width;
+    int64_t rows = 1;
+    Bytes step = 0;
+    int64_t slices = 1;
+    Bytes slice_step = 0;
+};
+inline Extent extent_of_rows(const void* ptr, int64_t rows, int64_t cols, int64_t ld, int es) {
+    return {ptr, static_cast<Bytes>(cols) * es, rows, static_cast<Bytes>(ld) * es};
+}
+inline Extent extent_of_stack(const void* ptr, int64_t slices, int64_t rows, int64_t cols, int64_t ld, int64_t stride, int es) {
+    return {ptr, static_cast<Bytes>(cols) * es, rows, static_cast<Bytes>(ld) * es, slices, static_cast<Bytes>(stride) * es};
+}
+inline Extent extent_of_vector(const void* ptr, int64_t n, int es) { return {ptr, static_cast<Bytes>(n) * es}; }
+
+// Whether any byte belongs to both. Rows that lie between each other's without touching, such as two column ranges of one buffer, do
+// not meet.
+bool extents_meet(const Extent& a, const Extent& b);
+
+// Whether any byte belongs to two slices.
+bool slices_meet(const Extent& a);
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Launch with programmatic stream serialization: if the kernel before it in the stream releases its dependents

@@ -298,7 +298,9 @@ extern "C" int tc_quantize_rows(const void* x, void* q, float* scale, int64_t ro
     TCB_REQUIRE(x && q && scale, "quantize_rows: null pointer argument");
     const int es = x_type == TC_F32 ? 4 : 2;
     TCB_REQUIRE(reinterpret_cast<uintptr_t>(x) % es == 0 && reinterpret_cast<uintptr_t>(scale) % 4 == 0, "quantize_rows: x and scale must be aligned to their types");
-    TCB_REQUIRE(q != x && scale != x && scale != q, "quantize_rows: q and scale must not overlap x or each other");
+    const Extent xs = extent_of_rows(x, rows, cols, ldx, es), qs = extent_of_rows(q, rows, cols, ldq, 1), scales = extent_of_vector(scale, rows, 4);
+    TCB_REQUIRE(!extents_meet(qs, xs) && !extents_meet(scales, xs) && !extents_meet(scales, qs),
+                "quantize_rows: q and scale must not overlap x or each other");
     const DeviceInfo* dev = nullptr;
     if (int rc = current_device(&dev)) return rc;
     auto s = static_cast<cudaStream_t>(stream);
