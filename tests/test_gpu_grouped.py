@@ -1029,3 +1029,191 @@ def test_tracers_and_profilers_see_the_calls(cuda_ops, clean_status):
     assert listed.issuperset("tiledcuda::" + name for name in names)
     a, b = other[:2]
     assert cuda_ops._direct_calls["grouped_gemm"](a, b, off, torch.empty(total, n, device=DEV)) is True
+
+
+# More than 32 tiles a pair of SMs: the ring in which a pair's tiles are worked out ahead goes round and is filled again.
+MANY = [4000, 129, 0, 255, 257, 16, 5111, 1, 3131]
+
+
+@pytest.mark.parametrize("dtype,out", [(F16, F16), (BF16, F32)])
+def test_many_tiles_a_pair_forward_and_dgrad(cuda_ops, clean_status, dtype, out):
+    g = gen(46)
+    n, k = 12800, 24
+    total = sum(MANY) + 3
+    few = halves(g, (64, k), dtype)     # few distinct rows, so that the 64-bit products are quick: r and r + 64 are the same
+    a = few.repeat(-(-total // 64), 1)[:total]
+    b = halves(g, (len(MANY), n, k), dtype)
+    off, mask = offsets_of(MANY, 2), inside(total, MANY, 2)
+    for call, w in ((cuda_ops.grouped_gemm, b), (cuda_ops.grouped_gemm_dgrad, b.transpose(1, 2).contiguous())):
+        c = torch.full((total, n), -7.0, dtype=out, device=DEV)
+        call(a, w, off, c)
+        at = 2
+        for e, size in enumerate(MANY):
+            exact = few.double() @ b[e].double().t()
+            s = few.double().abs() @ b[e].double().abs().t()
+            for i in range(at, at + size, 64):
+                rows = torch.arange(i, min(i + 64, at + size), device=DEV)
+                assert_within(c[rows], exact[rows % 64], product_error(s[rows % 64], k))
+            at += size
+        assert (c[~mask] == -7.0).all()
+
+
+@pytest.mark.parametrize("out", [F16, F32])
+def test_many_tiles_a_pair_i8(cuda_ops, clean_status, out):
+    g = gen(47)
+    m, n, k = 12900, 12800, 48
+    few, b = ints(g, (64, k)), ints(g, (n, k))
+    a = few.repeat(-(-m // 64), 1)[:m]
+    sa = (torch.rand(m, generator=g, device=DEV) + 0.5) * 0.01
+    sb = (torch.rand(n, generator=g, device=DEV) + 0.5) * 0.01
+    c = torch.full((m, n), math.nan, dtype=out, device=DEV)
+    cuda_ops.gemm_i8(a, b, sa, sb, c)
+    sums = few.double() @ b.double().t() * sb.double()
+    for i in range(0, m, 640):
+        rows = torch.arange(i, min(i + 640, m), device=DEV)
+        exact = sums[rows % 64] * sa[rows].double()[:, None]
+        assert_within(c[rows], exact, exact.abs() * 3.01 * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("experts,n,k", [(128, 1288, 1288), (150, 1032, 1290)])
+@pytest.mark.parametrize("dtype,out", [(F16, F32), (BF16, BF16)])
+def test_many_tiles_a_pair_wgrad(cuda_ops, clean_status, experts, n, k, dtype, out):
+    g = gen(48)
+    sizes = [(7 * e) % 41 for e in range(experts)]
+    total = sum(sizes) + 4
+    dc, a = halves(g, (total, n), dtype), halves(g, (total, k), dtype)
+    dc[:1], a[-3:] = math.nan, math.inf
+    db = torch.full((experts, n, k), math.nan, dtype=out, device=DEV)
+    cuda_ops.grouped_gemm_wgrad(dc, a, offsets_of(sizes, 1), db)
+    at = 1
+    for e, size in enumerate(sizes):
+        x, y = dc[at:at + size].double(), a[at:at + size].double()
+        assert_within(db[e], x.t() @ y, product_error(x.abs().t() @ y.abs(), size))
+        at += size
+
+
+@pytest.mark.parametrize("out", [F16, BF16, F32])
+@pytest.mark.parametrize("m,n,k", [(2500, 3000, 1040), (2500, 2999, 777), (4200, 2100, 2300)])
+def test_gemm_i8_in_pairs_over_several_stages(cuda_ops, clean_status, m, n, k, out):
+    g = gen(49)
+    a, b = ints(g, (m, k)), ints(g, (n, k))
+    sa = (torch.rand(m, generator=g, device=DEV) + 0.5) * 0.01
+    sb = (torch.rand(n, generator=g, device=DEV) + 0.5) * 0.01
+    c = torch.full((m, n), math.nan, dtype=out, device=DEV)
+    cuda_ops.gemm_i8(a, b, sa, sb, c)
+    exact = i8_exact(a, b, sa, sb)
+    assert_within(c, exact, exact.abs() * 3.01 * 2.0 ** -24)
+
+
+# Out of range, decreasing, and groups that own the same rows, more of them than the grid has tiles for (which is made for groups
+# that do not overlap): a row is then one of its groups' product or stays as it was, and nothing is written outside of the tensors.
+@pytest.mark.parametrize("raw", [[-5, 700, 300, 1500, 5000], [0, 1 << 40, 7, 7, -(1 << 40)], [0, 2000, 0, 2000, 0], [0, 2000, 1, 1999, 0],
+                                 [2 ** 31 - 1, -2 ** 31, 0, 2000, 3]])
+@pytest.mark.parametrize("total,n,k", [(2000, 2056, 136), (2000, 136, 72)])
+def test_bad_offsets_in_both_kernels(cuda_ops, raw, total, n, k):
+    from tiledcuda_b200 import _lib
+
+    g = gen(50)
+    clamped = [min(max(x, 0), total) for x in raw]
+    ranges = [(lo, max(lo, hi)) for lo, hi in zip(clamped, clamped[1:])]
+    off = torch.tensor(raw, dtype=torch.int64, device=DEV)
+    a, b = halves(g, (total, k), F16), halves(g, (4, n, k), F16)
+
+    def guarded(rows, cols):
+        store = torch.full((rows + 2, cols + 16), -7.0, device=DEV)
+        return store, store[1:-1, 8:-8]
+
+    def check_rows(store, c):
+        own = torch.zeros(total, dtype=torch.long, device=DEV)
+        for lo, hi in ranges:
+            own[lo:hi] += 1
+        assert (c[own == 0] == -7.0).all()
+        fits = torch.zeros(c.shape, dtype=torch.bool, device=DEV)
+        for e, (lo, hi) in enumerate(ranges):
+            exact = a[lo:hi].double() @ b[e].double().t()
+            s = a[lo:hi].double().abs() @ b[e].double().abs().t()
+            bound = product_error(s, k) + half_step(exact.abs() + product_error(s, k), F32)
+            fits[lo:hi] |= (c[lo:hi].double() - exact).abs() <= bound
+        if (own > 1).any():
+            fits |= c == -7.0
+        assert fits[own > 0].all()
+        c.fill_(-7.0)
+        assert (store == -7.0).all()
+
+    assert _lib.device_status() == 0
+    store, c = guarded(total, n)
+    cuda_ops.grouped_gemm(a, b, off, c)
+    assert _lib.device_status() == 16
+    check_rows(store, c)
+    cuda_ops.grouped_gemm_dgrad(a, b.transpose(1, 2).contiguous(), off, c)
+    assert _lib.device_status() == 16
+    check_rows(store, c)
+    q, qb, one = ints(g, (total, k)), ints(g, (4, n, k)), torch.ones(4, n, device=DEV)
+    cuda_ops.grouped_gemm_i8(q, qb, torch.ones(total, device=DEV), one, off, c)
+    assert _lib.device_status() == 16
+    overlap = sum(hi - lo for lo, hi in ranges) > sum(1 for t in range(total) if any(lo <= t < hi for lo, hi in ranges))
+    right, inside_any = torch.zeros(c.shape, dtype=torch.bool, device=DEV), torch.zeros(total, dtype=torch.bool, device=DEV)
+    for e, (lo, hi) in enumerate(ranges):
+        right[lo:hi] |= c[lo:hi] == (q[lo:hi].double() @ qb[e].double().t()).float()
+        inside_any[lo:hi] = True
+    assert (right | (c == -7.0) if overlap else right)[inside_any].all() and (c[~inside_any] == -7.0).all()
+    c.fill_(-7.0)
+    assert (store == -7.0).all()
+    n2, k2 = (1300, 1300) if n > 2000 else (n, k)
+    x, y = halves(g, (total, n2), F16), halves(g, (total, k2), F16)
+    stores = torch.full((4, n2 + 2, k2 + 16), -7.0, device=DEV)
+    db = stores[:, 1:-1, 8:-8]
+    cuda_ops.grouped_gemm_wgrad(x, y, off, db)
+    assert _lib.device_status() == 16
+    for e, (lo, hi) in enumerate(ranges):
+        xe, ye = x[lo:hi].double(), y[lo:hi].double()
+        assert_within(db[e], xe.t() @ ye, product_error(xe.abs().t() @ ye.abs(), hi - lo))
+    db.fill_(-7.0)
+    assert (stores == -7.0).all()
+
+
+def test_calls_from_several_host_threads(cuda_ops, clean_status):
+    """Each thread on a stream of its own, through the same entry points at once (the calls give up the interpreter lock)."""
+    import threading
+
+    g = gen(51)
+    sizes, n, k = [700, 650, 0, 1100, 33], 2056, 136
+    total, off = sum(sizes), offsets_of(sizes)
+    jobs = []
+    for i in range(4):
+        a, b, dc = halves(g, (total, k), F16), halves(g, (5, n, k), F16), halves(g, (total, n), F16)
+        jobs.append([a, b, dc, torch.empty(total, n, device=DEV), torch.empty(total, k, device=DEV), torch.empty(5, n, k, device=DEV),
+                     torch.empty(total, k, dtype=torch.int8, device=DEV), torch.empty(total, device=DEV)])
+    torch.cuda.synchronize()
+    errors = []
+
+    def work(job):
+        try:
+            a, b, dc, c, da, db, q, s = job
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(30):
+                    cuda_ops.quantize_rows(a, q, s)
+                    cuda_ops.grouped_gemm(a, b, off, c)
+                    cuda_ops.grouped_gemm_dgrad(dc, b, off, da)
+                    cuda_ops.grouped_gemm_wgrad(dc, a, off, db)
+                    with pytest.raises(ValueError, match="offsets"):
+                        cuda_ops.grouped_gemm(a, b, off[:2], c)
+        except BaseException as error:
+            errors.append(error)
+
+    threads = [threading.Thread(target=work, args=(job,)) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    torch.cuda.synchronize()
+    for a, b, dc, c, da, db, q, s in jobs:
+        want_q, want_s = quantized(a)
+        assert torch.equal(q, want_q) and torch.equal(s, want_s)
+        exact, m = plain_forward(a, b, sizes, 0)
+        assert_within(c, exact, product_error(m, k))
+        exact, m = plain_forward(dc, b.transpose(1, 2), sizes, 0)
+        assert_within(da, exact, product_error(m, n))
+        exact, m = plain_wgrad(dc, a, sizes, 0)
+        assert_within(db, exact, product_error(m, max(sizes)))
