@@ -118,9 +118,10 @@ int tc_gemm_i8(const void* A, const void* B, const float* scale_a, const float* 
  * decided by a router on the device need no synchronisation. Empty experts are fine; rows before offsets[0] and from
  * offsets[experts] on are not read into any result and their rows of C stay as they were. Offsets outside
  * [0, rows] are clamped to it, a decreasing pair makes an empty expert, and either is reported through tc_device_status()
- * (code 16); where experts come to own the same rows by it, a row of C is one of their products or stays as it was. 1 <= experts <= 1024; K <= 2^27; rows may be 0. Needs lda, ldb, stride_b multiples of 16 bytes and 16-byte
+ * (code 16); where experts come to own the same rows by it, a row of C is one of their products or stays as it was.
+ * 1 <= experts <= 1024; K <= 2^27; rows may be 0. Needs lda, ldb, stride_b multiples of 16 bytes and 16-byte
  * aligned A and B; N, K and ldc may be any size. C must not overlap anything the call reads (refused; rows that lie
- * between those of an operand without touching them do not). No workspace is used and nothing is kept
+ * between those of an operand without touching them are fine). No workspace is used and nothing is kept
  * between calls, so calls on several streams may overlap and a call may be captured into a graph (after a first one on
  * the device) and replayed with other offsets. One expert's products are the reference's `gemm`
  * (examples/cpp/01_gemm/02_gemm_all_mem/gemm.hpp:92-155); the grouping has no counterpart there. */

@@ -1040,8 +1040,8 @@ def test_many_tiles_a_pair_forward_and_dgrad(cuda_ops, clean_status, dtype, out)
     g = gen(46)
     n, k = 12800, 24
     total = sum(MANY) + 3
-    few = halves(g, (64, k), dtype)     # few distinct rows, so that the 64-bit products are quick: r and r + 64 are the same
-    a = few.repeat(-(-total // 64), 1)[:total]
+    few = halves(g, (61, k), dtype)     # few distinct rows, so that the 64-bit products are quick: r and r + 61 are the same
+    a = few.repeat(-(-total // 61), 1)[:total]
     b = halves(g, (len(MANY), n, k), dtype)
     off, mask = offsets_of(MANY, 2), inside(total, MANY, 2)
     for call, w in ((cuda_ops.grouped_gemm, b), (cuda_ops.grouped_gemm_dgrad, b.transpose(1, 2).contiguous())):
@@ -1051,9 +1051,9 @@ def test_many_tiles_a_pair_forward_and_dgrad(cuda_ops, clean_status, dtype, out)
         for e, size in enumerate(MANY):
             exact = few.double() @ b[e].double().t()
             s = few.double().abs() @ b[e].double().abs().t()
-            for i in range(at, at + size, 64):
-                rows = torch.arange(i, min(i + 64, at + size), device=DEV)
-                assert_within(c[rows], exact[rows % 64], product_error(s[rows % 64], k))
+            for i in range(at, at + size, 610):
+                rows = torch.arange(i, min(i + 610, at + size), device=DEV)
+                assert_within(c[rows], exact[rows % 61], product_error(s[rows % 61], k))
             at += size
         assert (c[~mask] == -7.0).all()
 
@@ -1062,8 +1062,8 @@ def test_many_tiles_a_pair_forward_and_dgrad(cuda_ops, clean_status, dtype, out)
 def test_many_tiles_a_pair_i8(cuda_ops, clean_status, out):
     g = gen(47)
     m, n, k = 12900, 12800, 48
-    few, b = ints(g, (64, k)), ints(g, (n, k))
-    a = few.repeat(-(-m // 64), 1)[:m]
+    few, b = ints(g, (61, k)), ints(g, (n, k))
+    a = few.repeat(-(-m // 61), 1)[:m]
     sa = (torch.rand(m, generator=g, device=DEV) + 0.5) * 0.01
     sb = (torch.rand(n, generator=g, device=DEV) + 0.5) * 0.01
     c = torch.full((m, n), math.nan, dtype=out, device=DEV)
@@ -1071,7 +1071,7 @@ def test_many_tiles_a_pair_i8(cuda_ops, clean_status, out):
     sums = few.double() @ b.double().t() * sb.double()
     for i in range(0, m, 640):
         rows = torch.arange(i, min(i + 640, m), device=DEV)
-        exact = sums[rows % 64] * sa[rows].double()[:, None]
+        exact = sums[rows % 61] * sa[rows].double()[:, None]
         assert_within(c[rows], exact, exact.abs() * 3.01 * 2.0 ** -24)
 
 

@@ -2,7 +2,8 @@
 // host longer than the device, and of the 4.7 us that a call through torch.ops costs, 2 are argument parsing and dispatch.
 // Each function returns True if it made the call. It returns False, and has done nothing, for arguments that are not plain
 // tensors or parameters, where something waits for the call in the dispatcher (a dispatch or function mode, a tracer, a function
-// transform, a profiler), and where the checks refused: the caller then takes the way through the dispatcher. A CUDA call that failed is a RuntimeError: the call is not made twice.
+// transform, a profiler), and where the checks refused: the caller then takes the way through the dispatcher. A CUDA call that
+// failed is a RuntimeError: the call is not made twice.
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/PythonTorchFunctionTLS.h>

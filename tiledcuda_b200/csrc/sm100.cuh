@@ -20,7 +20,7 @@ enum DeviceStatus : uint32_t {
     kDevTimeoutMma = 2,        // MMA issuer waited too long for operands / a free accumulator
     kDevTimeoutEpilogue = 3,   // epilogue waited too long for an accumulator
     kDevTimeoutSoftmax = 4,    // softmax warps waited too long
-    kDevIndexOutOfRange = 16,  // scatter_nd met an index outside the table
+    kDevIndexOutOfRange = 16,  // an index outside the table (scatter_nd), or offsets out of range or order (grouped products)
 };
 
 constexpr uint64_t kWaitLimitNs = 2000000000ull;  // 2 s: far above any legitimate wait here

@@ -263,7 +263,8 @@ def grouped_gemm(a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor, c: tor
 
     a [T,K], rows sorted by expert; b [E,N,K]; both fp16 or both bf16; c [T,N] of the same type or fp32. offsets is a
     CUDA int32 / int64 tensor [E + 1], nondecreasing, within [0, T]; it is read on the device only. Experts may be
-    empty; rows of c outside all groups stay as they were. Row strides of a and b must be multiples of 16 bytes.
+    empty; rows of c outside all groups stay as they were. Row strides of a and b must be multiples of 16 bytes. Like the other
+    operators here it is not recorded by autograd; its gradients are grouped_gemm_dgrad and grouped_gemm_wgrad.
     """
     refused = _through_op("grouped_gemm", a, b, offsets, c)
     if refused is _DONE:
