@@ -106,6 +106,13 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 // of this one is over (programmatic launch), and what it waits for may need that kernel's results: the clock of the limit
 // starts when that kernel has ended, however long it takes.
 //
+// A role that gives up stays a millisecond longer: nobody follows the copies and MMAs that may still be under way into and out of
+// the CTA's shared memory and TMEM then, and they take microseconds; the CTA lets go of both when all roles have left.
+__device__ __forceinline__ bool wait_gave_up() {
+    __nanosleep(1000000);
+    return false;
+}
+
 // mbar_wait: one thread. Returns false when another role has aborted or when the limit ran out (then it
 // records `code` in the CTA's abort word).
 static __device__ __noinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_word,
@@ -114,14 +121,14 @@ static __device__ __noinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parit
     uint64_t t0 = 0;
     while (!mbar_try_wait(bar, parity)) {
         if ((++it & 0xfffu) == 0) {
-            if (*abort_word != 0) return false;
+            if (*abort_word != 0) return wait_gave_up();
             if (t0 == 0) grid_dependency_wait();
             const uint64_t now = global_timer_ns();
             if (t0 == 0) {
                 t0 = now;
             } else if (now - t0 > kWaitLimitNs) {
                 *abort_word = code;
-                return false;
+                return wait_gave_up();
             }
         }
     }
@@ -164,7 +171,11 @@ static __device__ __noinline__ bool mbar_wait_warp_slow(uint64_t* bar, uint32_t 
                     give_up = 1;
                 }
             }
-            if (__any_sync(0xffffffffu, give_up)) return false;
+            if (__any_sync(0xffffffffu, give_up)) {
+                wait_gave_up();
+                __syncwarp();
+                return false;
+            }
         }
     }
     return true;
