@@ -194,7 +194,6 @@ grouped_split_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
         tma_prefetch_desc(&tmap_p);
         tma_prefetch_desc(&tmap_q);
     }
-    grid_launch_dependents();
     // Without offsets the tile follows from the sizes, and the set-up is over before the kernel in front is (0.8 us of a
     // call of 4 to 6).
     const bool dense = a.offsets == nullptr;
@@ -204,6 +203,9 @@ grouped_split_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
+    // The next kernel may come once TMEM is allocated, not before: where it shares an SM, it could take columns that a CTA of this
+    // one still has to get, and would then wait for this kernel with them.
+    grid_launch_dependents();
     grid_dependency_wait();   // the offsets may come from the kernel before this one
     if (!dense) {
         if (warp == 0) find_tile<kRaggedX>(a, row_tile, col0, shared_tile, blockIdx.x == 0);
